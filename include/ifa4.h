@@ -322,6 +322,111 @@ int32_t ifa4_decode_quant_fwd(const ifa4_args* args, const ifa4_paged_kv* kv,
 #define IFA4_DECODE_SCRATCH_BYTES (32u << 20)
 int32_t ifa4_decode_fwd_noalloc(const ifa4_args* args, void* stream);
 
+/*
+ * RMS norm of every query and key head with the position rotation in the same
+ * pass, the step before the attention (the norms of outputs/architecture.md:24-50;
+ * the reference has no kernel for it).  Per head row x at position p:
+ *   z = x * (mean(x^2) + eps)^-1/2 * weight       (weight NULL: z = x)
+ *   y = z with the rot_dim leading elements turned by the angles of position p
+ * half-split (interleaved = 0): element i < rot_dim / 2 turns with i + rot_dim / 2,
+ * interleaved: element 2i with 2i + 1; pair (a, b) with angle i becomes
+ *   (a cos[p, i] - b sin[p, i],  b cos[p, i] + a sin[p, i]).
+ * fp32 throughout, one rounding to `dtype` at the end.
+ * Layouts (element strides, last dim contiguous): q, q_out [total, n_heads,
+ * head_dim], k, k_out [total, kv_heads, head_dim] in dtype (rows 16-byte aligned,
+ * strides multiples of 8); weights [head_dim] in w_dtype; cos, sin
+ * [max_position, rot_dim / 2] fp32 (rows 16-byte aligned, angle_stride elements
+ * apart); positions int32 [total], read on the device: one outside
+ * [0, max_position) takes the nearest row of the table (results unspecified).
+ * rot_dim 0: no rotation, cos, sin and positions are not read.
+ */
+typedef struct ifa4_norm_rope {
+  uint32_t struct_size;    /* sizeof(ifa4_norm_rope) */
+  int32_t dtype;           /* IFA4_BF16 or IFA4_FP16 */
+  int32_t w_dtype;         /* IFA4_BF16, IFA4_FP16 or IFA4_FP32 */
+  int32_t head_dim;        /* 64 or 128 */
+  int32_t n_heads;
+  int32_t kv_heads;
+  int32_t rot_dim;         /* a multiple of 16, 0 .. head_dim */
+  int32_t interleaved;     /* 0 or 1 */
+  int32_t max_position;    /* rows of cos and sin */
+  float eps;               /* >= 0 */
+  int64_t total;           /* tokens */
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  int64_t q_stride_t, q_stride_h, k_stride_t, k_stride_h;
+  int64_t q_out_stride_t, q_out_stride_h, k_out_stride_t, k_out_stride_h;
+  const void* q_weight;    /* NULL: q is not normed */
+  const void* k_weight;
+  const float* cos;
+  const float* sin;
+  int64_t angle_stride;
+  const int32_t* positions;
+} ifa4_norm_rope;
+
+int32_t ifa4_qk_norm_rope_fwd(const ifa4_norm_rope* args, void* stream);
+
+/*
+ * Its backward pass.  gq, gk: gradients of q_out and k_out (NULL: that output has
+ * none; its dq / dk and weight gradient are then not written); dq, dk: gradients
+ * of q and k, in dtype; dq_weight, dk_weight [head_dim] in w_dtype (NULL exactly
+ * where the weight is NULL or its output has no gradient).  Reads q, k, the weights,
+ * the table and the positions of args again, not q_out / k_out.  The weight
+ * gradients are summed in fp32 in a fixed order through the workspace
+ * (ifa4_qk_norm_rope_bwd_workspace_bytes, 256-byte aligned, scratch for one call; 0
+ * bytes without weights).
+ */
+typedef struct ifa4_norm_rope_grad {
+  uint32_t struct_size;    /* sizeof(ifa4_norm_rope_grad) */
+  const void* gq;
+  const void* gk;
+  void* dq;
+  void* dk;
+  int64_t gq_stride_t, gq_stride_h, gk_stride_t, gk_stride_h;
+  int64_t dq_stride_t, dq_stride_h, dk_stride_t, dk_stride_h;
+  void* dq_weight;
+  void* dk_weight;
+} ifa4_norm_rope_grad;
+
+size_t ifa4_qk_norm_rope_bwd_workspace_bytes(const ifa4_norm_rope* args);
+int32_t ifa4_qk_norm_rope_bwd(const ifa4_norm_rope* args, const ifa4_norm_rope_grad* grad,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Append new keys and values to a paged cache, normed and turned on the way (the
+ * cache write of the serving backend, outputs/architecture.md:117-127; the reference
+ * has no kernel for it).  args describes the new tokens' k and, where n_heads > 0,
+ * their q (q_out written; n_heads 0: none; k_out and positions are not read).  Token
+ * i of the n = cu_seqlens[b+1] - cu_seqlens[b] new tokens of sequence b has position
+ *   p = seqused_k[b] - n + i
+ * (kv->seqused_k counts the new keys: it is what the attention call after this one
+ * takes); its k, normed and turned by position p, and its v go to row p % block_size of
+ * block kv->block_table[b, p / block_size], in the type kv_dtype: args.dtype, or
+ * IFA4_FP8_E4M3, which stores the e4m3 value nearest to k * (1 / k_scale) (ties to
+ * even, magnitudes past 448 as 448).  Tokens of no sequence, with p < 0 or past the
+ * table, or whose table entry lies outside the pool are not written (q_out of a token of
+ * no sequence neither).  Two tokens sent to one row leave one of them.
+ * Cache strides are in cache elements, multiples of 16 bytes, as for decode.
+ */
+typedef struct ifa4_kv_append {
+  uint32_t struct_size;    /* sizeof(ifa4_kv_append) */
+  int32_t kv_dtype;
+  const void* v;           /* [total, kv_heads, head_dim] in args.dtype */
+  int64_t v_stride_t, v_stride_h;
+  void* k_cache;
+  void* v_cache;
+  int64_t k_cache_stride_t, k_cache_stride_h, v_cache_stride_t, v_cache_stride_h;
+  const int32_t* cu_seqlens;  /* device int32 [batch + 1]: the new tokens */
+  int32_t batch;
+  float k_scale;           /* > 0, finite; read for an e4m3 cache only */
+  float v_scale;
+} ifa4_kv_append;
+
+int32_t ifa4_kv_append_paged(const ifa4_norm_rope* args, const ifa4_kv_append* append,
+                             const ifa4_paged_kv* kv, void* stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif

@@ -2,7 +2,7 @@
 
 Outputs (next to the Python package, git-ignored, shipped with the tree):
   inkling_fa4/libifa4.so        HIP kernels + C ABI (include/ifa4.h); no torch
-  inkling_fa4/_ifa4_torch.so    torch.ops.inkling_fa4.{fwd,decode} binding
+  inkling_fa4/_ifa4_torch.so    torch.ops.inkling_fa4.* binding
 
 Usage:  python inkling-fa4-relative-attention_amd/build.py [--jobs N]
 Cross-compiles for gfx950 without a GPU.
@@ -22,7 +22,9 @@ BUILD = os.path.join(HERE, "_build")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 HIPCC = os.path.join(ROCM, "bin", "hipcc")
 
-LIB_SOURCES = ["prefill_fwd.hip", "decode_fwd.hip", "decode_noalloc.hip", "ifa4_api.cpp"]
+LIB_SOURCES = ["prefill_fwd.hip", "decode_fwd.hip", "decode_noalloc.hip", "norm_rope.hip",
+               "ifa4_api.cpp", "norm_rope_api.cpp"]
+EXT_SOURCES = ["torch_ext.cpp", "torch_norm_rope.cpp"]
 LIB_NAME = "libifa4.so"
 EXT_NAME = "_ifa4_torch.so"
 
@@ -69,7 +71,7 @@ def build_library(jobs, out_dir=PKG, defines=(), build_dir=BUILD, csrc=CSRC, inc
     return out
 
 
-def build_torch_binding():
+def build_torch_binding(jobs=4):
     import torch
     from torch.utils import cpp_extension
 
@@ -78,11 +80,15 @@ def build_torch_binding():
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     out = os.path.join(PKG, EXT_NAME)
     tmp = out + ".tmp"
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared",
-           os.path.join(CSRC, "torch_ext.cpp"), "-o", tmp,
-           f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-           f"-I{INCLUDE}", f"-I{ROCM}/include"]
-    cmd += [f"-I{p}" for p in inc]
+    os.makedirs(BUILD, exist_ok=True)
+    flags = ["-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+             "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f"-I{INCLUDE}", f"-I{CSRC}",
+             f"-I{ROCM}/include"] + [f"-I{p}" for p in inc]
+    objs = [os.path.join(BUILD, os.path.splitext(src)[0] + ".o") for src in EXT_SOURCES]
+    with ThreadPoolExecutor(max_workers=jobs) as ex:
+        list(ex.map(_run, [["g++"] + flags + ["-c", os.path.join(CSRC, src), "-o", obj]
+                           for src, obj in zip(EXT_SOURCES, objs)]))
+    cmd = ["g++", "-shared", "-fPIC"] + objs + ["-o", tmp]
     cmd += [f"-L{p}" for p in libdirs] + [f"-L{PKG}", f"-L{ROCM}/lib"]
     cmd += ["-lifa4", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch", "-lamdhip64",
             "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{ROCM}/lib"]
@@ -93,7 +99,7 @@ def build_torch_binding():
 
 def build(jobs=4):
     lib = build_library(jobs)
-    ext = build_torch_binding()
+    ext = build_torch_binding(jobs)
     return lib, ext
 
 
@@ -105,7 +111,7 @@ def main():
     lib = build_library(args.jobs)
     print("built", os.path.relpath(lib, REPO))
     if not args.lib_only:
-        ext = build_torch_binding()
+        ext = build_torch_binding(args.jobs)
         print("built", os.path.relpath(ext, REPO))
     return 0
 

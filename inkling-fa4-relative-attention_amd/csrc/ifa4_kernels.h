@@ -102,6 +102,63 @@ struct DecodeParams {
   int32_t max_blocks;  // table entries per sequence
 };
 
+// Head norm and rotation (norm_rope.hip).  q and k rows in, q_out and k_out rows out.
+struct NormRopeParams {
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  int64_t q_st, q_sh, k_st, k_sh, qo_st, qo_sh, ko_st, ko_sh;
+  const void* q_weight;      // [head_dim] or NULL: not normed
+  const void* k_weight;
+  const float* cos;          // [max_position, rot / 2], rows angle_stride apart
+  const float* sin;
+  const int32_t* positions;  // [total] (rot > 0; a cache append has its own)
+  int64_t angle_stride;
+  int64_t total;             // tokens
+  int32_t n_heads, kv_heads;
+  int32_t w_dtype;           // 0 bf16, 1 fp16, 2 fp32
+  int32_t rot;               // leading elements of a head that turn
+  int32_t pairs;             // 1: neighbours turn together, 0: elements rot / 2 apart
+  int32_t max_position;
+  int32_t heads_per;         // heads of a token that one lane group walks over (set by the launch)
+  float eps;
+};
+
+// Where the keys and values of new tokens go (paged cache, as in DecodeParams).
+struct AppendParams {
+  const void* v;
+  void* k_cache;
+  void* v_cache;
+  const int32_t* cu;         // [batch + 1] new tokens of each sequence
+  const int32_t* seqused_k;  // keys of each sequence, the new ones included
+  const int32_t* block_table;
+  int64_t v_st, v_sh, kc_st, kc_sh, kc_sblk, vc_st, vc_sh, vc_sblk, bt_stride;
+  int32_t batch, block_shift, num_blocks, max_blocks;
+  float inv_k_scale, inv_v_scale;
+};
+
+// Gradients of the norm and rotation; gq or gk NULL: that output has none.
+struct NormRopeGrad {
+  const void* gq;
+  const void* gk;
+  void* dq;
+  void* dk;
+  int64_t gq_st, gq_sh, gk_st, gk_sh, dq_st, dq_sh, dk_st, dk_sh;
+  void* dq_weight;
+  void* dk_weight;
+  float* partial;  // [norm_rope_bwd_rows][2][head_dim], or NULL without weights
+};
+
+// Workgroups of the backward pass at most, each with a row of partial weight gradients.
+constexpr int64_t kNormRopeBwdBlocks = 1024;
+int64_t norm_rope_bwd_rows(int64_t total, int head_dim);
+// cache: 0 none, 1 of the inputs' type, 2 e4m3
+hipError_t launch_norm_rope(const NormRopeParams& p, const AppendParams& a, int cache, int head_dim,
+                            int dtype, hipStream_t stream);
+hipError_t launch_norm_rope_bwd(const NormRopeParams& p, const NormRopeGrad& g, int head_dim,
+                                int dtype, hipStream_t stream);
+
 int prefill_block_q();
 int prefill_proj_block_q();  // query rows per workgroup of the fused-projection kernel
 int prefill_block_k();

@@ -1,0 +1,514 @@
+// RMS norm of query and key heads with the position rotation in the same pass
+// (forward, backward), and the same on the way into a paged KV cache, for gfx950.
+//
+// Mathematics, per head row x of D elements at position p:
+//   r = 1 / sqrt(mean(x^2) + eps),  z = x r w                      (w NULL: z = x)
+//   y_e = z_e c_e + z_e' s_e   for the rot leading elements, e' the partner of e:
+//     half-split   e' = e +- rot / 2,  angle index e mod (rot / 2)
+//     interleaved  e' = e ^ 1,         angle index e / 2
+//   c = cos[p], s = -sin[p] for the first of a pair and +sin[p] for the second;
+//   elements from rot on: y = z.
+// Written y = r (x A + x' B) with A = w c, B = w' s: A and B depend on the token and
+// on q or k alone, so a token's heads share them.
+// Backward, with g the gradient of y: the rotation's transpose is the rotation by -p, so
+//   gz_e = g_e c_e - g_e' s_e;   dw = sum over rows of gz x r;
+//   dx = r gz w - x (r^3 / D) sum_e(gz_e w_e x_e).
+// r is computed again from x, which the backward pass reads anyway: nothing but the
+// inputs is kept between the passes.  All of it is in fp32 with one rounding at the end.
+//
+// Layout.  A row is held by D / 8 neighbouring lanes, 16 bytes each; such a lane group
+// takes a token and walks over a chunk of its heads (q heads, then k heads, then for
+// the cache v heads), two rows' loads in flight at a time, with the token's A and B in
+// registers.  Row sums meet by DPP adds, partners by lane exchange of the packed 16-bit
+// row (half-split) or inside the lane (interleaved).
+#include <type_traits>
+
+#include "ifa4_device.hpp"
+#include "ifa4_kernels.h"
+
+namespace ifa4 {
+namespace {
+
+constexpr int kThreads = 256;
+
+template <int D>
+struct RowShape {
+  static constexpr int kLpr = D / 8;            // lanes per row
+  static constexpr int kPerWave = 64 / kLpr;    // rows side by side in a wave
+  static constexpr int kPerBlock = kThreads / kLpr;
+};
+
+template <int kCtrl>
+__device__ __forceinline__ float dpp(float x) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), kCtrl, 0xf, 0xf, false));
+}
+// Sum over the lanes of a row (16 or 8), in every lane.
+template <int kLpr>
+__device__ __forceinline__ float row_sum(float x) {
+  if constexpr (kLpr == 16) {
+    x += dpp<0x128>(x);  // row_ror 8, 4, 2, 1
+    x += dpp<0x124>(x);
+    x += dpp<0x122>(x);
+    x += dpp<0x121>(x);
+  } else {
+    x += dpp<0xb1>(x);   // lane ^ 1, lane ^ 2, then the other quad of the eight
+    x += dpp<0x4e>(x);
+    x += dpp<0x141>(x);
+  }
+  return x;
+}
+
+template <typename Tag>
+__device__ __forceinline__ void unpack8(u32x4_t w, float* f) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = Elem<Tag>::lo(w[i]);
+    f[2 * i + 1] = Elem<Tag>::hi(w[i]);
+  }
+}
+template <typename Tag>
+__device__ __forceinline__ u32x4_t pack8(const float* f) {
+  return u32x4_t{Elem<Tag>::pack2(f[0], f[1]), Elem<Tag>::pack2(f[2], f[3]),
+                 Elem<Tag>::pack2(f[4], f[5]), Elem<Tag>::pack2(f[6], f[7])};
+}
+
+// Element i of a norm weight (dtype: ifa4_dtype) as fp32; 1 without a weight.
+__device__ __forceinline__ float weight_at(const void* w, int dtype, int i) {
+  if (w == nullptr) return 1.f;
+  if (dtype == 2) return static_cast<const float*>(w)[i];
+  const uint32_t b = static_cast<const uint16_t*>(w)[i];
+  return dtype == 0 ? __uint_as_float(b << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)b);
+}
+
+// Where the elements of a lane turn: the partner lane's distance (half-split) and the
+// first angle of the lane; turns: the lane lies in the rot leading elements.
+struct Turn {
+  int hop;    // half-split: partner = lane + hop
+  int angle;  // index of the lane's first cos / sin
+  bool turns, second;
+};
+template <bool kPairs>
+__device__ __forceinline__ Turn turn_of(const NormRopeParams& p, int c) {
+  Turn t;
+  const int half = p.rot / 2;
+  t.turns = 8 * c < p.rot;
+  t.second = !kPairs && 8 * c >= half;
+  t.hop = kPairs || !t.turns ? 0 : (t.second ? -(half / 8) : half / 8);
+  t.angle = kPairs ? 4 * c : 8 * c - (t.second ? half : 0);
+  return t;
+}
+
+// cos and signed sin of the lane's eight elements at position pos (1 and 0 where nothing turns).
+template <bool kPairs>
+__device__ __forceinline__ void angles(const NormRopeParams& p, const Turn& t, int pos, float* cs,
+                                       float* sn) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    cs[e] = 1.f;
+    sn[e] = 0.f;
+  }
+  if (!t.turns) return;
+  // positions outside the table read its nearest row, never past it
+  const int64_t row = (int64_t)min(max(pos, 0), p.max_position - 1) * p.angle_stride + t.angle;
+  const f32x4_t* cp = reinterpret_cast<const f32x4_t*>(p.cos + row);
+  const f32x4_t* sp = reinterpret_cast<const f32x4_t*>(p.sin + row);
+  if constexpr (kPairs) {
+    const f32x4_t a = cp[0], b = sp[0];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      cs[e] = a[e / 2];
+      sn[e] = (e & 1) ? b[e / 2] : -b[e / 2];
+    }
+  } else {
+    const f32x4_t a0 = cp[0], a1 = cp[1], b0 = sp[0], b1 = sp[1];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      cs[e] = e < 4 ? a0[e] : a1[e - 4];
+      const float b = e < 4 ? b0[e] : b1[e - 4];
+      sn[e] = t.second ? b : -b;
+    }
+  }
+}
+
+// Partners of the lane's eight elements (packed): the row of lane + hop, or the lane's own
+// with neighbours swapped; zeros where nothing turns (an infinity there times a sine of 0
+// would be NaN).
+template <bool kPairs>
+__device__ __forceinline__ u32x4_t partners(u32x4_t w, const Turn& t, int lane) {
+  u32x4_t r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t x = kPairs ? __builtin_amdgcn_alignbit(w[i], w[i], 16)
+                              : (uint32_t)__builtin_amdgcn_ds_bpermute(4 * (lane + t.hop), (int)w[i]);
+    r[i] = t.turns ? x : 0u;
+  }
+  return r;
+}
+
+// A and B of the lane's elements for one weight.
+template <bool kPairs>
+__device__ __forceinline__ void coefficients(const float* w, const float* wp, const float* cs,
+                                             const float* sn, float* a, float* b) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    a[e] = w[e] * cs[e];
+    b[e] = wp[e] * sn[e];
+  }
+}
+
+// Eight fp32 values -> OCP e4m3, nearest even; magnitudes past 448 become 448, NaN stays.
+__device__ __forceinline__ u32x2_t pack_fp8(const float* f) {
+  u32x2_t r;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float v = f[4 * h + i];
+      x[i] = v != v ? v : fminf(fmaxf(v, -448.f), 448.f);
+    }
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+    r[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], w, true);
+  }
+  return r;
+}
+
+// Last sequence b with cu[b] <= t, by the lanes of a group together (one of them probes
+// one entry a round: 16 or 8 ways); a guess that holds, as with one token a sequence,
+// skips the search.  Whatever cu holds the result lies in [0, batch).
+template <int kLpr>
+__device__ __forceinline__ int find_sequence(const int32_t* cu, int batch, int t, int lane) {
+  const int guess = min(t, batch - 1);
+  int lo = 0, hi = batch;
+  if (cu[guess] <= t && t < cu[guess + 1]) {
+    lo = guess;
+    hi = guess + 1;
+  }
+  const int c = lane % kLpr, g0 = lane - c;
+  while (wave_any(hi - lo > 1)) {
+    const int step = max((hi - lo + kLpr - 1) / kLpr, 1);
+    const int at = lo + c * step;
+    const bool below = c == 0 || (at < hi && cu[at] <= t);
+    const uint64_t m = __builtin_amdgcn_ballot_w64(below) >> g0;
+    const int n = __builtin_ctzll(~(m & ((1ull << kLpr) - 1)));  // leading probes that hold
+    const int from = lo;
+    lo = from + (n - 1) * step;
+    hi = min(hi, from + n * step);
+  }
+  return lo;
+}
+
+// Where a new token's key and value go: its position, and the block and row (row -1: nowhere);
+// covered: the token belongs to a sequence.
+struct Slot {
+  int pos, row;
+  int64_t block;
+  bool covered;
+};
+template <int kLpr>
+__device__ __forceinline__ Slot find_slot(const AppendParams& a, int t, int lane) {
+  const int b = find_sequence<kLpr>(a.cu, a.batch, t, lane);
+  const int s = a.cu[b], e = a.cu[b + 1];
+  Slot r;
+  r.pos = a.seqused_k[b] - (e - t);
+  r.row = -1;
+  r.block = 0;
+  r.covered = t >= s && t < e;
+  const int cap = a.max_blocks << a.block_shift;
+  if (r.covered && r.pos >= 0 && r.pos < cap) {
+    const int ent = a.block_table[(int64_t)b * a.bt_stride + (r.pos >> a.block_shift)];
+    if ((unsigned)ent < (unsigned)a.num_blocks) {
+      r.block = ent;
+      r.row = r.pos & ((1 << a.block_shift) - 1);
+    }
+  }
+  return r;
+}
+
+// ---- forward, and the append to a paged cache -------------------------------------------------
+// kCache: 0 none (q and k come back), 1 cache of the inputs' type, 2 e4m3 cache.
+template <int D, typename Tag, bool kPairs, int kCache>
+__global__ __launch_bounds__(kThreads) void norm_rope_kernel(NormRopeParams p, AppendParams ap) {
+  using S = RowShape<D>;
+  constexpr int kLpr = S::kLpr;
+  const int lane = threadIdx.x & 63, c = lane % kLpr;
+  const int64_t t64 = (int64_t)blockIdx.x * S::kPerBlock + threadIdx.x / kLpr;
+  const bool in = t64 < p.total;
+  const int t = in ? (int)t64 : (int)p.total - 1;  // idle groups follow the last token, and store nothing
+  const Turn turn = turn_of<kPairs>(p, c);
+
+  Slot slot{};
+  int pos = 0;
+  if constexpr (kCache != 0) {
+    slot = find_slot<kLpr>(ap, t, lane);
+    pos = slot.pos;
+  } else if (p.positions != nullptr) {
+    pos = p.positions[t];
+  }
+  float cs[8], sn[8];
+  angles<kPairs>(p, turn, pos, cs, sn);
+  float aq[8], bq[8], ak[8], bk[8];
+  {
+    float w[8], wp[8];
+    const int cp = c + turn.hop;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      w[e] = weight_at(p.q_weight, p.w_dtype, 8 * c + e);
+      wp[e] = weight_at(p.q_weight, p.w_dtype, kPairs ? 8 * c + (e ^ 1) : 8 * cp + e);
+    }
+    coefficients<kPairs>(w, wp, cs, sn, aq, bq);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      w[e] = weight_at(p.k_weight, p.w_dtype, 8 * c + e);
+      wp[e] = weight_at(p.k_weight, p.w_dtype, kPairs ? 8 * c + (e ^ 1) : 8 * cp + e);
+    }
+    coefficients<kPairs>(w, wp, cs, sn, ak, bk);
+  }
+
+  const int hq = p.n_heads, hk = hq + p.kv_heads;
+  const int h_end = min((int)(blockIdx.y + 1) * p.heads_per, kCache != 0 ? hk + p.kv_heads : hk);
+  auto row_in = [&](int h) -> const uint16_t* {
+    const uint16_t* base = h < hq ? static_cast<const uint16_t*>(p.q) + t * p.q_st + h * p.q_sh
+                           : h < hk
+                               ? static_cast<const uint16_t*>(p.k) + t * p.k_st + (h - hq) * p.k_sh
+                               : static_cast<const uint16_t*>(ap.v) + t * ap.v_st + (h - hk) * ap.v_sh;
+    return base + 8 * c;
+  };
+  auto put = [&](int h, u32x4_t raw) {
+    const bool is_q = h < hq, is_v = kCache != 0 && h >= hk;
+    float x[8], px[8], y[8];
+    unpack8<Tag>(raw, x);
+    const u32x4_t praw = partners<kPairs>(raw, turn, lane);
+    unpack8<Tag>(praw, px);
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+    ss = row_sum<kLpr>(ss);
+    const bool norm = !is_v && (is_q ? p.q_weight : p.k_weight) != nullptr;
+    const float r = norm ? 1.f / sqrtf(ss * (1.f / D) + p.eps) : 1.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float a = is_q ? aq[e] : ak[e], b = is_q ? bq[e] : bk[e];
+      y[e] = is_v ? x[e] : r * fmaf(x[e], a, px[e] * b);
+    }
+    if (!in || (kCache != 0 && !slot.covered)) return;
+    if (kCache == 0 || is_q) {
+      uint16_t* dst = is_q ? static_cast<uint16_t*>(p.q_out) + t * p.qo_st + h * p.qo_sh
+                           : static_cast<uint16_t*>(p.k_out) + t * p.ko_st + (h - hq) * p.ko_sh;
+      *reinterpret_cast<u32x4_t*>(dst + 8 * c) = pack8<Tag>(y);
+      return;
+    }
+    if (slot.row < 0) return;
+    const int64_t at = is_v ? slot.block * ap.vc_sblk + slot.row * ap.vc_st + (h - hk) * ap.vc_sh
+                            : slot.block * ap.kc_sblk + slot.row * ap.kc_st + (h - hq) * ap.kc_sh;
+    if constexpr (kCache == 1) {
+      uint16_t* dst = static_cast<uint16_t*>(is_v ? ap.v_cache : ap.k_cache) + at;
+      *reinterpret_cast<u32x4_t*>(dst + 8 * c) = is_v ? raw : pack8<Tag>(y);
+    } else if constexpr (kCache == 2) {
+      const float mul = is_v ? ap.inv_v_scale : ap.inv_k_scale;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] *= mul;
+      uint8_t* dst = static_cast<uint8_t*>(is_v ? ap.v_cache : ap.k_cache) + at;
+      *reinterpret_cast<u32x2_t*>(dst + 8 * c) = pack_fp8(y);
+    }
+  };
+  for (int h = (int)blockIdx.y * p.heads_per; h < h_end; h += 2) {
+    const u32x4_t r0 = ld_global_16(row_in(h));
+    const bool two = h + 1 < h_end;
+    u32x4_t r1{};
+    if (two) r1 = ld_global_16(row_in(h + 1));
+    put(h, r0);
+    if (two) put(h + 1, r1);
+  }
+}
+
+// ---- backward -------------------------------------------------------------------------------
+// A workgroup walks over tokens and leaves its sums of the weight gradients in one row of the
+// workspace, [q or k][D]; the second kernel adds the rows in a fixed order.
+template <int D, typename Tag, bool kPairs>
+__global__ __launch_bounds__(kThreads) void norm_rope_bwd_kernel(NormRopeParams p, NormRopeGrad g) {
+  using S = RowShape<D>;
+  constexpr int kLpr = S::kLpr;
+  __shared__ float sums[S::kPerBlock][2][D];
+  const int lane = threadIdx.x & 63, c = lane % kLpr, grp = threadIdx.x / kLpr;
+  const Turn turn = turn_of<kPairs>(p, c);
+  float wq[8], wk[8], dwq[8], dwk[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    wq[e] = weight_at(p.q_weight, p.w_dtype, 8 * c + e);
+    wk[e] = weight_at(p.k_weight, p.w_dtype, 8 * c + e);
+    dwq[e] = dwk[e] = 0.f;
+  }
+  const int hq = p.n_heads;
+  const int h_beg = g.gq != nullptr ? 0 : hq, h_all = g.gk != nullptr ? hq + p.kv_heads : hq;
+  for (int64_t t0 = (int64_t)blockIdx.x * S::kPerBlock; t0 < p.total;
+       t0 += (int64_t)gridDim.x * S::kPerBlock) {
+    const bool in = t0 + grp < p.total;
+    const int64_t t = in ? t0 + grp : p.total - 1;
+    float cs[8], sn[8];
+    angles<kPairs>(p, turn, p.positions != nullptr ? p.positions[t] : 0, cs, sn);
+    auto load = [&](int h, u32x4_t& xr, u32x4_t& gr) {
+      const bool is_q = h < hq;
+      const int64_t k = h - hq;
+      xr = ld_global_16(is_q ? static_cast<const uint16_t*>(p.q) + t * p.q_st + h * p.q_sh + 8 * c
+                             : static_cast<const uint16_t*>(p.k) + t * p.k_st + k * p.k_sh + 8 * c);
+      gr = ld_global_16(is_q ? static_cast<const uint16_t*>(g.gq) + t * g.gq_st + h * g.gq_sh + 8 * c
+                             : static_cast<const uint16_t*>(g.gk) + t * g.gk_st + k * g.gk_sh + 8 * c);
+    };
+    auto put = [&](int h, u32x4_t xr, u32x4_t gr) {
+      const bool is_q = h < hq;
+      float x[8], gy[8], pg[8], gw[8];
+      unpack8<Tag>(xr, x);
+      unpack8<Tag>(gr, gy);
+      const u32x4_t pgr = partners<kPairs>(gr, turn, lane);
+      unpack8<Tag>(pgr, pg);
+      float ss = 0.f, dot = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        gy[e] = fmaf(gy[e], cs[e], -pg[e] * sn[e]);  // gz
+        gw[e] = gy[e] * (is_q ? wq[e] : wk[e]);
+        ss = fmaf(x[e], x[e], ss);
+        dot = fmaf(gw[e], x[e], dot);
+      }
+      ss = row_sum<kLpr>(ss);
+      dot = row_sum<kLpr>(dot);
+      if ((is_q ? p.q_weight : p.k_weight) != nullptr) {
+        const float r = 1.f / sqrtf(ss * (1.f / D) + p.eps);
+        const float f = r * r * r * (1.f / D) * dot;
+        const float keep = in ? r : 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float dw = gy[e] * x[e] * keep;
+          if (is_q)
+            dwq[e] += dw;
+          else
+            dwk[e] += dw;
+          gw[e] = fmaf(-x[e], f, r * gw[e]);
+        }
+      }
+      if (!in) return;
+      uint16_t* dst = is_q ? static_cast<uint16_t*>(g.dq) + t * g.dq_st + h * g.dq_sh
+                           : static_cast<uint16_t*>(g.dk) + t * g.dk_st + (h - hq) * g.dk_sh;
+      *reinterpret_cast<u32x4_t*>(dst + 8 * c) = pack8<Tag>(gw);
+    };
+    for (int h = h_beg; h < h_all; h += 2) {
+      u32x4_t x0, g0, x1{}, g1{};
+      load(h, x0, g0);
+      const bool two = h + 1 < h_all;
+      if (two) load(h + 1, x1, g1);
+      put(h, x0, g0);
+      if (two) put(h + 1, x1, g1);
+    }
+  }
+  if (g.partial == nullptr) return;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    sums[grp][0][8 * c + e] = dwq[e];
+    sums[grp][1][8 * c + e] = dwk[e];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * D; i += kThreads) {
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < S::kPerBlock; ++k) s += sums[k][i / D][i % D];
+    g.partial[(int64_t)blockIdx.x * 2 * D + i] = s;
+  }
+}
+
+// dw of 32 columns of [q or k][D]: 32 threads a column over the partial rows, then in LDS.
+constexpr int kSumCols = 32, kSumRows = 32;
+__global__ __launch_bounds__(kSumCols * kSumRows) void norm_rope_dw_kernel(NormRopeGrad g,
+                                                                           int head_dim, int rows,
+                                                                           int w_dtype) {
+  __shared__ float part[kSumRows][kSumCols + 1];
+  const int col = threadIdx.x % kSumCols, rg = threadIdx.x / kSumCols;
+  const int i = blockIdx.x * kSumCols + col;
+  float s = 0.f;
+#pragma unroll 8
+  for (int r = rg; r < rows; r += kSumRows) s += g.partial[(int64_t)r * 2 * head_dim + i];
+  part[rg][col] = s;
+  __syncthreads();
+  if (rg != 0) return;
+#pragma unroll
+  for (int r = 1; r < kSumRows; ++r) s += part[r][col];
+  void* dst = i < head_dim ? g.dq_weight : g.dk_weight;
+  if (dst == nullptr) return;
+  const int e = i % head_dim;
+  if (w_dtype == 2)
+    static_cast<float*>(dst)[e] = s;
+  else if (w_dtype == 0)
+    static_cast<__bf16*>(dst)[e] = (__bf16)s;
+  else
+    static_cast<_Float16*>(dst)[e] = (_Float16)s;
+}
+
+template <int D, typename Tag, bool kPairs>
+hipError_t launch_fwd(NormRopeParams p, const AppendParams& a, int cache, hipStream_t stream) {
+  using S = RowShape<D>;
+  const int heads = p.n_heads + (cache != 0 ? 2 : 1) * p.kv_heads;
+  const int64_t blocks = (p.total + S::kPerBlock - 1) / S::kPerBlock;
+  // Heads a lane group walks over: all of a token's where the tokens fill the chip, fewer
+  // for fewer tokens.
+  int64_t chunks = (2048 + blocks - 1) / blocks;
+  if (chunks > (heads + 1) / 2) chunks = (heads + 1) / 2;
+  p.heads_per = (int)((heads + chunks - 1) / chunks);
+  const dim3 grid((unsigned)blocks, (unsigned)((heads + p.heads_per - 1) / p.heads_per));
+  if (cache == 0)
+    hipLaunchKernelGGL((norm_rope_kernel<D, Tag, kPairs, 0>), grid, dim3(kThreads), 0, stream, p, a);
+  else if (cache == 1)
+    hipLaunchKernelGGL((norm_rope_kernel<D, Tag, kPairs, 1>), grid, dim3(kThreads), 0, stream, p, a);
+  else
+    hipLaunchKernelGGL((norm_rope_kernel<D, Tag, kPairs, 2>), grid, dim3(kThreads), 0, stream, p, a);
+  return hipGetLastError();
+}
+
+template <int D, typename Tag, bool kPairs>
+hipError_t launch_bwd(const NormRopeParams& p, const NormRopeGrad& g, hipStream_t stream) {
+  const int64_t rows = norm_rope_bwd_rows(p.total, D);
+  hipLaunchKernelGGL((norm_rope_bwd_kernel<D, Tag, kPairs>), dim3((unsigned)rows), dim3(kThreads), 0,
+                     stream, p, g);
+  if (g.partial != nullptr) {
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(norm_rope_dw_kernel, dim3(2 * D / kSumCols), dim3(kSumCols * kSumRows), 0,
+                       stream, g, D, (int)rows, p.w_dtype);
+  }
+  return hipGetLastError();
+}
+
+// f(D, Tag, pairs) for the call's head_dim, type and kind of rotation.
+template <typename F>
+hipError_t dispatch(const NormRopeParams& p, int head_dim, int dtype, F f) {
+  auto by_pairs = [&](auto d, auto tag) {
+    return p.pairs ? f(d, tag, std::true_type{}) : f(d, tag, std::false_type{});
+  };
+  auto by_type = [&](auto d) {
+    return dtype == 0 ? by_pairs(d, Bf16Tag{}) : by_pairs(d, F16Tag{});
+  };
+  return head_dim == 128 ? by_type(std::integral_constant<int, 128>{})
+                         : by_type(std::integral_constant<int, 64>{});
+}
+
+}  // namespace
+
+int64_t norm_rope_bwd_rows(int64_t total, int head_dim) {
+  const int64_t per = kThreads / (head_dim / 8);
+  const int64_t blocks = (total + per - 1) / per;
+  return blocks < kNormRopeBwdBlocks ? blocks : kNormRopeBwdBlocks;
+}
+
+hipError_t launch_norm_rope(const NormRopeParams& p, const AppendParams& a, int cache, int head_dim,
+                            int dtype, hipStream_t stream) {
+  return dispatch(p, head_dim, dtype, [&](auto d, auto tag, auto pairs) {
+    return launch_fwd<decltype(d)::value, decltype(tag), decltype(pairs)::value>(p, a, cache, stream);
+  });
+}
+
+hipError_t launch_norm_rope_bwd(const NormRopeParams& p, const NormRopeGrad& g, int head_dim,
+                                int dtype, hipStream_t stream) {
+  return dispatch(p, head_dim, dtype, [&](auto d, auto tag, auto pairs) {
+    return launch_bwd<decltype(d)::value, decltype(tag), decltype(pairs)::value>(p, g, stream);
+  });
+}
+
+}  // namespace ifa4

@@ -9,39 +9,18 @@
 // Mirrors the wrapper signature of inkling_fa4_rel_attention_triton
 // (src/inkling_fa4/triton_kernel.py:84-107); the Python layer (inkling_fa4.ops)
 // keeps the positional API and adds softmax_scale / return_lse.
-#include <ATen/ATen.h>
-#include <ATen/hip/EmptyTensor.h>
-#include <torch/library.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/library.h>
 
 #include <tuple>
 
-#include "ifa4.h"
+#include "torch_util.h"
 
 namespace {
 
-int32_t dtype_code(at::ScalarType t) {
-  switch (t) {
-    case at::kBFloat16: return IFA4_BF16;
-    case at::kHalf: return IFA4_FP16;
-    case at::kFloat: return IFA4_FP32;
-    default: return -1;
-  }
-}
-
-// Uninitialised tensors on q's GPU from the caching allocator, without a dispatcher
-// round per tensor (the output, the LSE and the workspace of a call: 9.4 -> 8.4 us
-// of host time for a short prompt).  Where deterministic algorithms are on, through
-// at::empty, which fills them: rows no sequence covers come back as it leaves them.
-at::Tensor empty_on(const at::Tensor& q, at::IntArrayRef sizes, at::ScalarType dtype) {
-  if (at::globalContext().deterministicAlgorithms())
-    return at::empty(sizes, q.options().dtype(dtype).memory_format(at::MemoryFormat::Contiguous));
-  return at::Tensor(at::detail::empty_cuda(sizes, dtype, q.device(), std::nullopt));
-}
-
-void check_status(int32_t st, const char* what) {
-  TORCH_CHECK(st == IFA4_OK, "inkling_fa4.", what, ": ", ifa4_status_str(st));
-}
+using ifa4_torch::check_status;
+using ifa4_torch::dtype_code;
+using ifa4_torch::empty_on;
 
 ifa4_args make_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                     const at::Tensor& rel, const at::Tensor& cu_q, const at::Tensor& cu_k,

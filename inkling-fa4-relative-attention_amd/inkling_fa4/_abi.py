@@ -80,10 +80,52 @@ class Ifa4RelProj(ctypes.Structure):
                 ("r_stride_t", _c_int64), ("r_stride_h", _c_int64), ("wt", _vp)]
 
 
+class Ifa4NormRope(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("dtype", _c_int32), ("w_dtype", _c_int32), ("head_dim", _c_int32),
+        ("n_heads", _c_int32), ("kv_heads", _c_int32), ("rot_dim", _c_int32),
+        ("interleaved", _c_int32), ("max_position", _c_int32), ("eps", ctypes.c_float),
+        ("total", _c_int64),
+        ("q", _vp), ("k", _vp), ("q_out", _vp), ("k_out", _vp),
+        ("q_stride_t", _c_int64), ("q_stride_h", _c_int64),
+        ("k_stride_t", _c_int64), ("k_stride_h", _c_int64),
+        ("q_out_stride_t", _c_int64), ("q_out_stride_h", _c_int64),
+        ("k_out_stride_t", _c_int64), ("k_out_stride_h", _c_int64),
+        ("q_weight", _vp), ("k_weight", _vp), ("cos", _vp), ("sin", _vp),
+        ("angle_stride", _c_int64), ("positions", _vp),
+    ]
+
+
+class Ifa4NormRopeGrad(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("gq", _vp), ("gk", _vp), ("dq", _vp), ("dk", _vp),
+        ("gq_stride_t", _c_int64), ("gq_stride_h", _c_int64),
+        ("gk_stride_t", _c_int64), ("gk_stride_h", _c_int64),
+        ("dq_stride_t", _c_int64), ("dq_stride_h", _c_int64),
+        ("dk_stride_t", _c_int64), ("dk_stride_h", _c_int64),
+        ("dq_weight", _vp), ("dk_weight", _vp),
+    ]
+
+
+class Ifa4KvAppend(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32), ("kv_dtype", _c_int32),
+        ("v", _vp), ("v_stride_t", _c_int64), ("v_stride_h", _c_int64),
+        ("k_cache", _vp), ("v_cache", _vp),
+        ("k_cache_stride_t", _c_int64), ("k_cache_stride_h", _c_int64),
+        ("v_cache_stride_t", _c_int64), ("v_cache_stride_h", _c_int64),
+        ("cu_seqlens", _vp), ("batch", _c_int32),
+        ("k_scale", ctypes.c_float), ("v_scale", ctypes.c_float),
+    ]
+
+
 _P_ARGS = ctypes.POINTER(Ifa4Args)
 _P_PAGED = ctypes.POINTER(Ifa4PagedKV)
 _P_QUANT = ctypes.POINTER(Ifa4KvQuant)
 _P_TILE = ctypes.POINTER(Ifa4Tile)
+_P_NORM = ctypes.POINTER(Ifa4NormRope)
 _P_I32 = ctypes.POINTER(ctypes.c_int32)
 _P_I64 = ctypes.POINTER(ctypes.c_int64)
 
@@ -110,6 +152,11 @@ SIGNATURES = {
     "ifa4_decode_quant_workspace_bytes": (ctypes.c_size_t, [_P_ARGS, _P_PAGED, _P_QUANT]),
     "ifa4_decode_quant_fwd": (_c_int32, [_P_ARGS, _P_PAGED, _P_QUANT, _vp, ctypes.c_size_t,
                                          _vp]),
+    "ifa4_qk_norm_rope_fwd": (_c_int32, [_P_NORM, _vp]),
+    "ifa4_qk_norm_rope_bwd_workspace_bytes": (ctypes.c_size_t, [_P_NORM]),
+    "ifa4_qk_norm_rope_bwd": (_c_int32, [_P_NORM, ctypes.POINTER(Ifa4NormRopeGrad), _vp,
+                                         ctypes.c_size_t, _vp]),
+    "ifa4_kv_append_paged": (_c_int32, [_P_NORM, ctypes.POINTER(Ifa4KvAppend), _P_PAGED, _vp]),
 }
 
 _lib = None
@@ -166,6 +213,29 @@ def make_quant(**kw):
     for k, v in kw.items():
         setattr(qt, k, v)
     return qt
+
+
+def _filled(cls, kw):
+    x = cls()
+    x.struct_size = ctypes.sizeof(cls)
+    for k, v in kw.items():
+        setattr(x, k, v)
+    return x
+
+
+def make_norm_rope(**kw):
+    """Ifa4NormRope with struct_size filled and eps 1e-6, fields from kw."""
+    return _filled(Ifa4NormRope, dict({"eps": 1e-6}, **kw))
+
+
+def make_norm_rope_grad(**kw):
+    """Ifa4NormRopeGrad with struct_size filled, fields from kw."""
+    return _filled(Ifa4NormRopeGrad, kw)
+
+
+def make_kv_append(**kw):
+    """Ifa4KvAppend with struct_size filled and scales 1, fields from kw."""
+    return _filled(Ifa4KvAppend, dict({"k_scale": 1.0, "v_scale": 1.0}, **kw))
 
 
 def prefill_tile(head_dim, batch=0, n_heads=1, seq_len=0, causal=True):

@@ -17,6 +17,9 @@ Contents
                  the oracle over a paged cache (the serving format of
                  outputs/architecture.md:117-120; no kernel counterpart in
                  the reference).
+  norm_rope.py   RMS norm of head rows, the position rotation, their backward
+                 pass, and the positions of an append, in fp64 (no kernel
+                 counterpart in the reference).
 
 How each function is pinned (see tests/test_oracle_*.py):
   ref_rel_attn   golden vectors written by tests/golden/make_golden.py from
