@@ -303,6 +303,36 @@ int32_t ifa4_decode_quant_fwd(const ifa4_args* args, const ifa4_paged_kv* kv,
                               size_t workspace_bytes, void* stream);
 
 /*
+ * Decode of a batch whose sequences begin with the same keys (a shared prompt): the
+ * result of paged decode with bottom-right alignment (args.flags must hold
+ * IFA4_FLAG_BOTTOM_RIGHT), computed with the prefix read and multiplied once for the
+ * whole batch.  The caller states that keys 0 .. prefix_len - 1 of every sequence that
+ * has them are those of prefix_table (any sequence's table row serves): row j % block_size
+ * of block prefix_table[j / block_size].  Table rows stay whole: of the prefix the call
+ * takes as many keys as fill its tiles from prefix_table and the rest from each
+ * sequence's own row.  A sequence may be shorter than the prefix, or empty (out = 0, lse
+ * = -inf).  quant: NULL for a 16-bit cache.  Differences from paged decode: the bias of
+ * the batch spans less than 2 GiB; biases down to the lowest finite fp32 keep their
+ * softmax (a row with no other key gets the mean of its values); values of prefix keys
+ * that some sequence does not see must be finite.  The workspace
+ * (ifa4_decode_shared_workspace_bytes, 256-byte aligned, contents on entry irrelevant) is
+ * scratch for one call.  The reference has no kernel for it.
+ */
+typedef struct ifa4_shared_prefix {
+  uint32_t struct_size;         /* sizeof(ifa4_shared_prefix) */
+  int32_t prefix_len;           /* keys, >= 0 */
+  const int32_t* prefix_table;  /* device int32 [prefix_blocks] */
+  int32_t prefix_blocks;        /* >= ceil(prefix_len / block_size) */
+} ifa4_shared_prefix;
+
+size_t ifa4_decode_shared_workspace_bytes(const ifa4_args* args, const ifa4_paged_kv* kv,
+                                          const ifa4_shared_prefix* prefix,
+                                          const ifa4_kv_quant* quant);
+int32_t ifa4_decode_shared_fwd(const ifa4_args* args, const ifa4_paged_kv* kv,
+                               const ifa4_shared_prefix* prefix, const ifa4_kv_quant* quant,
+                               void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Allocation-free decode: ifa4_decode_fwd with the library's own workspace
  * instead of a workspace argument.  No counterpart in the reference; it is for
  * callers that cannot allocate device memory (code under HIP graph capture,

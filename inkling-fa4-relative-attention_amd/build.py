@@ -22,8 +22,8 @@ BUILD = os.path.join(HERE, "_build")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 HIPCC = os.path.join(ROCM, "bin", "hipcc")
 
-LIB_SOURCES = ["prefill_fwd.hip", "decode_fwd.hip", "decode_noalloc.hip", "norm_rope.hip",
-               "ifa4_api.cpp", "norm_rope_api.cpp"]
+LIB_SOURCES = ["prefill_fwd.hip", "decode_fwd.hip", "decode_noalloc.hip", "decode_shared.hip",
+               "norm_rope.hip", "ifa4_api.cpp", "norm_rope_api.cpp"]
 EXT_SOURCES = ["torch_ext.cpp", "torch_norm_rope.cpp"]
 LIB_NAME = "libifa4.so"
 EXT_NAME = "_ifa4_torch.so"

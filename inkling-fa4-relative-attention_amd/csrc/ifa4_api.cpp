@@ -487,6 +487,113 @@ int32_t run_decode(const ifa4_args* args, const ifa4_paged_kv* kv, const ifa4_kv
   return e == hipSuccess ? IFA4_OK : IFA4_ELAUNCH;
 }
 
+// Elements of the bias from the first row's first to the last row's last.
+int64_t shared_rel_span(const ifa4_args* a) {
+  return (a->total_q - 1) * a->rel_stride_t + (a->n_heads - 1) * a->rel_stride_h + a->rel_width;
+}
+
+// Checks of a decode call behind a shared prefix.
+int32_t check_shared(const ifa4_args* a, const ifa4_paged_kv* kv, const ifa4_shared_prefix* sp,
+                     const ifa4_kv_quant* qt) {
+  if (kv == nullptr || sp == nullptr || sp->struct_size != sizeof(ifa4_shared_prefix))
+    return IFA4_EINVAL;
+  const int32_t st = check_decode(a, kv, qt);
+  if (st != IFA4_OK) return st;
+  if ((a->flags & IFA4_FLAG_BOTTOM_RIGHT) == 0) return IFA4_EUNSUPPORTED;
+  if (sp->prefix_len < 0 || sp->prefix_blocks < 0) return IFA4_EINVAL;
+  if (a->batch == 0) return IFA4_OK;
+  if (sp->prefix_len > 0 && (sp->prefix_table == nullptr || !aligned(sp->prefix_table, 4)))
+    return IFA4_EINVAL;
+  if ((int64_t)sp->prefix_blocks * kv->block_size < sp->prefix_len) return IFA4_EINVAL;
+  // the bias of all rows is read through one buffer resource
+  const int64_t esize = a->rel_dtype == IFA4_FP32 ? 4 : 2;
+  if (a->rel_extent > 0 && shared_rel_span(a) * esize >= (int64_t(1) << 31))
+    return IFA4_EUNSUPPORTED;
+  if ((int64_t)a->batch * a->n_heads >= (int64_t(1) << 24)) return IFA4_EUNSUPPORTED;
+  return IFA4_OK;
+}
+
+ifa4::SharedPlan shared_plan(const ifa4_args* a, const ifa4_shared_prefix* sp) {
+  return ifa4::shared_plan(a->batch, a->kv_heads, a->n_heads / a->kv_heads, sp->prefix_len,
+                           a->max_seqlen_k);
+}
+
+// Workspace: O of every part and query head, then their maxima and sums.
+struct SharedLayout {
+  int64_t o_bytes, ml_bytes;
+  int64_t total() const { return o_bytes + ml_bytes; }
+};
+SharedLayout shared_layout(const ifa4_args* a, const ifa4::SharedPlan& pl) {
+  const int64_t rows = (pl.prefix_chunks + pl.own_chunks) * a->batch * a->n_heads;
+  return SharedLayout{(rows * a->head_dim * 4 + 255) / 256 * 256, (rows * 8 + 255) / 256 * 256};
+}
+
+int32_t run_shared(const ifa4_args* a, const ifa4_paged_kv* kv, const ifa4_shared_prefix* sp,
+                   const ifa4_kv_quant* qt, void* workspace, size_t workspace_bytes, void* stream) {
+  const int32_t st = check_shared(a, kv, sp, qt);
+  if (st != IFA4_OK || a->batch == 0) return st;
+  const ifa4::SharedPlan pl = shared_plan(a, sp);
+  const SharedLayout l = shared_layout(a, pl);
+  if (l.total() > 0 && (workspace == nullptr || workspace_bytes < (size_t)l.total() ||
+                        !aligned(workspace, 256)))
+    return IFA4_EWORKSPACE;
+  if (pl.prefix_blocks + (int64_t)a->batch * a->kv_heads * pl.own_chunks > INT32_MAX)
+    return IFA4_EUNSUPPORTED;
+  ifa4::SharedParams p{};
+  p.q = a->q;
+  p.k = a->k;
+  p.v = a->v;
+  p.rel = a->rel;
+  p.out = a->out;
+  p.lse = a->lse;
+  p.cu_q = a->cu_seqlens_q;
+  p.seqused_k = kv->seqused_k;
+  p.block_table = kv->block_table;
+  p.prefix_table = sp->prefix_table;
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + l.o_bytes);
+  p.q_st = a->q_stride_t;
+  p.q_sh = a->q_stride_h;
+  p.k_st = a->k_stride_t;
+  p.k_sh = a->k_stride_h;
+  p.v_st = a->v_stride_t;
+  p.v_sh = a->v_stride_h;
+  p.rel_st = a->rel_stride_t;
+  p.rel_sh = a->rel_stride_h;
+  p.o_st = a->out_stride_t;
+  p.o_sh = a->out_stride_h;
+  p.lse_sh = a->lse_stride_h;
+  p.k_sblk = kv->k_stride_block;
+  p.v_sblk = kv->v_stride_block;
+  p.bt_stride = kv->block_table_stride;
+  p.rel_span = a->rel_extent > 0 ? shared_rel_span(a) : 0;
+  p.total_q = clamp_rows(a->total_q);
+  p.batch = a->batch;
+  p.n_heads = a->n_heads;
+  p.kv_heads = a->kv_heads;
+  p.group = a->n_heads / a->kv_heads;
+  p.rel_extent = a->rel_extent;
+  p.rel_dtype = a->rel_dtype;
+  p.window_left = a->window_left < (1 << 30) ? a->window_left : (1 << 30);
+  p.block_shift = __builtin_ctz((unsigned)kv->block_size);
+  p.num_blocks = kv->num_blocks;
+  p.max_blocks = kv->max_blocks_per_seq;
+  p.prefix_entries = sp->prefix_blocks;
+  p.prefix_keys = (int32_t)pl.prefix_keys;
+  p.chunk_keys = (int32_t)pl.chunk_keys;
+  p.prefix_chunks = (int32_t)pl.prefix_chunks;
+  p.row_tiles = (int32_t)pl.row_tiles;
+  p.prefix_blocks = (int32_t)pl.prefix_blocks;
+  p.own_keys = (int32_t)pl.own_keys;
+  p.own_chunks = (int32_t)pl.own_chunks;
+  p.kv_fp8 = qt != nullptr ? 1 : 0;
+  p.scale = qt != nullptr ? a->softmax_scale * qt->k_scale : a->softmax_scale;
+  p.v_scale = qt != nullptr ? qt->v_scale : 1.f;
+  const hipError_t e = ifa4::launch_decode_shared(p, a->head_dim, a->qkv_dtype,
+                                                  static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? IFA4_OK : IFA4_ELAUNCH;
+}
+
 }  // namespace
 
 namespace ifa4 {
@@ -686,6 +793,19 @@ int32_t ifa4_decode_quant_fwd(const ifa4_args* args, const ifa4_paged_kv* kv,
                               size_t workspace_bytes, void* stream) {
   if (quant == nullptr) return IFA4_EINVAL;
   return run_decode(args, kv, quant, workspace, workspace_bytes, stream);
+}
+
+size_t ifa4_decode_shared_workspace_bytes(const ifa4_args* args, const ifa4_paged_kv* kv,
+                                          const ifa4_shared_prefix* prefix,
+                                          const ifa4_kv_quant* quant) {
+  if (check_shared(args, kv, prefix, quant) != IFA4_OK || args->batch == 0) return 0;
+  return (size_t)shared_layout(args, shared_plan(args, prefix)).total();
+}
+
+int32_t ifa4_decode_shared_fwd(const ifa4_args* args, const ifa4_paged_kv* kv,
+                               const ifa4_shared_prefix* prefix, const ifa4_kv_quant* quant,
+                               void* workspace, size_t workspace_bytes, void* stream) {
+  return run_shared(args, kv, prefix, quant, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -150,6 +150,42 @@ struct NormRopeGrad {
   float* partial;  // [norm_rope_bwd_rows][2][head_dim], or NULL without weights
 };
 
+// Paged decode behind a prefix that the whole batch shares (decode_shared.hip).
+struct SharedParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* rel;
+  void* out;
+  float* lse;
+  const int32_t* cu_q;
+  const int32_t* seqused_k;
+  const int32_t* block_table;
+  const int32_t* prefix_table;
+  float* part_o;    // [prefix_chunks + own_chunks][batch][n_heads][head_dim]
+  float2* part_ml;  // [prefix_chunks + own_chunks][batch][n_heads]: maximum (natural units), sum
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, rel_st, rel_sh, o_st, o_sh, lse_sh;
+  int64_t k_sblk, v_sblk, bt_stride;
+  int64_t rel_span;        // elements of the bias, first to last
+  int32_t total_q, batch, n_heads, kv_heads, group;
+  int32_t rel_extent, rel_dtype, window_left;
+  int32_t block_shift, num_blocks, max_blocks;
+  int32_t prefix_entries;  // of prefix_table that may be read
+  int32_t prefix_keys;     // keys of the prefix that are computed once for all, whole tiles
+  int32_t chunk_keys;      // of a prefix workgroup
+  int32_t prefix_chunks;
+  int32_t row_tiles;       // prefix workgroups side by side over batch * group rows
+  int32_t prefix_blocks;   // workgroups of the prefix, all XCDs' shares alike
+  int32_t own_keys;        // keys of an own workgroup
+  int32_t own_chunks;
+  int32_t kv_fp8;
+  float scale;             // softmax_scale (times the K scale of an e4m3 cache)
+  float v_scale;
+};
+constexpr int kSharedTile = 64, kSharedRows = 128, kSharedOwnStep = 128;
+hipError_t launch_decode_shared(const SharedParams& p, int head_dim, int qkv_dtype,
+                                hipStream_t stream);
+
 // Workgroups of the backward pass at most, each with a row of partial weight gradients.
 constexpr int64_t kNormRopeBwdBlocks = 1024;
 int64_t norm_rope_bwd_rows(int64_t total, int head_dim);

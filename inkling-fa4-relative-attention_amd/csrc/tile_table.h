@@ -441,4 +441,32 @@ inline PrefillSplit prefill_split_for(int64_t batch, int64_t n_heads, int64_t ma
   return s;
 }
 
+// Decode behind a shared prefix (decode_shared.hip): how the prefix and the sequences' own
+// keys are cut into workgroups of 128 rows x chunk_keys, and (sequence, kv head) x own_keys.
+struct SharedPlan {
+  int64_t prefix_keys;  // of the prefix that goes through its workgroups: whole 64-key tiles
+  int64_t chunk_keys, prefix_chunks, row_tiles, prefix_blocks, own_keys, own_chunks;
+};
+constexpr int64_t kSharedSlots = 512;     // resident workgroups
+constexpr int64_t kSharedMinTiles = 4;    // shortest prefix chunk
+constexpr int64_t kSharedOwnKeys = 512;
+inline SharedPlan shared_plan(int64_t batch, int64_t kv_heads, int64_t group, int64_t prefix_len,
+                              int64_t max_seqlen_k) {
+  SharedPlan s{};
+  const int64_t shared = prefix_len < max_seqlen_k ? prefix_len : max_seqlen_k;
+  const int64_t tiles = shared / 64;
+  s.prefix_keys = tiles * 64;
+  s.row_tiles = (batch * group + 127) / 128;
+  const int64_t side = s.row_tiles * kv_heads;  // workgroups of one chunk
+  int64_t chunks = side < kSharedSlots ? kSharedSlots / side : 1;
+  int64_t chunk = (tiles + chunks - 1) / chunks;
+  if (chunk < kSharedMinTiles) chunk = kSharedMinTiles;
+  s.chunk_keys = chunk * 64;
+  s.prefix_chunks = (tiles + chunk - 1) / chunk;
+  s.prefix_blocks = (s.prefix_chunks * kv_heads + 7) / 8 * 8 * s.row_tiles;
+  s.own_keys = kSharedOwnKeys;
+  s.own_chunks = (max_seqlen_k - s.prefix_keys + s.own_keys - 1) / s.own_keys;
+  return s;
+}
+
 }  // namespace ifa4

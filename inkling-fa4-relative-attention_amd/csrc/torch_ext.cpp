@@ -1,6 +1,7 @@
 // Thin PyTorch-ROCm binding over the C ABI (include/ifa4.h).
 //
-// Registers torch.ops.inkling_fa4.fwd / .fwd_rproj / .decode / .decode_paged.  The binding checks tensor
+// Registers torch.ops.inkling_fa4.fwd / .fwd_rproj / .decode / .decode_paged /
+// .decode_shared_prefix.  The binding checks tensor
 // devices, dtypes and shapes, allocates out / lse / the decode workspace from
 // torch's caching allocator, fills an ifa4_args and calls the library on the
 // current HIP stream.  No math happens here, and there is no fallback: a
@@ -9,6 +10,7 @@
 // Mirrors the wrapper signature of inkling_fa4_rel_attention_triton
 // (src/inkling_fa4/triton_kernel.py:84-107); the Python layer (inkling_fa4.ops)
 // keeps the positional API and adds softmax_scale / return_lse.
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 
@@ -220,6 +222,66 @@ std::tuple<at::Tensor, at::Tensor> decode(const at::Tensor& q, const at::Tensor&
   return {out, lse};
 }
 
+// A paged cache's checks and description: the ABI arguments of the call over the first
+// block's rows (which carry the row / head strides), with the pool as k and v, and *kv.
+ifa4_args paged_args(const char* op, const at::Tensor& q, const at::Tensor& k_cache,
+                     const at::Tensor& v_cache, const at::Tensor& rel, const at::Tensor& cu_q,
+                     const at::Tensor& seqused_k, const at::Tensor& block_table, int64_t max_q,
+                     int64_t max_k, int64_t rel_extent, bool causal, int64_t window_left,
+                     double softmax_scale, int64_t flags, ifa4_paged_kv* kv) {
+  TORCH_CHECK(k_cache.dim() == 4 && v_cache.dim() == 4,
+              "inkling_fa4.", op, ": k_cache / v_cache must be "
+              "[num_blocks, block_size, kv_heads, head_dim]");
+  TORCH_CHECK(k_cache.sizes() == v_cache.sizes(),
+              "inkling_fa4.", op, ": k_cache and v_cache shapes differ");
+  TORCH_CHECK(block_table.is_cuda() && seqused_k.is_cuda() &&
+                  block_table.device() == q.device() && seqused_k.device() == q.device(),
+              "inkling_fa4.", op, ": block_table / seqused_k must be on q's GPU");
+  TORCH_CHECK(block_table.scalar_type() == at::kInt && seqused_k.scalar_type() == at::kInt,
+              "inkling_fa4.", op, ": block_table and seqused_k must be int32");
+  TORCH_CHECK(block_table.dim() == 2 && block_table.stride(1) == 1,
+              "inkling_fa4.", op, ": block_table must be 2-D with contiguous rows");
+  TORCH_CHECK(seqused_k.dim() == 1 && seqused_k.is_contiguous(),
+              "inkling_fa4.", op, ": seqused_k must be 1-D contiguous");
+  TORCH_CHECK(block_table.size(0) == cu_q.numel() - 1 && seqused_k.numel() == cu_q.numel() - 1,
+              "inkling_fa4.", op, ": block_table / seqused_k need one row per sequence");
+  const at::Tensor k_rows = k_cache.select(0, 0);
+  const at::Tensor v_rows = v_cache.select(0, 0);
+  ifa4_args a = make_args(q, k_rows, v_rows, rel, cu_q, cu_q, max_q, max_k, rel_extent, causal,
+                          window_left, softmax_scale, flags);
+  a.k = k_cache.data_ptr();
+  a.v = v_cache.data_ptr();
+  a.cu_seqlens_k = nullptr;
+  a.total_k = 0;
+  *kv = ifa4_paged_kv{};
+  kv->struct_size = sizeof(ifa4_paged_kv);
+  kv->block_size = static_cast<int32_t>(k_cache.size(1));
+  kv->block_table = block_table.data_ptr<int32_t>();
+  kv->seqused_k = seqused_k.data_ptr<int32_t>();
+  kv->block_table_stride = block_table.stride(0);
+  kv->k_stride_block = k_cache.stride(0);
+  kv->v_stride_block = v_cache.stride(0);
+  kv->num_blocks = static_cast<int32_t>(k_cache.size(0));
+  kv->max_blocks_per_seq = static_cast<int32_t>(block_table.size(1));
+  return a;
+}
+
+// The call's outputs, described in *a: out of q's shape, lse [n_heads, total_q] or empty.
+std::tuple<at::Tensor, at::Tensor> make_outputs(const at::Tensor& q, bool return_lse,
+                                                ifa4_args* a) {
+  at::Tensor out = empty_on(q, q.sizes(), q.scalar_type());
+  at::Tensor lse = return_lse ? empty_on(q, {q.size(1), q.size(0)}, at::kFloat)
+                              : empty_on(q, {0}, at::kFloat);
+  a->out = out.data_ptr();
+  a->out_stride_t = out.stride(0);
+  a->out_stride_h = out.stride(1);
+  if (return_lse) {
+    a->lse = lse.data_ptr<float>();
+    a->lse_stride_h = lse.stride(0);
+  }
+  return {out, lse};
+}
+
 // Decode over a paged KV cache: k_cache / v_cache [num_blocks, block_size,
 // kv_heads, head_dim], block_table int32 [batch, max_blocks_per_seq],
 // seqused_k int32 [batch].  Same outputs as decode().
@@ -229,53 +291,10 @@ std::tuple<at::Tensor, at::Tensor> decode_paged(
     const at::Tensor& block_table, int64_t max_q, int64_t max_k, int64_t rel_extent, bool causal,
     int64_t window_left, double softmax_scale, bool return_lse, int64_t flags, double k_scale,
     double v_scale) {
-  TORCH_CHECK(k_cache.dim() == 4 && v_cache.dim() == 4,
-              "inkling_fa4.decode_paged: k_cache / v_cache must be "
-              "[num_blocks, block_size, kv_heads, head_dim]");
-  TORCH_CHECK(k_cache.sizes() == v_cache.sizes(),
-              "inkling_fa4.decode_paged: k_cache and v_cache shapes differ");
-  TORCH_CHECK(block_table.is_cuda() && seqused_k.is_cuda() &&
-                  block_table.device() == q.device() && seqused_k.device() == q.device(),
-              "inkling_fa4.decode_paged: block_table / seqused_k must be on q's GPU");
-  TORCH_CHECK(block_table.scalar_type() == at::kInt && seqused_k.scalar_type() == at::kInt,
-              "inkling_fa4.decode_paged: block_table and seqused_k must be int32");
-  TORCH_CHECK(block_table.dim() == 2 && block_table.stride(1) == 1,
-              "inkling_fa4.decode_paged: block_table must be 2-D with contiguous rows");
-  TORCH_CHECK(seqused_k.dim() == 1 && seqused_k.is_contiguous(),
-              "inkling_fa4.decode_paged: seqused_k must be 1-D contiguous");
-  TORCH_CHECK(block_table.size(0) == cu_q.numel() - 1 && seqused_k.numel() == cu_q.numel() - 1,
-              "inkling_fa4.decode_paged: block_table / seqused_k need one row per sequence");
-  // The per-token view [blocks * block_size, kv_heads, head_dim] of the first
-  // block carries the row / head strides; block strides travel separately.
-  const at::Tensor k_rows = k_cache.select(0, 0);
-  const at::Tensor v_rows = v_cache.select(0, 0);
-  ifa4_args a = make_args(q, k_rows, v_rows, rel, cu_q, cu_q, max_q, max_k, rel_extent, causal,
-                          window_left, softmax_scale, flags);
-  a.k = k_cache.data_ptr();
-  a.v = v_cache.data_ptr();
-  a.cu_seqlens_k = nullptr;
-  a.total_k = 0;
-  ifa4_paged_kv kv{};
-  kv.struct_size = sizeof(ifa4_paged_kv);
-  kv.block_size = static_cast<int32_t>(k_cache.size(1));
-  kv.block_table = block_table.data_ptr<int32_t>();
-  kv.seqused_k = seqused_k.data_ptr<int32_t>();
-  kv.block_table_stride = block_table.stride(0);
-  kv.k_stride_block = k_cache.stride(0);
-  kv.v_stride_block = v_cache.stride(0);
-  kv.num_blocks = static_cast<int32_t>(k_cache.size(0));
-  kv.max_blocks_per_seq = static_cast<int32_t>(block_table.size(1));
-
-  at::Tensor out = empty_on(q, q.sizes(), q.scalar_type());
-  at::Tensor lse = return_lse ? empty_on(q, {q.size(1), q.size(0)}, at::kFloat)
-                              : empty_on(q, {0}, at::kFloat);
-  a.out = out.data_ptr();
-  a.out_stride_t = out.stride(0);
-  a.out_stride_h = out.stride(1);
-  if (return_lse) {
-    a.lse = lse.data_ptr<float>();
-    a.lse_stride_h = lse.stride(0);
-  }
+  ifa4_paged_kv kv;
+  ifa4_args a = paged_args("decode_paged", q, k_cache, v_cache, rel, cu_q, seqused_k, block_table,
+                           max_q, max_k, rel_extent, causal, window_left, softmax_scale, flags, &kv);
+  const auto [out, lse] = make_outputs(q, return_lse, &a);
   const bool kv_fp8 = k_cache.scalar_type() == at::kFloat8_e4m3fn;
   const ifa4_kv_quant qt = kv_quant(k_scale, v_scale);
   const size_t ws_bytes = kv_fp8 ? ifa4_decode_quant_workspace_bytes(&a, &kv, &qt)
@@ -291,6 +310,42 @@ std::tuple<at::Tensor, at::Tensor> decode_paged(
   check_status(kv_fp8 ? ifa4_decode_quant_fwd(&a, &kv, &qt, aligned_ws, ws_bytes, stream)
                       : ifa4_decode_paged_fwd(&a, &kv, aligned_ws, ws_bytes, stream),
                "decode_paged");
+  return {out, lse};
+}
+
+// Decode over a paged KV cache whose first prefix_len keys are those of prefix_table for
+// every sequence; bottom-right alignment.  Same outputs as decode_paged().
+std::tuple<at::Tensor, at::Tensor> decode_shared_prefix(
+    const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+    const at::Tensor& rel, const at::Tensor& cu_q, const at::Tensor& seqused_k,
+    const at::Tensor& block_table, const at::Tensor& prefix_table, int64_t prefix_len,
+    int64_t max_q, int64_t max_k, int64_t rel_extent, int64_t window_left, double softmax_scale,
+    bool return_lse, double k_scale, double v_scale) {
+  constexpr const char* op = "decode_shared_prefix";
+  ifa4_paged_kv kv;
+  ifa4_args a = paged_args(op, q, k_cache, v_cache, rel, cu_q, seqused_k, block_table, max_q, max_k,
+                           rel_extent, true, window_left, softmax_scale, IFA4_FLAG_BOTTOM_RIGHT, &kv);
+  TORCH_CHECK(prefix_table.is_cuda() && prefix_table.device() == q.device() &&
+                  prefix_table.scalar_type() == at::kInt && prefix_table.dim() == 1 &&
+                  prefix_table.is_contiguous(),
+              "inkling_fa4.", op, ": prefix_table must be int32, 1-D, contiguous, on q's GPU");
+  TORCH_CHECK(prefix_len >= 0 && prefix_len <= INT32_MAX && prefix_table.numel() <= INT32_MAX,
+              "inkling_fa4.", op, ": prefix_len out of range");
+  const c10::DeviceGuard guard(q.device());
+  ifa4_shared_prefix sp{};
+  sp.struct_size = sizeof(ifa4_shared_prefix);
+  sp.prefix_len = static_cast<int32_t>(prefix_len);
+  sp.prefix_table = prefix_table.data_ptr<int32_t>();
+  sp.prefix_blocks = static_cast<int32_t>(prefix_table.numel());
+  const auto [out, lse] = make_outputs(q, return_lse, &a);
+  const ifa4_kv_quant qt = kv_quant(k_scale, v_scale);
+  const ifa4_kv_quant* quant = k_cache.scalar_type() == at::kFloat8_e4m3fn ? &qt : nullptr;
+  // invalid arguments: 0 bytes, and the call reports which status
+  const size_t ws_bytes = ifa4_decode_shared_workspace_bytes(&a, &kv, &sp, quant);
+  const at::Tensor ws = ws_bytes > 0 ? empty_on(q, {(int64_t)ws_bytes}, at::kByte) : at::Tensor();
+  check_status(ifa4_decode_shared_fwd(&a, &kv, &sp, quant, ws_bytes > 0 ? ws.data_ptr() : nullptr,
+                                      ws_bytes, c10::hip::getCurrentHIPStream(q.device().index()).stream()),
+               op);
   return {out, lse};
 }
 
@@ -315,6 +370,11 @@ TORCH_LIBRARY(inkling_fa4, m) {
       "Tensor cu_seqlens_q, Tensor seqused_k, Tensor block_table, int max_seqlen_q, "
       "int max_seqlen_k, int rel_extent, bool causal, int window_left, float softmax_scale, "
       "bool return_lse, int flags, float k_scale, float v_scale) -> (Tensor, Tensor)");
+  m.def(
+      "decode_shared_prefix(Tensor q, Tensor k_cache, Tensor v_cache, Tensor rel_logits, "
+      "Tensor cu_seqlens_q, Tensor seqused_k, Tensor block_table, Tensor prefix_table, "
+      "int prefix_len, int max_seqlen_q, int max_seqlen_k, int rel_extent, int window_left, "
+      "float softmax_scale, bool return_lse, float k_scale, float v_scale) -> (Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(inkling_fa4, CUDA, m) {
@@ -322,4 +382,5 @@ TORCH_LIBRARY_IMPL(inkling_fa4, CUDA, m) {
   m.impl("fwd_rproj", &fwd_rproj);
   m.impl("decode", &decode);
   m.impl("decode_paged", &decode_paged);
+  m.impl("decode_shared_prefix", &decode_shared_prefix);
 }

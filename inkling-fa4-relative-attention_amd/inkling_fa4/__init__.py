@@ -3,7 +3,8 @@
 Same export names as the reference package (src/inkling_fa4/__init__.py:1-11),
 minus `ref_rel_attn`: the fp32 oracle is test infrastructure and lives in the
 repository's `oracle/` package, outside the product.  Added: the paged-KV
-decode entry point `inkling_fa4_rel_attention_decode_paged` and the fused
+decode entry points `inkling_fa4_rel_attention_decode_paged` and
+`inkling_fa4_rel_attention_decode_shared_prefix`; the fused
 relative-logit projection `inkling_fa4_rel_attention_rproj`; and the steps before
 the attention, `inkling_fa4_qk_norm_rope` and `inkling_fa4_kv_append_paged`.
 """
@@ -13,6 +14,7 @@ from .ops import (
     inkling_fa4_rel_attention,
     inkling_fa4_rel_attention_decode,
     inkling_fa4_rel_attention_decode_paged,
+    inkling_fa4_rel_attention_decode_shared_prefix,
     inkling_fa4_rel_attention_decode_triton,
     inkling_fa4_rel_attention_kv_pruned_triton,
     inkling_fa4_rel_attention_rproj,
@@ -24,6 +26,7 @@ __all__ = [
     "inkling_fa4_rel_attention",
     "inkling_fa4_rel_attention_decode",
     "inkling_fa4_rel_attention_decode_paged",
+    "inkling_fa4_rel_attention_decode_shared_prefix",
     "inkling_fa4_rel_attention_triton",
     "inkling_fa4_rel_attention_decode_triton",
     "inkling_fa4_rel_attention_kv_pruned_triton",

@@ -80,6 +80,11 @@ class Ifa4RelProj(ctypes.Structure):
                 ("r_stride_t", _c_int64), ("r_stride_h", _c_int64), ("wt", _vp)]
 
 
+class Ifa4SharedPrefix(ctypes.Structure):
+    _fields_ = [("struct_size", ctypes.c_uint32), ("prefix_len", _c_int32),
+                ("prefix_table", _vp), ("prefix_blocks", _c_int32)]
+
+
 class Ifa4NormRope(ctypes.Structure):
     _fields_ = [
         ("struct_size", ctypes.c_uint32),
@@ -125,6 +130,7 @@ _P_ARGS = ctypes.POINTER(Ifa4Args)
 _P_PAGED = ctypes.POINTER(Ifa4PagedKV)
 _P_QUANT = ctypes.POINTER(Ifa4KvQuant)
 _P_TILE = ctypes.POINTER(Ifa4Tile)
+_P_SHARED = ctypes.POINTER(Ifa4SharedPrefix)
 _P_NORM = ctypes.POINTER(Ifa4NormRope)
 _P_I32 = ctypes.POINTER(ctypes.c_int32)
 _P_I64 = ctypes.POINTER(ctypes.c_int64)
@@ -152,6 +158,10 @@ SIGNATURES = {
     "ifa4_decode_quant_workspace_bytes": (ctypes.c_size_t, [_P_ARGS, _P_PAGED, _P_QUANT]),
     "ifa4_decode_quant_fwd": (_c_int32, [_P_ARGS, _P_PAGED, _P_QUANT, _vp, ctypes.c_size_t,
                                          _vp]),
+    "ifa4_decode_shared_workspace_bytes": (ctypes.c_size_t, [_P_ARGS, _P_PAGED, _P_SHARED,
+                                                             _P_QUANT]),
+    "ifa4_decode_shared_fwd": (_c_int32, [_P_ARGS, _P_PAGED, _P_SHARED, _P_QUANT, _vp,
+                                          ctypes.c_size_t, _vp]),
     "ifa4_qk_norm_rope_fwd": (_c_int32, [_P_NORM, _vp]),
     "ifa4_qk_norm_rope_bwd_workspace_bytes": (ctypes.c_size_t, [_P_NORM]),
     "ifa4_qk_norm_rope_bwd": (_c_int32, [_P_NORM, ctypes.POINTER(Ifa4NormRopeGrad), _vp,
@@ -221,6 +231,11 @@ def _filled(cls, kw):
     for k, v in kw.items():
         setattr(x, k, v)
     return x
+
+
+def make_shared_prefix(**kw):
+    """Ifa4SharedPrefix with struct_size filled, fields from kw."""
+    return _filled(Ifa4SharedPrefix, kw)
 
 
 def make_norm_rope(**kw):

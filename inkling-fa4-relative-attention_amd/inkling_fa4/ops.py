@@ -11,7 +11,8 @@ plus the same entry points under names without the `_triton` suffix, and
 `inkling_fa4_rel_attention_decode_paged` for a paged KV cache (block tables),
 the format of the serving caller (outputs/architecture.md:117-120), and
 `inkling_fa4_rel_attention_rproj` with the bias computed in the kernel from the
-RelLogitsProj factors (outputs/architecture.md:24,52-54).
+RelLogitsProj factors (outputs/architecture.md:24,52-54);
+`inkling_fa4_rel_attention_decode_shared_prefix` for a paged batch behind one prompt.
 
 Differences from the reference wrappers (all deliberate):
   * one kernel launch for the whole batch and no host synchronisation (the
@@ -183,6 +184,35 @@ def inkling_fa4_rel_attention_decode_paged(q, k_cache, v_cache, rel_logits, cu_s
                      block_table, int(max_seqlen_q), int(max_seqlen_k), int(rel_extent),
                      bool(causal), _window_left(window_size), scale, bool(return_lse),
                      _flag_bits(bottom_right), float(k_scale), float(v_scale))
+    return (out, lse) if return_lse else out
+
+
+def inkling_fa4_rel_attention_decode_shared_prefix(q, k_cache, v_cache, rel_logits, cu_seqlens_q,
+                                                   seqused_k, block_table, prefix_table,
+                                                   prefix_len, max_seqlen_q, max_seqlen_k,
+                                                   rel_extent, window_size=(-1, -1), *,
+                                                   softmax_scale=None, return_lse=False,
+                                                   k_scale=1.0, v_scale=1.0):
+    """Paged decode of a batch whose sequences begin with the same keys: the result of
+    inkling_fa4_rel_attention_decode_paged(..., bottom_right=True), with the keys and values
+    of the prefix read and multiplied once for the whole batch.
+
+    The caller states that the first prefix_len keys of every sequence are those of
+    prefix_table, int32 [>= ceil(prefix_len / block_size)] (any sequence's row of
+    block_table serves): key j in block prefix_table[j // block_size] at row
+    j % block_size.  The rows of block_table stay whole: of the prefix, the keys that do
+    not fill a tile of 64 are read through them.  seqused_k counts all keys; a sequence may
+    be shorter than the prefix or empty (out 0, lse -inf).  The other arguments, types and
+    head layouts as in inkling_fa4_rel_attention_decode_paged.  Values of prefix keys that
+    some sequence does not see (a window, a shorter sequence) must be finite.
+    """
+    if k_cache.dim() != 4:
+        raise ValueError("k_cache must be [num_blocks, block_size, kv_heads, head_dim]")
+    scale = _resolve(q, k_cache.shape[1:], None, None, None, softmax_scale)
+    out, lse = _call("decode_shared_prefix", q, k_cache, v_cache, rel_logits, cu_seqlens_q,
+                     seqused_k, block_table, prefix_table, int(prefix_len), int(max_seqlen_q),
+                     int(max_seqlen_k), int(rel_extent), _window_left(window_size), scale,
+                     bool(return_lse), float(k_scale), float(v_scale))
     return (out, lse) if return_lse else out
 
 
