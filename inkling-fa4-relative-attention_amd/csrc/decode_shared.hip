@@ -101,20 +101,11 @@ __device__ __forceinline__ int first_key(const SharedParams& p, int pos) {
   return p.window_left >= 0 ? max(0, pos - p.window_left) : 0;
 }
 
-// Table entries of the keys a workgroup or wave walks over: lane L holds entry base + L, base a
-// multiple of 64 (32 keys from a multiple of 32 on never straddle two windows).
-struct PageWindow {
-  const int32_t* table;
-  int entries;  // of the table that may be read
-  int base, held;
-};
-__device__ __forceinline__ int pages_at(PageWindow& w, int i, int lane) {
-  const int base = i & ~63;
-  if (base != w.base) {
-    w.base = base;
-    w.held = base + lane < w.entries ? w.table[base + lane] : -1;
-  }
-  return __builtin_amdgcn_readlane(w.held, i - base);
+// Table entry of key k0 (wave-uniform), by a scalar load: a load through the vector memory
+// counter would have to wait for the K and V rows in flight before it.
+__device__ __forceinline__ int page_at(const int32_t* table, int i, int entries) {
+  typedef const __attribute__((address_space(4))) int32_t* scalar_ptr;
+  return ((scalar_ptr)(uintptr_t)table)[min(i, entries - 1)];
 }
 
 template <int D, typename Tag, typename Rel, int Eb>
@@ -271,6 +262,15 @@ __global__ __launch_bounds__(kThreads, 2) void decode_shared_kernel(SharedParams
             *reinterpret_cast<const u32x4_t*>(kl + row * D + 8 * ((2 * kk + half) ^ sw)), qf[kk],
             s[blk]);
     }
+    // four fragment reads in flight ahead of the products
+    constexpr int kReads = kNb * kKSteps, kAhead = 4;
+    __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+    for (int i = 0; i < kReads - kAhead; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
     __builtin_amdgcn_s_setprio(0);
     auto read_vt = [&](int db, int t) -> u32x4_t {
       u32x2_t w[2];
@@ -355,55 +355,90 @@ __global__ __launch_bounds__(kThreads, 2) void decode_shared_kernel(SharedParams
       }
       if (t + 1 < 2 * kNb) pcur = make_p(t + 1);
     }
+    // each product followed by the two reads of the next block's fragment and a share of its
+    // exponentials (about 28 vector instructions over the products of a block)
+#pragma unroll
+    for (int t = 0; t < 2 * kNb - 1; ++t) {
+#pragma unroll
+      for (int db = 0; db < kDBlocks; ++db) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+        __builtin_amdgcn_sched_group_barrier(0x402, 28 / kDBlocks, 1);
+      }
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, kDBlocks, 1);
     __builtin_amdgcn_s_setprio(0);
   };
 
   // ---- K / V rows to LDS ----------------------------------------------------------------------
-  // `rows` rows of one tensor from key k0 on, `nwaves`-th share of a tile; the rows of one DMA (or
-  // of one register load, e4m3) lie in one block.  Keys from key_stop on read as zero.
-  const char* const kpool = static_cast<const char*>(p.k) + (int64_t)kvh * p.k_sh * Eb;
-  const char* const vpool = static_cast<const char*>(p.v) + (int64_t)kvh * p.v_sh * Eb;
+  // 32 rows of one tensor at a time, in groups of rows that lie in one block (blocks hold eight
+  // or more, or the rows of one load where that is more).  The groups' table entries are read
+  // ahead of their rows.
   const int bmask = (1 << p.block_shift) - 1;
-  PageWindow pages;
-  pages.table = prefix ? p.prefix_table : p.block_table + (int64_t)seq * p.bt_stride;
-  pages.entries = prefix ? p.prefix_entries : (pos_max >> p.block_shift) + 1;
-  pages.base = -1;
-  // Resource over rows [k0, k0 + n) of the cache, all in one block; empty where the entry lies
-  // outside the pool.
-  auto rows_rsrc = [&](bool is_v, int k0, int n) {
-    const int ent = pages_at(pages, k0 >> p.block_shift, lane);
-    const int64_t st = is_v ? p.v_st : p.k_st;
-    const bool good = (unsigned)ent < (unsigned)p.num_blocks && n > 0;
-    const int64_t at = (good ? (int64_t)ent : 0) * (is_v ? p.v_sblk : p.k_sblk) +
-                       (int64_t)(k0 & bmask) * st;
-    return make_rsrc_uniform((is_v ? vpool : kpool) + at * Eb,
-                             good ? (uint32_t)(((n - 1) * st + D) * Eb) : 0u);
-  };
-  constexpr int kLoadRows = 1024 / (D * Eb);   // rows of one wave load or DMA
-  constexpr int kLoads32 = 32 / kLoadRows;     // per 32 rows
-  constexpr int kLpr = D * Eb / 16;            // lanes per row
+  const int32_t* const table =
+      prefix ? p.prefix_table : p.block_table + (int64_t)seq * p.bt_stride;
+  const int entries = prefix ? p.prefix_entries : (pos_max >> p.block_shift) + 1;
+  constexpr int kLoadRows = 1024 / (D * Eb);  // rows of one wave load or DMA
+  constexpr int kLoads32 = 32 / kLoadRows;
+  constexpr int kGroupRows = kLoadRows > 8 ? kLoadRows : 8;
+  constexpr int kGroups = 32 / kGroupRows, kPerGroup = kGroupRows / kLoadRows;
+  constexpr int kLpr = D * Eb / 16;           // lanes per row
   const int ld_row = lane / kLpr, ld_chunk = lane % kLpr;
-  const uint32_t lds0 = lds_addr(stages);
-  // 32 rows of K or V from key k0 on into LDS rows tile_row .. + 31 of the tensor at `dst`
-  auto dma32 = [&](bool is_v, int k0, int stop, int tile_row, uint32_t dst) {
-    const uint32_t rowb = (uint32_t)(is_v ? p.v_st : p.k_st) * 2;
+  struct Pages {
+    int ent[kGroups];
+  };
+  auto pages_of = [&](int k0) {
+    Pages pg;
 #pragma unroll
-    for (int u = 0; u < kLoads32; ++u) {
-      const int at = kLoadRows * u;
-      const rsrc_t rs = rows_rsrc(is_v, k0 + at, min(kLoadRows, stop - k0 - at));
-      const int row = tile_row + at + ld_row;
-      dma_16_tile(rs, ld_row * rowb + 16u * (uint32_t)(ld_chunk ^ swz<L::kChunks>(row)),
-                  dst + (uint32_t)((tile_row + at) * D * 2));
+    for (int i = 0; i < kGroups; ++i)
+      pg.ent[i] = page_at(table, (k0 + kGroupRows * i) >> p.block_shift, entries);
+    return pg;
+  };
+  // One tensor's rows: pool base of the kv head, bytes between blocks and rows, LDS byte offset
+  // of a lane in each load (row times pitch, and the chunk's place).
+  struct Tensor {
+    const char* pool;
+    int64_t block;
+    uint32_t row;
+  };
+  auto tensor = [&](bool is_v) {
+    return Tensor{static_cast<const char*>(is_v ? p.v : p.k) +
+                      (int64_t)kvh * (is_v ? p.v_sh : p.k_sh) * Eb,
+                  (is_v ? p.v_sblk : p.k_sblk) * Eb, (uint32_t)(is_v ? p.v_st : p.k_st) * Eb};
+  };
+  // Resource over the group's rows [k0, min(k0 + kGroupRows, stop)): what lies past it, and a
+  // whole group whose entry lies outside the pool, reads as zero.
+  auto group_rsrc = [&](const Tensor& t, int ent, int k0, int stop) {
+    const int n = min(kGroupRows, stop - k0);
+    const bool good = (unsigned)ent < (unsigned)p.num_blocks && n > 0;
+    const uint32_t at = good ? (uint32_t)ent : 0u;
+    const char* base = t.pool + (int64_t)at * t.block + (uint32_t)(k0 & bmask) * t.row;
+    return make_rsrc_uniform(base, good ? (uint32_t)(n - 1) * t.row + D * Eb : 0u);
+  };
+  const uint32_t lds0 = lds_addr(stages);
+  // 16-bit: rows k0 .. k0 + 31 by DMA to LDS rows tile_row .. of the tensor at LDS address dst
+  auto dma32 = [&](const Tensor& t, const Pages& pg, int k0, int stop, int tile_row, uint32_t dst) {
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) {
+      const rsrc_t rs = group_rsrc(t, pg.ent[i], k0 + kGroupRows * i, stop);
+#pragma unroll
+      for (int u = 0; u < kPerGroup; ++u) {
+        const int at = kGroupRows * i + kLoadRows * u;
+        const int chunk = ld_chunk ^ swz<L::kChunks>(tile_row + at + ld_row);
+        dma_16_tile(rs, (uint32_t)(kLoadRows * u + ld_row) * t.row + 16u * (uint32_t)chunk,
+                    dst + (uint32_t)((tile_row + at) * D * 2));
+      }
     }
   };
   // e4m3: the same rows into registers, and from there to LDS in the 16-bit type
-  auto load32 = [&](bool is_v, int k0, int stop, u32x4_t* reg) {
-    const uint32_t rowb = (uint32_t)(is_v ? p.v_st : p.k_st);
+  auto load32 = [&](const Tensor& t, const Pages& pg, int k0, int stop, u32x4_t* reg) {
 #pragma unroll
-    for (int u = 0; u < kLoads32; ++u) {
-      const int at = kLoadRows * u;
-      const rsrc_t rs = rows_rsrc(is_v, k0 + at, min(kLoadRows, stop - k0 - at));
-      reg[u] = buf_load_16(rs, ld_row * rowb + 16u * ld_chunk);
+    for (int i = 0; i < kGroups; ++i) {
+      const rsrc_t rs = group_rsrc(t, pg.ent[i], k0 + kGroupRows * i, stop);
+#pragma unroll
+      for (int u = 0; u < kPerGroup; ++u)
+        reg[kPerGroup * i + u] =
+            buf_load_16(rs, (uint32_t)(kLoadRows * u + ld_row) * t.row + 16u * ld_chunk);
     }
   };
   auto put32 = [&](const u32x4_t* reg, int tile_row, uint16_t* dst) {
@@ -427,16 +462,19 @@ __global__ __launch_bounds__(kThreads, 2) void decode_shared_kernel(SharedParams
     // waves 0, 1 bring K, waves 2, 3 V; 32 rows each
     const bool is_v = wave >= 2;
     const int my_row = 32 * (wave & 1);
+    const Tensor mine_kv = tensor(is_v);
     const int kt0 = key_beg / kTile, kt1 = (key_end + kTile - 1) / kTile;
     auto run_tile = [&](int kt, const uint16_t* stage) {
       const int kb = kt * kTile;
       if (kb <= pos_max && kb + kTile > lo_min)
         compute(std::integral_constant<int, 2>{}, kb, stage, stage + L::kTensor);
     };
+    Pages pg = pages_of(kt0 * kTile + my_row);
     if constexpr (Eb == 2) {
       auto fetch = [&](int kt, int stage) {
-        dma32(is_v, kt * kTile + my_row, p.prefix_keys, my_row,
+        dma32(mine_kv, pg, kt * kTile + my_row, p.prefix_keys, my_row,
               lds0 + (uint32_t)(stage * L::kStage + (is_v ? L::kTensor : 0)) * 2);
+        pg = pages_of((kt + 1) * kTile + my_row);
       };
       fetch(kt0, 0);
       for (int kt = kt0; kt < kt1; ++kt) {
@@ -449,11 +487,15 @@ __global__ __launch_bounds__(kThreads, 2) void decode_shared_kernel(SharedParams
       }
     } else {
       u32x4_t reg[kLoads32];
-      load32(is_v, kt0 * kTile + my_row, p.prefix_keys, reg);
+      auto fetch = [&](int kt) {
+        load32(mine_kv, pg, kt * kTile + my_row, p.prefix_keys, reg);
+        pg = pages_of((kt + 1) * kTile + my_row);
+      };
+      fetch(kt0);
       for (int kt = kt0; kt < kt1; ++kt) {
         uint16_t* stage = stages + ((kt - kt0) & 1) * L::kStage;
         put32(reg, my_row, stage + (is_v ? L::kTensor : 0));
-        if (kt + 1 < kt1) load32(is_v, (kt + 1) * kTile + my_row, p.prefix_keys, reg);
+        if (kt + 1 < kt1) fetch(kt + 1);
         lds_barrier();
         run_tile(kt, stage);
       }
@@ -477,17 +519,22 @@ __global__ __launch_bounds__(kThreads, 2) void decode_shared_kernel(SharedParams
   // ---- own keys ---------------------------------------------------------------------------------
   uint16_t* const kown = stages + wave * 2 * L::kOwn;
   uint16_t* const vown = kown + L::kOwn;
-  const int s0 = key_beg & ~(kOwnStep - 1);
-  for (int k0 = s0 + kOwnStep * wave; k0 < key_end; k0 += kOwnStep * kWaves) {
+  const Tensor tk = tensor(false), tv = tensor(true);
+  const int s0 = (key_beg & ~(kOwnStep - 1)) + kOwnStep * wave;
+  Pages pg = pages_of(s0);
+  for (int k0 = s0; k0 < key_end; k0 += kOwnStep * kWaves) {
     if constexpr (Eb == 2) {
-      dma32(false, k0, key_end, 0, lds0 + (uint32_t)(wave * 2 * L::kOwn) * 2);
-      dma32(true, k0, key_end, 0, lds0 + (uint32_t)(wave * 2 * L::kOwn + L::kOwn) * 2);
+      const uint32_t dst = lds0 + (uint32_t)(wave * 2 * L::kOwn) * 2;
+      dma32(tk, pg, k0, key_end, 0, dst);
+      dma32(tv, pg, k0, key_end, 0, dst + L::kOwn * 2);
+      pg = pages_of(k0 + kOwnStep * kWaves);
       __builtin_amdgcn_s_waitcnt(kVm0);
       asm volatile("" ::: "memory");
     } else {
       u32x4_t kr[kLoads32], vr[kLoads32];
-      load32(false, k0, key_end, kr);
-      load32(true, k0, key_end, vr);
+      load32(tk, pg, k0, key_end, kr);
+      load32(tv, pg, k0, key_end, vr);
+      pg = pages_of(k0 + kOwnStep * kWaves);
       put32(kr, 0, kown);
       put32(vr, 0, vown);
     }
