@@ -515,7 +515,7 @@ int32_t check_shared(const ifa4_args* a, const ifa4_paged_kv* kv, const ifa4_sha
 
 ifa4::SharedPlan shared_plan(const ifa4_args* a, const ifa4_shared_prefix* sp) {
   return ifa4::shared_plan(a->batch, a->kv_heads, a->n_heads / a->kv_heads, sp->prefix_len,
-                           a->max_seqlen_k);
+                           a->max_seqlen_k, ifa4::kSharedSlots);
 }
 
 // Workspace: O of every part and query head, then their maxima and sums.
@@ -537,7 +537,7 @@ int32_t run_shared(const ifa4_args* a, const ifa4_paged_kv* kv, const ifa4_share
   if (l.total() > 0 && (workspace == nullptr || workspace_bytes < (size_t)l.total() ||
                         !aligned(workspace, 256)))
     return IFA4_EWORKSPACE;
-  if (pl.prefix_blocks + (int64_t)a->batch * a->kv_heads * pl.own_chunks > INT32_MAX)
+  if (pl.prefix_blocks + (int64_t)a->batch * a->kv_heads * pl.own_chunks > (1 << 30))
     return IFA4_EUNSUPPORTED;
   ifa4::SharedParams p{};
   p.q = a->q;
@@ -584,9 +584,15 @@ int32_t run_shared(const ifa4_args* a, const ifa4_paged_kv* kv, const ifa4_share
   p.prefix_chunks = (int32_t)pl.prefix_chunks;
   p.row_tiles = (int32_t)pl.row_tiles;
   p.prefix_blocks = (int32_t)pl.prefix_blocks;
-  p.own_keys = (int32_t)pl.own_keys;
   p.own_chunks = (int32_t)pl.own_chunks;
+  p.own_pieces = (int32_t)((int64_t)a->batch * a->kv_heads * pl.own_chunks);
   p.kv_fp8 = qt != nullptr ? 1 : 0;
+  p.by_tiles = ifa4::FastDiv::of(pl.row_tiles);
+  p.by_kv = ifa4::FastDiv::of(p.kv_heads);
+  p.by_batch = ifa4::FastDiv::of(p.batch);
+  p.by_group = ifa4::FastDiv::of(p.group);
+  p.by_heads = ifa4::FastDiv::of(p.n_heads);
+  p.by_chunk = ifa4::FastDiv::of(pl.chunk_keys);
   p.scale = qt != nullptr ? a->softmax_scale * qt->k_scale : a->softmax_scale;
   p.v_scale = qt != nullptr ? qt->v_scale : 1.f;
   const hipError_t e = ifa4::launch_decode_shared(p, a->head_dim, a->qkv_dtype,

@@ -150,6 +150,19 @@ struct NormRopeGrad {
   float* partial;  // [norm_rope_bwd_rows][2][head_dim], or NULL without weights
 };
 
+// n / d for 32-bit n by a multiplication: magic = floor(2^32 / d) gives the quotient or one less.
+struct FastDiv {
+  uint32_t magic, d;
+  static FastDiv of(int64_t d) {
+    const uint64_t m = (uint64_t(1) << 32) / (uint64_t)d;
+    return FastDiv{m > 0xffffffffu ? 0xffffffffu : (uint32_t)m, (uint32_t)d};
+  }
+  __host__ __device__ uint32_t div(uint32_t n) const {
+    const uint32_t q = (uint32_t)(((uint64_t)n * magic) >> 32);
+    return q + (n - q * d >= d ? 1u : 0u);
+  }
+};
+
 // Paged decode behind a prefix that the whole batch shares (decode_shared.hip).
 struct SharedParams {
   const void* q;
@@ -176,13 +189,16 @@ struct SharedParams {
   int32_t prefix_chunks;
   int32_t row_tiles;       // prefix workgroups side by side over batch * group rows
   int32_t prefix_blocks;   // workgroups of the prefix, all XCDs' shares alike
-  int32_t own_keys;        // keys of an own workgroup
-  int32_t own_chunks;
+  int32_t own_chunks;      // pieces of a (sequence, kv head)'s own keys
+  int32_t own_pieces;      // batch * kv_heads * own_chunks
   int32_t kv_fp8;
+  FastDiv by_tiles, by_kv, by_batch, by_group, by_heads, by_chunk;  // divisions by row_tiles,
+                           // kv_heads, batch, group, n_heads, chunk_keys
   float scale;             // softmax_scale (times the K scale of an e4m3 cache)
   float v_scale;
 };
-constexpr int kSharedTile = 64, kSharedRows = 128, kSharedOwnStep = 128;
+constexpr int kSharedTile = 64, kSharedRows = 128, kSharedOwnRound = 128;
+constexpr int kSharedSlots = 512;  // resident workgroups, two a CU
 hipError_t launch_decode_shared(const SharedParams& p, int head_dim, int qkv_dtype,
                                 hipStream_t stream);
 

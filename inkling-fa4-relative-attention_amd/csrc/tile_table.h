@@ -441,31 +441,63 @@ inline PrefillSplit prefill_split_for(int64_t batch, int64_t n_heads, int64_t ma
   return s;
 }
 
-// Decode behind a shared prefix (decode_shared.hip): how the prefix and the sequences' own
-// keys are cut into workgroups of 128 rows x chunk_keys, and (sequence, kv head) x own_keys.
+// Decode behind a shared prefix (decode_shared.hip): how the prefix is cut into pieces of 128 rows
+// x chunk_keys, and each (sequence, kv head)'s own keys into own_chunks pieces.
 struct SharedPlan {
-  int64_t prefix_keys;  // of the prefix that goes through its workgroups: whole 64-key tiles
-  int64_t chunk_keys, prefix_chunks, row_tiles, prefix_blocks, own_keys, own_chunks;
+  int64_t prefix_keys;  // of the prefix that goes through its pieces: whole 64-key tiles
+  int64_t chunk_keys, prefix_chunks, row_tiles, prefix_blocks, own_chunks;
 };
-constexpr int64_t kSharedSlots = 512;     // resident workgroups
-constexpr int64_t kSharedMinTiles = 4;    // shortest prefix chunk
-constexpr int64_t kSharedOwnKeys = 512;
+// Cycles, measured inside the kernel (d 128, two workgroups on a CU): a prefix piece without its
+// tiles (rows, first tile, the part's way out), a tile, a part's share of the merge; an own piece
+// without its rounds, and a round of its waves (128 keys).
+constexpr int64_t kSharedPiece = 13000, kSharedTileCost = 4000, kSharedPart = 70;
+constexpr int64_t kSharedOwnPiece = 7000, kSharedOwnRoundCost = 7000;
 inline SharedPlan shared_plan(int64_t batch, int64_t kv_heads, int64_t group, int64_t prefix_len,
-                              int64_t max_seqlen_k) {
+                              int64_t max_seqlen_k, int64_t slots) {
   SharedPlan s{};
   const int64_t shared = prefix_len < max_seqlen_k ? prefix_len : max_seqlen_k;
   const int64_t tiles = shared / 64;
   s.prefix_keys = tiles * 64;
   s.row_tiles = (batch * group + 127) / 128;
-  const int64_t side = s.row_tiles * kv_heads;  // workgroups of one chunk
-  int64_t chunks = side < kSharedSlots ? kSharedSlots / side : 1;
-  int64_t chunk = (tiles + chunks - 1) / chunks;
-  if (chunk < kSharedMinTiles) chunk = kSharedMinTiles;
+  const int64_t side = s.row_tiles * kv_heads;  // pieces of one chunk
+  // own keys: rounds of 128 keys, lengths taken as three quarters of the longest
+  const int64_t rounds = (max_seqlen_k - s.prefix_keys + 127) / 128, segments = batch * kv_heads;
+  auto own_chunks = [&](int64_t room) {
+    const int64_t own = (room + segments - 1) / segments;
+    return own < rounds ? own : rounds;
+  };
+  auto own_cost = [&](int64_t own, int64_t room) {
+    const int64_t each = (rounds + own - 1) / own;
+    return (segments * own + room - 1) / room *
+           (kSharedOwnPiece + each * kSharedOwnRoundCost * 3 / 4);
+  };
+  // The chunk length of least cost, from the one that fills the slots on; own pieces run beside
+  // the prefix's where those leave room, else after them.
+  const int64_t most = side < slots ? slots / side : 1;
+  int64_t best = -1, chunk = 1;
+  s.own_chunks = rounds > 0 ? own_chunks(slots) : 0;
+  for (int64_t t = (tiles + most - 1) / most; t > 0 && t <= tiles; t += t / 4 + 1) {
+    const int64_t pieces = (tiles + t - 1) / t * side;
+    const int64_t prefix = (pieces + slots - 1) / slots * (kSharedPiece + t * kSharedTileCost);
+    int64_t own = 0, cost = prefix;
+    if (rounds > 0) {
+      const int64_t room = pieces < slots ? slots - pieces : slots;
+      own = own_chunks(room);
+      const int64_t c = own_cost(own, room);
+      cost = pieces >= slots ? prefix + c : c > prefix ? c : prefix;
+    }
+    cost += pieces * kSharedPart;
+    if (best < 0 || cost < best) {
+      best = cost;
+      chunk = t;
+      s.own_chunks = own;
+    } else if (2 * best < prefix) {
+      break;
+    }
+  }
   s.chunk_keys = chunk * 64;
   s.prefix_chunks = (tiles + chunk - 1) / chunk;
   s.prefix_blocks = (s.prefix_chunks * kv_heads + 7) / 8 * 8 * s.row_tiles;
-  s.own_keys = kSharedOwnKeys;
-  s.own_chunks = (max_seqlen_k - s.prefix_keys + s.own_keys - 1) / s.own_keys;
   return s;
 }
 

@@ -24,10 +24,12 @@ using ifa4_torch::check_status;
 using ifa4_torch::dtype_code;
 using ifa4_torch::empty_on;
 
+// k and v: [tokens, heads, dim], or with `paged` the pools [blocks, rows, heads, dim].
 ifa4_args make_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                     const at::Tensor& rel, const at::Tensor& cu_q, const at::Tensor& cu_k,
                     int64_t max_q, int64_t max_k, int64_t rel_extent, bool causal,
-                    int64_t window_left, double softmax_scale, int64_t flags) {
+                    int64_t window_left, double softmax_scale, int64_t flags, bool paged = false) {
+  const int64_t at = paged ? 1 : 0;  // dimension of k and v that holds the tokens
   TORCH_CHECK(q.is_cuda() && k.is_cuda() && v.is_cuda() && rel.is_cuda() && cu_q.is_cuda() &&
                   cu_k.is_cuda(),
               "inkling_fa4: every tensor must be on the GPU");
@@ -35,16 +37,16 @@ ifa4_args make_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& 
   TORCH_CHECK(k.device() == dev && v.device() == dev && rel.device() == dev &&
                   cu_q.device() == dev && cu_k.device() == dev,
               "inkling_fa4: tensors must be on one device");
-  TORCH_CHECK(q.dim() == 3 && k.dim() == 3 && v.dim() == 3 && rel.dim() == 3,
+  TORCH_CHECK(q.dim() == 3 && k.dim() == 3 + at && v.dim() == 3 + at && rel.dim() == 3,
               "inkling_fa4: q, k, v, rel_logits must be 3-D [tokens, heads, dim]");
   TORCH_CHECK(k.sizes() == v.sizes(), "inkling_fa4: k and v shapes differ");
-  TORCH_CHECK(q.size(2) == k.size(2), "inkling_fa4: q and k head_dim differ");
+  TORCH_CHECK(q.size(2) == k.size(at + 2), "inkling_fa4: q and k head_dim differ");
   TORCH_CHECK(rel.size(0) == q.size(0) && rel.size(1) == q.size(1),
               "inkling_fa4: rel_logits must be [total_q, n_heads, >= rel_extent]");
   const bool kv_fp8 = k.scalar_type() == at::kFloat8_e4m3fn;
   TORCH_CHECK(k.scalar_type() == v.scalar_type() && (kv_fp8 || q.scalar_type() == k.scalar_type()),
               "inkling_fa4: q, k, v dtypes differ (k/v may both be float8_e4m3fn in decode)");
-  TORCH_CHECK(q.stride(2) == 1 && k.stride(2) == 1 && v.stride(2) == 1 && rel.stride(2) == 1,
+  TORCH_CHECK(q.stride(2) == 1 && k.stride(at + 2) == 1 && v.stride(at + 2) == 1 && rel.stride(2) == 1,
               "inkling_fa4: the last dim of q, k, v, rel_logits must be contiguous");
   TORCH_CHECK(cu_q.scalar_type() == at::kInt && cu_k.scalar_type() == at::kInt,
               "inkling_fa4: cu_seqlens must be int32");
@@ -69,17 +71,17 @@ ifa4_args make_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& 
   a.cu_seqlens_k = cu_k.data_ptr<int32_t>();
   a.q_stride_t = q.stride(0);
   a.q_stride_h = q.stride(1);
-  a.k_stride_t = k.stride(0);
-  a.k_stride_h = k.stride(1);
-  a.v_stride_t = v.stride(0);
-  a.v_stride_h = v.stride(1);
+  a.k_stride_t = k.stride(at);
+  a.k_stride_h = k.stride(at + 1);
+  a.v_stride_t = v.stride(at);
+  a.v_stride_h = v.stride(at + 1);
   a.rel_stride_t = rel.stride(0);
   a.rel_stride_h = rel.stride(1);
   a.total_q = q.size(0);
-  a.total_k = k.size(0);
+  a.total_k = paged ? 0 : k.size(0);
   a.batch = static_cast<int32_t>(cu_q.numel() - 1);
   a.n_heads = static_cast<int32_t>(q.size(1));
-  a.kv_heads = static_cast<int32_t>(k.size(1));
+  a.kv_heads = static_cast<int32_t>(k.size(at + 1));
   a.head_dim = static_cast<int32_t>(q.size(2));
   a.rel_extent = static_cast<int32_t>(rel_extent);
   a.rel_width = static_cast<int32_t>(rel.size(2));
@@ -222,8 +224,8 @@ std::tuple<at::Tensor, at::Tensor> decode(const at::Tensor& q, const at::Tensor&
   return {out, lse};
 }
 
-// A paged cache's checks and description: the ABI arguments of the call over the first
-// block's rows (which carry the row / head strides), with the pool as k and v, and *kv.
+// A paged cache's checks and description: the ABI arguments of the call, with the pool as k
+// and v, and *kv.
 ifa4_args paged_args(const char* op, const at::Tensor& q, const at::Tensor& k_cache,
                      const at::Tensor& v_cache, const at::Tensor& rel, const at::Tensor& cu_q,
                      const at::Tensor& seqused_k, const at::Tensor& block_table, int64_t max_q,
@@ -245,14 +247,10 @@ ifa4_args paged_args(const char* op, const at::Tensor& q, const at::Tensor& k_ca
               "inkling_fa4.", op, ": seqused_k must be 1-D contiguous");
   TORCH_CHECK(block_table.size(0) == cu_q.numel() - 1 && seqused_k.numel() == cu_q.numel() - 1,
               "inkling_fa4.", op, ": block_table / seqused_k need one row per sequence");
-  const at::Tensor k_rows = k_cache.select(0, 0);
-  const at::Tensor v_rows = v_cache.select(0, 0);
-  ifa4_args a = make_args(q, k_rows, v_rows, rel, cu_q, cu_q, max_q, max_k, rel_extent, causal,
-                          window_left, softmax_scale, flags);
-  a.k = k_cache.data_ptr();
-  a.v = v_cache.data_ptr();
+  TORCH_CHECK_INDEX(k_cache.size(0) > 0, "inkling_fa4.", op, ": the pool has no blocks");
+  ifa4_args a = make_args(q, k_cache, v_cache, rel, cu_q, cu_q, max_q, max_k, rel_extent, causal,
+                          window_left, softmax_scale, flags, true);
   a.cu_seqlens_k = nullptr;
-  a.total_k = 0;
   *kv = ifa4_paged_kv{};
   kv->struct_size = sizeof(ifa4_paged_kv);
   kv->block_size = static_cast<int32_t>(k_cache.size(1));
