@@ -30,6 +30,7 @@ namespace ifa4 {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kAhead = 4;  // rows a lane group has in flight
 
 template <int D>
 struct RowShape {
@@ -72,12 +73,29 @@ __device__ __forceinline__ u32x4_t pack8(const float* f) {
                  Elem<Tag>::pack2(f[4], f[5]), Elem<Tag>::pack2(f[6], f[7])};
 }
 
-// Element i of a norm weight (dtype: ifa4_dtype) as fp32; 1 without a weight.
-__device__ __forceinline__ float weight_at(const void* w, int dtype, int i) {
-  if (w == nullptr) return 1.f;
-  if (dtype == 2) return static_cast<const float*>(w)[i];
-  const uint32_t b = static_cast<const uint16_t*>(w)[i];
-  return dtype == 0 ? __uint_as_float(b << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)b);
+// Elements i to i + 7 of a norm weight (dtype: ifa4_dtype) as fp32; 1 without a weight.  A
+// weight is aligned to its elements only.
+template <typename T>
+struct __attribute__((packed, aligned(2))) Loose {
+  T v;
+};
+__device__ __forceinline__ void weights8(const void* w, int dtype, int i, float* f) {
+  if (w == nullptr) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = 1.f;
+  } else if (dtype == 2) {
+    const auto* at = reinterpret_cast<const Loose<f32x4_t>*>(static_cast<const float*>(w) + i);
+    const f32x4_t a = at[0].v, b = at[1].v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = e < 4 ? a[e] : b[e - 4];
+  } else {
+    const u32x4_t a =
+        reinterpret_cast<const Loose<u32x4_t>*>(static_cast<const uint16_t*>(w) + i)->v;
+    if (dtype == 0)
+      unpack8<Bf16Tag>(a, f);
+    else
+      unpack8<F16Tag>(a, f);
+  }
 }
 
 // Where the elements of a lane turn: the partner lane's distance (half-split) and the
@@ -145,14 +163,18 @@ __device__ __forceinline__ u32x4_t partners(u32x4_t w, const Turn& t, int lane) 
   return r;
 }
 
-// A and B of the lane's elements for one weight.
+// A and B of the lane's elements for one weight: w and, at the partners, w'.
 template <bool kPairs>
-__device__ __forceinline__ void coefficients(const float* w, const float* wp, const float* cs,
+__device__ __forceinline__ void coefficients(const NormRopeParams& p, const void* weight,
+                                             const Turn& t, int c, const float* cs,
                                              const float* sn, float* a, float* b) {
+  float w[8], wp[8];
+  weights8(weight, p.w_dtype, 8 * c, w);
+  if constexpr (!kPairs) weights8(weight, p.w_dtype, 8 * (c + t.hop), wp);
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     a[e] = w[e] * cs[e];
-    b[e] = wp[e] * sn[e];
+    b[e] = (kPairs ? w[e ^ 1] : wp[e]) * sn[e];
   }
 }
 
@@ -237,6 +259,27 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(NormRopeParams p, A
   const int t = in ? (int)t64 : (int)p.total - 1;  // idle groups follow the last token, and store nothing
   const Turn turn = turn_of<kPairs>(p, c);
 
+  const int hq = p.n_heads, hk = hq + p.kv_heads;
+  const int h_end = min((int)(blockIdx.y + 1) * p.heads_per, kCache != 0 ? hk + p.kv_heads : hk);
+  const int64_t lane_q = t * p.q_st + 8 * c, lane_k = t * p.k_st + 8 * c;
+  const int64_t lane_v = kCache != 0 ? t * ap.v_st + 8 * c : 0;
+  auto load = [&](int h, u32x4_t* raw) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int g = h + i;
+      if (g >= h_end) continue;
+      if (g < hq)
+        raw[i] = ld_global_16(static_cast<const uint16_t*>(p.q) + lane_q + g * p.q_sh);
+      else if (g < hk)
+        raw[i] = ld_global_16(static_cast<const uint16_t*>(p.k) + lane_k + (g - hq) * p.k_sh);
+      else if constexpr (kCache != 0)
+        raw[i] = ld_global_16(static_cast<const uint16_t*>(ap.v) + lane_v + (g - hk) * ap.v_sh);
+    }
+  };
+  int h = (int)blockIdx.y * p.heads_per;
+  u32x4_t raw[kAhead] = {};
+  load(h, raw);  // on their way while the position is looked up
+
   Slot slot{};
   int pos = 0;
   if constexpr (kCache != 0) {
@@ -245,80 +288,70 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(NormRopeParams p, A
   } else if (p.positions != nullptr) {
     pos = p.positions[t];
   }
-  float cs[8], sn[8];
-  angles<kPairs>(p, turn, pos, cs, sn);
   float aq[8], bq[8], ak[8], bk[8];
   {
-    float w[8], wp[8];
-    const int cp = c + turn.hop;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      w[e] = weight_at(p.q_weight, p.w_dtype, 8 * c + e);
-      wp[e] = weight_at(p.q_weight, p.w_dtype, kPairs ? 8 * c + (e ^ 1) : 8 * cp + e);
-    }
-    coefficients<kPairs>(w, wp, cs, sn, aq, bq);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      w[e] = weight_at(p.k_weight, p.w_dtype, 8 * c + e);
-      wp[e] = weight_at(p.k_weight, p.w_dtype, kPairs ? 8 * c + (e ^ 1) : 8 * cp + e);
-    }
-    coefficients<kPairs>(w, wp, cs, sn, ak, bk);
+    float cs[8], sn[8];
+    angles<kPairs>(p, turn, pos, cs, sn);
+    coefficients<kPairs>(p, p.q_weight, turn, c, cs, sn, aq, bq);
+    coefficients<kPairs>(p, p.k_weight, turn, c, cs, sn, ak, bk);
   }
+  const bool stores = in && (kCache == 0 || slot.covered);
 
-  const int hq = p.n_heads, hk = hq + p.kv_heads;
-  const int h_end = min((int)(blockIdx.y + 1) * p.heads_per, kCache != 0 ? hk + p.kv_heads : hk);
-  auto row_in = [&](int h) -> const uint16_t* {
-    const uint16_t* base = h < hq ? static_cast<const uint16_t*>(p.q) + t * p.q_st + h * p.q_sh
-                           : h < hk
-                               ? static_cast<const uint16_t*>(p.k) + t * p.k_st + (h - hq) * p.k_sh
-                               : static_cast<const uint16_t*>(ap.v) + t * ap.v_st + (h - hk) * ap.v_sh;
-    return base + 8 * c;
-  };
-  auto put = [&](int h, u32x4_t raw) {
-    const bool is_q = h < hq, is_v = kCache != 0 && h >= hk;
-    float x[8], px[8], y[8];
-    unpack8<Tag>(raw, x);
-    const u32x4_t praw = partners<kPairs>(raw, turn, lane);
-    unpack8<Tag>(praw, px);
+  auto turned = [&](u32x4_t w, const float* a, const float* b, bool norm, float* y) {
+    float x[8], px[8];
+    unpack8<Tag>(w, x);
+    unpack8<Tag>(partners<kPairs>(w, turn, lane), px);
     float ss = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
     ss = row_sum<kLpr>(ss);
-    const bool norm = !is_v && (is_q ? p.q_weight : p.k_weight) != nullptr;
-    const float r = norm ? 1.f / sqrtf(ss * (1.f / D) + p.eps) : 1.f;
+    const float r = norm ? rsqrtf(ss * (1.f / D) + p.eps) : 1.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float a = is_q ? aq[e] : ak[e], b = is_q ? bq[e] : bk[e];
-      y[e] = is_v ? x[e] : r * fmaf(x[e], a, px[e] * b);
-    }
-    if (!in || (kCache != 0 && !slot.covered)) return;
-    if (kCache == 0 || is_q) {
-      uint16_t* dst = is_q ? static_cast<uint16_t*>(p.q_out) + t * p.qo_st + h * p.qo_sh
-                           : static_cast<uint16_t*>(p.k_out) + t * p.ko_st + (h - hq) * p.ko_sh;
-      *reinterpret_cast<u32x4_t*>(dst + 8 * c) = pack8<Tag>(y);
-      return;
-    }
-    if (slot.row < 0) return;
-    const int64_t at = is_v ? slot.block * ap.vc_sblk + slot.row * ap.vc_st + (h - hk) * ap.vc_sh
-                            : slot.block * ap.kc_sblk + slot.row * ap.kc_st + (h - hq) * ap.kc_sh;
+    for (int e = 0; e < 8; ++e) y[e] = r * fmaf(x[e], a[e], px[e] * b[e]);
+  };
+  auto put_cache = [&](void* cache, int64_t at, const float* y, float mul, u32x4_t raw16) {
     if constexpr (kCache == 1) {
-      uint16_t* dst = static_cast<uint16_t*>(is_v ? ap.v_cache : ap.k_cache) + at;
-      *reinterpret_cast<u32x4_t*>(dst + 8 * c) = is_v ? raw : pack8<Tag>(y);
-    } else if constexpr (kCache == 2) {
-      const float mul = is_v ? ap.inv_v_scale : ap.inv_k_scale;
+      *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(cache) + at + 8 * c) = raw16;
+    } else {
+      float z[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] *= mul;
-      uint8_t* dst = static_cast<uint8_t*>(is_v ? ap.v_cache : ap.k_cache) + at;
-      *reinterpret_cast<u32x2_t*>(dst + 8 * c) = pack_fp8(y);
+      for (int e = 0; e < 8; ++e) z[e] = y[e] * mul;
+      *reinterpret_cast<u32x2_t*>(static_cast<uint8_t*>(cache) + at + 8 * c) = pack_fp8(z);
     }
   };
-  for (int h = (int)blockIdx.y * p.heads_per; h < h_end; h += 2) {
-    const u32x4_t r0 = ld_global_16(row_in(h));
-    const bool two = h + 1 < h_end;
-    u32x4_t r1{};
-    if (two) r1 = ld_global_16(row_in(h + 1));
-    put(h, r0);
-    if (two) put(h + 1, r1);
+  auto put = [&](int g, u32x4_t w) {
+    float y[8];
+    if (g < hq) {
+      turned(w, aq, bq, p.q_weight != nullptr, y);
+      uint16_t* dst = static_cast<uint16_t*>(p.q_out) + t * p.qo_st + g * p.qo_sh + 8 * c;
+      if (stores) *reinterpret_cast<u32x4_t*>(dst) = pack8<Tag>(y);
+    } else if (g < hk) {
+      turned(w, ak, bk, p.k_weight != nullptr, y);
+      if constexpr (kCache == 0) {
+        uint16_t* dst = static_cast<uint16_t*>(p.k_out) + t * p.ko_st + (g - hq) * p.ko_sh + 8 * c;
+        if (stores) *reinterpret_cast<u32x4_t*>(dst) = pack8<Tag>(y);
+      } else if (stores && slot.row >= 0) {
+        put_cache(ap.k_cache, slot.block * ap.kc_sblk + slot.row * ap.kc_st + (g - hq) * ap.kc_sh, y,
+                  ap.inv_k_scale, pack8<Tag>(y));
+      }
+    } else if constexpr (kCache != 0) {
+      if (!stores || slot.row < 0) return;
+      unpack8<Tag>(w, y);
+      put_cache(ap.v_cache, slot.block * ap.vc_sblk + slot.row * ap.vc_st + (g - hk) * ap.vc_sh, y,
+                ap.inv_v_scale, w);
+    }
+  };
+  while (true) {
+    u32x4_t next[kAhead] = {};
+    const bool more = h + kAhead < h_end;
+    if (more) load(h + kAhead, next);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (h + i < h_end) put(h + i, raw[i]);
+    if (!more) break;
+    h += kAhead;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) raw[i] = next[i];
   }
 }
 
@@ -332,13 +365,9 @@ __global__ __launch_bounds__(kThreads) void norm_rope_bwd_kernel(NormRopeParams 
   __shared__ float sums[S::kPerBlock][2][D];
   const int lane = threadIdx.x & 63, c = lane % kLpr, grp = threadIdx.x / kLpr;
   const Turn turn = turn_of<kPairs>(p, c);
-  float wq[8], wk[8], dwq[8], dwk[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    wq[e] = weight_at(p.q_weight, p.w_dtype, 8 * c + e);
-    wk[e] = weight_at(p.k_weight, p.w_dtype, 8 * c + e);
-    dwq[e] = dwk[e] = 0.f;
-  }
+  float wq[8], wk[8], dwq[8] = {}, dwk[8] = {};
+  weights8(p.q_weight, p.w_dtype, 8 * c, wq);
+  weights8(p.k_weight, p.w_dtype, 8 * c, wk);
   const int hq = p.n_heads;
   const int h_beg = g.gq != nullptr ? 0 : hq, h_all = g.gk != nullptr ? hq + p.kv_heads : hq;
   for (int64_t t0 = (int64_t)blockIdx.x * S::kPerBlock; t0 < p.total;
@@ -373,7 +402,7 @@ __global__ __launch_bounds__(kThreads) void norm_rope_bwd_kernel(NormRopeParams 
       ss = row_sum<kLpr>(ss);
       dot = row_sum<kLpr>(dot);
       if ((is_q ? p.q_weight : p.k_weight) != nullptr) {
-        const float r = 1.f / sqrtf(ss * (1.f / D) + p.eps);
+        const float r = rsqrtf(ss * (1.f / D) + p.eps);
         const float f = r * r * r * (1.f / D) * dot;
         const float keep = in ? r : 0.f;
 #pragma unroll
