@@ -3,6 +3,8 @@
 // current stream of the tensors' GPU.
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
 #include <optional>
@@ -191,6 +193,85 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> qk_norm_rope_bwd(
           dkw.defined() ? dkw : none()};
 }
 
+// The operators by name: calls that go on to the kernels, or to whatever a caller put before them.
+template <typename F>
+c10::TypedOperatorHandle<F> operator_named(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
+}
+
+// A gradient as the kernels read it: contiguous last dim, 16-byte rows (an expanded, sliced or
+// shifted one is copied).
+OptTensor gradient_rows(const at::Tensor& g) {
+  if (!g.defined()) return std::nullopt;
+  const bool fine = g.stride(2) == 1 && g.stride(0) % 8 == 0 && g.stride(1) % 8 == 0 &&
+                    reinterpret_cast<uintptr_t>(g.data_ptr()) % 16 == 0;
+  return fine ? g : g.clone(at::MemoryFormat::Contiguous);
+}
+
+// qk_norm_rope in an autograd graph.  It keeps the inputs, nothing else; its gradients have
+// no gradient of their own.
+struct QkNormRope : torch::autograd::Function<QkNormRope> {
+  static torch::autograd::variable_list forward(
+      torch::autograd::AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k,
+      const OptTensor& q_weight, const OptTensor& k_weight, const OptTensor& cos,
+      const OptTensor& sin, const OptTensor& positions, double eps, bool interleaved) {
+    static const auto op = operator_named<decltype(qk_norm_rope)>("inkling_fa4::qk_norm_rope");
+    const at::AutoDispatchBelowADInplaceOrView below;
+    auto [q_out, k_out] =
+        op.call(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved);
+    auto kept = [](const OptTensor& t) { return given(t) ? *t : at::Tensor(); };
+    ctx->save_for_backward(
+        {q, k, kept(q_weight), kept(k_weight), kept(cos), kept(sin), kept(positions)});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->set_materialize_grads(false);
+    return {q_out, k_out};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    static const auto op =
+        operator_named<decltype(qk_norm_rope_bwd)>("inkling_fa4::qk_norm_rope_bwd");
+    const torch::autograd::variable_list saved = ctx->get_saved_variables();
+    bool needs[4];
+    size_t edge = 0;  // only tensors that were given have an edge
+    for (int i = 0; i < 4; ++i) needs[i] = saved[i].defined() && ctx->needs_input_grad(edge++);
+    torch::autograd::variable_list out(9);
+    const OptTensor gq = gradient_rows(needs[0] || needs[2] ? grads[0] : at::Tensor());
+    const OptTensor gk = gradient_rows(needs[1] || needs[3] ? grads[1] : at::Tensor());
+    if (!given(gq) && !given(gk)) return out;
+    auto maybe = [&](int i) { return saved[i].defined() ? OptTensor(saved[i]) : std::nullopt; };
+    std::optional<at::AutoDispatchBelowADInplaceOrView> below;
+    if (!at::GradMode::is_enabled()) below.emplace();
+    auto [dq, dk, dqw, dkw] =
+        op.call(gq, gk, saved[0], saved[1], maybe(2), maybe(3), maybe(4), maybe(5), maybe(6),
+                ctx->saved_data["eps"].toDouble(), ctx->saved_data["interleaved"].toBool());
+    if (needs[0] && given(gq)) out[0] = dq;
+    if (needs[1] && given(gk)) out[1] = dk;
+    if (needs[2] && given(gq)) out[2] = dqw;
+    if (needs[3] && given(gk)) out[3] = dkw;
+    return out;
+  }
+};
+
+std::tuple<at::Tensor, at::Tensor> qk_norm_rope_autograd(
+    const at::Tensor& q, const at::Tensor& k, const OptTensor& q_weight, const OptTensor& k_weight,
+    const OptTensor& cos, const OptTensor& sin, const OptTensor& positions, double eps,
+    bool interleaved) {
+  auto wants = [](const OptTensor& t) { return given(t) && t->requires_grad(); };
+  if (at::GradMode::is_enabled()) {
+    TORCH_CHECK_VALUE(!wants(cos) && !wants(sin),
+                      "inkling_fa4.qk_norm_rope: cos and sin have no gradient");
+    if (wants(q) || wants(k) || wants(q_weight) || wants(k_weight)) {
+      auto out = QkNormRope::apply(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved);
+      return {out[0], out[1]};
+    }
+  }
+  static const auto op = operator_named<decltype(qk_norm_rope)>("inkling_fa4::qk_norm_rope");
+  const at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved);
+}
+
 at::Tensor kv_append_paged(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache,
                            const at::Tensor& v_cache, const at::Tensor& cu_seqlens,
                            const at::Tensor& seqused_k, const at::Tensor& block_table,
@@ -288,4 +369,9 @@ TORCH_LIBRARY_IMPL(inkling_fa4, CUDA, m) {
   m.impl("qk_norm_rope", &qk_norm_rope);
   m.impl("qk_norm_rope_bwd", &qk_norm_rope_bwd);
   m.impl("kv_append_paged", &kv_append_paged);
+}
+
+TORCH_LIBRARY_IMPL(inkling_fa4, Autograd, m) {
+  m.impl("qk_norm_rope", &qk_norm_rope_autograd);
+  m.impl("qk_norm_rope_bwd", torch::autograd::autogradNotImplementedFallback());
 }

@@ -17,7 +17,6 @@ cu_seqlens, seqused_k and block tables stay on the device and are not checked ag
 the contract; what they hold never leads to an access outside the tensors.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
 from ._native import ops as _ops
 
@@ -33,45 +32,6 @@ def _op(name):
 
 def _wants_grad(*tensors):
     return any(getattr(t, "requires_grad", False) for t in tensors)
-
-
-def _rows(g):
-    """A gradient as the kernels read it: contiguous last dim, 16-byte rows (an expanded or
-    sliced one is copied)."""
-    if g is None or (g.stride(2) == 1 and g.stride(0) % 8 == 0 and g.stride(1) % 8 == 0
-                     and g.data_ptr() % 16 == 0):
-        return g
-    return g.contiguous()
-
-
-class _QkNormRope(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
-        out = _op("qk_norm_rope")(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
-        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
-        ctx.settings = (eps, interleaved)
-        ctx.set_materialize_grads(False)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, gq, gk):
-        saved = ctx.saved_tensors
-        q_weight, k_weight = saved[2:4]
-        need_q, need_k, need_qw, need_kw = ctx.needs_input_grad[:4]
-        gq = _rows(gq) if need_q or need_qw else None
-        gk = _rows(gk) if need_k or need_kw else None
-        grads = [None] * 9
-        if gq is None and gk is None:
-            return tuple(grads)
-        dq, dk, dqw, dkw = _op("qk_norm_rope_bwd")(gq, gk, *saved, *ctx.settings)
-        if gq is not None:
-            grads[0] = dq if need_q else None
-            grads[2] = dqw if need_qw and q_weight is not None else None
-        if gk is not None:
-            grads[1] = dk if need_k else None
-            grads[3] = dkw if need_kw and k_weight is not None else None
-        return tuple(grads)
 
 
 def inkling_fa4_qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None,
@@ -90,12 +50,6 @@ def inkling_fa4_qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=N
     """
     if q_weight is None and k_weight is None and cos is None:
         raise ValueError("nothing to do: give a weight, or cos and sin")
-    if torch.is_grad_enabled():
-        if _wants_grad(cos, sin):
-            raise ValueError("cos and sin have no gradient")
-        if _wants_grad(q, k, q_weight, k_weight):
-            return _QkNormRope.apply(q, k, q_weight, k_weight, cos, sin, positions, float(eps),
-                                     bool(interleaved))
     return _op("qk_norm_rope")(q, k, q_weight, k_weight, cos, sin, positions, float(eps),
                                bool(interleaved))
 

@@ -170,6 +170,51 @@ def test_gradients_that_are_expanded_sliced_or_missing(cuda):
     assert torch.equal(got[0], want[3])
 
 
+def test_gradients_that_start_off_a_16_byte_boundary(cuda):
+    """Contiguous gradients at an odd offset are as good as aligned ones."""
+    x = [_dev(t, cuda) for t in _inputs(9, 3, 2, 64, torch.float16, torch.float32, 64, 21)]
+    leaves = [t.clone().requires_grad_() for t in x[:4]]
+    want = torch.autograd.grad(inkling_fa4_qk_norm_rope(*leaves, *x[4:7]), leaves, x[7:])
+
+    def shifted(t):
+        flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=cuda)[1:]
+        return flat.copy_(t.reshape(-1)).view(t.shape)
+    got = torch.autograd.grad(inkling_fa4_qk_norm_rope(*leaves, *x[4:7]), leaves,
+                              [shifted(t) for t in x[7:]])
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize("absent", [(), (2, 3, 4, 5, 6), (2,), (3,), (4, 5, 6)])
+def test_gradients_of_some_inputs(cuda, absent):
+    """Each input's gradient asked for by itself, with weights and tables that are not there,
+    is the one of the full backward pass."""
+    x = [_dev(t, cuda) for t in _inputs(9, 3, 2, 64, torch.bfloat16, torch.float32, 64, 22)]
+    x = [None if i in absent else t for i, t in enumerate(x)]
+    if all(i in absent for i in (2, 3, 4)):
+        x[4:7] = [_dev(t, cuda) for t in _inputs(9, 3, 2, 64, torch.bfloat16, None, 64, 22)[4:7]]
+    here = [i for i in range(4) if x[i] is not None]
+    for i in here:
+        x[i] = x[i].clone().requires_grad_()
+    full = torch.autograd.grad(inkling_fa4_qk_norm_rope(*x[:7]), [x[i] for i in here], x[7:])
+    for i, want in zip(here, full):
+        y = [t if j == i or t is None else t.detach() for j, t in enumerate(x)]
+        for leaves in (x, y):  # one leaf of several, and the only one
+            out = inkling_fa4_qk_norm_rope(*leaves[:7])
+            got, = torch.autograd.grad(out, leaves[i], x[7:])
+            assert torch.equal(got, want), i
+
+
+def test_no_second_derivative(cuda):
+    x = [_dev(t, cuda) for t in _inputs(5, 2, 1, 64, torch.bfloat16, torch.float32, 64, 23)]
+    leaves = [t.clone().requires_grad_() for t in x[:4]]
+    out = inkling_fa4_qk_norm_rope(*leaves, *x[4:7])
+    first = torch.autograd.grad(out, leaves, x[7:], create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(sum(t.float().sum() for t in first), leaves, allow_unused=True)
+    with pytest.raises(ValueError):
+        inkling_fa4_qk_norm_rope(*leaves, x[4].clone().requires_grad_(), *x[5:7])
+
+
 def test_same_bits_every_time(cuda):
     q, k, qw, kw, cos, sin, pos, gq, gk = (
         _dev(x, cuda) for x in _inputs(4099, 8, 2, 128, torch.bfloat16, torch.float32, 128, 9))
