@@ -613,16 +613,30 @@ __global__ __launch_bounds__(kThreads, 2) void decode_shared_kernel(SharedParams
   }
   }
 
-  // ---- own keys: piece i goes to workgroup (prefix_blocks + i) % grid, so that the workgroups
-  // without a prefix piece come first -----------------------------------------------------------------
+  // ---- own keys -----------------------------------------------------------------------------------
+  // The workgroups by rank, those without a prefix piece first: each of these takes own_first
+  // pieces, then all take one after the other.  (Padding of the XCDs' shares makes some workgroups
+  // of the prefix's range idle: the last `pad` of each eight at the range's end.)
   const SharedParams p = fields();
   const int G = p.group;
   const int64_t rows_all = (int64_t)p.batch * p.n_heads;
   uint16_t* const kown = stages + wave * 2 * L::kOwn;
   uint16_t* const vown = kown + L::kOwn;
-  int first = (int)blockIdx.x - p.prefix_blocks;
-  if (first < 0) first += (int)gridDim.x;
-  for (int piece = first; piece < p.own_pieces; piece += (int)gridDim.x) {
+  const int pairs = p.kv_heads * p.prefix_chunks, pad = -pairs & 7;
+  const int idle = (int)gridDim.x - pairs * p.row_tiles;
+  int rank = (int)blockIdx.x - p.prefix_blocks;
+  if (rank < 0) {
+    const uint32_t at8 = blockIdx.x >> 3, group8 = p.by_tiles.div(at8);
+    const int pair = (int)group8 * 8 + (int)(blockIdx.x & 7);
+    const int tile = (int)at8 - (int)group8 * p.row_tiles;
+    rank = pair < pairs ? idle + pair * p.row_tiles + tile
+                        : (int)gridDim.x - p.prefix_blocks + tile * pad + pair - pairs;
+  }
+  const int mine = rank < idle ? p.own_first : 0;
+  for (int i = 0;; ++i) {
+    const int piece = i < mine ? rank + i * idle
+                               : p.own_first * idle + rank + (i - mine) * (int)gridDim.x;
+    if (piece >= p.own_pieces) break;
     const uint32_t each = p.by_kv.div((uint32_t)piece);
     const int kvh = piece - (int)each * p.kv_heads;
     const int chunk = (int)p.by_batch.div(each);

@@ -515,7 +515,7 @@ int32_t check_shared(const ifa4_args* a, const ifa4_paged_kv* kv, const ifa4_sha
 
 ifa4::SharedPlan shared_plan(const ifa4_args* a, const ifa4_shared_prefix* sp) {
   return ifa4::shared_plan(a->batch, a->kv_heads, a->n_heads / a->kv_heads, sp->prefix_len,
-                           a->max_seqlen_k, ifa4::kSharedSlots);
+                           a->max_seqlen_k, a->window_left, a->rel_extent, ifa4::kSharedSlots);
 }
 
 // Workspace: O of every part and query head, then their maxima and sums.
@@ -585,6 +585,7 @@ int32_t run_shared(const ifa4_args* a, const ifa4_paged_kv* kv, const ifa4_share
   p.row_tiles = (int32_t)pl.row_tiles;
   p.prefix_blocks = (int32_t)pl.prefix_blocks;
   p.own_chunks = (int32_t)pl.own_chunks;
+  p.own_first = (int32_t)pl.own_first;
   p.own_pieces = (int32_t)((int64_t)a->batch * a->kv_heads * pl.own_chunks);
   p.kv_fp8 = qt != nullptr ? 1 : 0;
   p.by_tiles = ifa4::FastDiv::of(pl.row_tiles);

@@ -190,6 +190,7 @@ struct SharedParams {
   int32_t row_tiles;       // prefix workgroups side by side over batch * group rows
   int32_t prefix_blocks;   // workgroups of the prefix, all XCDs' shares alike
   int32_t own_chunks;      // pieces of a (sequence, kv head)'s own keys
+  int32_t own_first;       // of them for a workgroup without a prefix piece, ahead of the others
   int32_t own_pieces;      // batch * kv_heads * own_chunks
   int32_t kv_fp8;
   FastDiv by_tiles, by_kv, by_batch, by_group, by_heads, by_chunk;  // divisions by row_tiles,

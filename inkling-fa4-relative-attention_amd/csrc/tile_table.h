@@ -442,59 +442,80 @@ inline PrefillSplit prefill_split_for(int64_t batch, int64_t n_heads, int64_t ma
 }
 
 // Decode behind a shared prefix (decode_shared.hip): how the prefix is cut into pieces of 128 rows
-// x chunk_keys, and each (sequence, kv head)'s own keys into own_chunks pieces.
+// x chunk_keys, and each (sequence, kv head)'s own keys into own_chunks pieces; own_first: pieces of
+// own keys that a workgroup without a prefix piece takes before the others take one.
 struct SharedPlan {
   int64_t prefix_keys;  // of the prefix that goes through its pieces: whole 64-key tiles
-  int64_t chunk_keys, prefix_chunks, row_tiles, prefix_blocks, own_chunks;
+  int64_t chunk_keys, prefix_chunks, row_tiles, prefix_blocks, own_chunks, own_first;
 };
 // Cycles, measured inside the kernel (d 128, two workgroups on a CU): a prefix piece without its
-// tiles (rows, first tile, the part's way out), a tile, a part's share of the merge; an own piece
-// without its rounds, and a round of its waves (128 keys).
+// tiles (rows, first tile, the part's way out), a tile (a quarter more with a bias), a part's share
+// of the merge, a piece that a window hides; an own piece without its rounds, and a round of its
+// waves (128 keys).
 constexpr int64_t kSharedPiece = 13000, kSharedTileCost = 4000, kSharedPart = 70;
+constexpr int64_t kSharedHidden = 8000;
 constexpr int64_t kSharedOwnPiece = 7000, kSharedOwnRoundCost = 7000;
 inline SharedPlan shared_plan(int64_t batch, int64_t kv_heads, int64_t group, int64_t prefix_len,
-                              int64_t max_seqlen_k, int64_t slots) {
+                              int64_t max_seqlen_k, int64_t window_left, int64_t rel_extent,
+                              int64_t slots) {
   SharedPlan s{};
   const int64_t shared = prefix_len < max_seqlen_k ? prefix_len : max_seqlen_k;
   const int64_t tiles = shared / 64;
   s.prefix_keys = tiles * 64;
   s.row_tiles = (batch * group + 127) / 128;
   const int64_t side = s.row_tiles * kv_heads;  // pieces of one chunk
+  const bool window = window_left >= 0 && window_left / 64 + 2 < tiles;
+  const int64_t seen = window ? window_left / 64 + 2 : tiles;  // tiles that a row meets at most
+  const int64_t band = (rel_extent + 63) / 64 < tiles ? (rel_extent + 63) / 64 : tiles;  // with bias
   // own keys: rounds of 128 keys, lengths taken as three quarters of the longest
   const int64_t rounds = (max_seqlen_k - s.prefix_keys + 127) / 128, segments = batch * kv_heads;
-  auto own_chunks = [&](int64_t room) {
-    const int64_t own = (room + segments - 1) / segments;
-    return own < rounds ? own : rounds;
-  };
-  auto own_cost = [&](int64_t own, int64_t room) {
-    const int64_t each = (rounds + own - 1) / own;
-    return (segments * own + room - 1) / room *
-           (kSharedOwnPiece + each * kSharedOwnRoundCost * 3 / 4);
-  };
-  // The chunk length of least cost, from the one that fills the slots on; own pieces run beside
-  // the prefix's where those leave room, else after them.
-  const int64_t most = side < slots ? slots / side : 1;
+  const int64_t most_own = rounds < 1 ? 0 : rounds < 64 ? rounds : 64;
+  // The cut of least cost, from the chunk length that fills the slots on (with a window four times
+  // as many pieces, most of them hidden).  Own pieces run beside the prefix's on the workgroups
+  // that have none of it, then after them on all.
+  const int64_t fill = side < slots ? slots / side * (window ? 4 : 1) : 1;
   int64_t best = -1, chunk = 1;
-  s.own_chunks = rounds > 0 ? own_chunks(slots) : 0;
-  for (int64_t t = (tiles + most - 1) / most; t > 0 && t <= tiles; t += t / 4 + 1) {
-    const int64_t pieces = (tiles + t - 1) / t * side;
-    const int64_t prefix = (pieces + slots - 1) / slots * (kSharedPiece + t * kSharedTileCost);
-    int64_t own = 0, cost = prefix;
-    if (rounds > 0) {
-      const int64_t room = pieces < slots ? slots - pieces : slots;
-      own = own_chunks(room);
-      const int64_t c = own_cost(own, room);
-      cost = pieces >= slots ? prefix + c : c > prefix ? c : prefix;
+  int64_t t = (tiles + fill - 1) / fill;
+  do {
+    const int64_t chunks = t > 0 ? (tiles + t - 1) / t : 0, pieces = chunks * side;
+    const int64_t meet = t > 0 ? (seen + t - 1) / t + (window ? 1 : 0) : 0;
+    const int64_t work = (meet < chunks ? meet : chunks) * side;  // pieces that are not hidden
+    const int64_t idle = work < slots ? slots - work : 0;
+    // the longest piece in quarters of a tile: the last, or the one before it
+    const int64_t last = tiles - (chunks - 1) * t, before = band - last < t ? band - last : t;
+    int64_t quarters = 4 * last + (band < last ? band : last);
+    if (chunks > 1 && quarters < 4 * t + before) quarters = 4 * t + (before > 0 ? before : 0);
+    if (window) quarters = (t < seen ? t : seen) * (band > 0 ? 5 : 4);
+    int64_t prefix = (work + slots - 1) / slots * (kSharedPiece + quarters * kSharedTileCost / 4);
+    if (window) prefix += (pieces - 1) / slots * kSharedHidden;
+    if (t == 0) prefix = 0;
+    for (int64_t own = most_own > 0 ? 1 : 0; own <= most_own;
+         own = 2 * own < most_own || own == most_own ? 2 * own : most_own) {
+      const int64_t total = segments * own;
+      int64_t first = 0, cost = prefix;
+      if (own > 0) {
+        int64_t each = kSharedOwnPiece + (rounds + own - 1) / own * kSharedOwnRoundCost * 3 / 4;
+        // hidden pieces are not known to the launch: they take their turn with the others
+        if (window && total > slots - pieces) each += kSharedHidden;
+        if (idle > 0 && !window) first = prefix / each < total / idle ? prefix / each : total / idle;
+        const int64_t left = total - idle * first;
+        const int64_t beside = (first + (left > 0 ? 1 : 0)) * each;
+        cost = left <= idle ? (beside > prefix ? beside : prefix)
+                            : prefix + (left + slots - 1) / slots * each;
+      }
+      cost += work * kSharedPart + total * group * kSharedPart / 128;
+      if (best < 0 || cost < best) {
+        best = cost;
+        chunk = t;
+        s.own_chunks = own;
+        s.own_first = first;
+      }
+      if (own == 0) break;
     }
-    cost += pieces * kSharedPart;
-    if (best < 0 || cost < best) {
-      best = cost;
-      chunk = t;
-      s.own_chunks = own;
-    } else if (2 * best < prefix) {
-      break;
-    }
-  }
+    if (best <= prefix) break;  // the prefix alone takes as long, and longer from here on
+    t += t / 16 + 1;
+  } while (t <= tiles);
+  if (chunk < 1) chunk = 1;
   s.chunk_keys = chunk * 64;
   s.prefix_chunks = (tiles + chunk - 1) / chunk;
   s.prefix_blocks = (s.prefix_chunks * kv_heads + 7) / 8 * 8 * s.row_tiles;
