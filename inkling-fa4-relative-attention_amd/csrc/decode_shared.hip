@@ -100,6 +100,20 @@ __device__ __forceinline__ int wave_min(int x) {
   return __builtin_amdgcn_readfirstlane(x);
 }
 __device__ __forceinline__ int wave_max(int x) { return -wave_min(-x); }
+template <int kCtrl>
+__device__ __forceinline__ float max_dpp(float x) {
+  const int y = __builtin_amdgcn_mov_dpp(__float_as_int(x), kCtrl, 0xf, 0xf, false);
+  return fmaxf(x, __int_as_float(y));
+}
+__device__ __forceinline__ float wave_max(float x) {
+  x = max_dpp<0x140>(max_dpp<0x141>(max_dpp<0x4e>(max_dpp<0xb1>(x))));
+  const int i = __float_as_int(x);
+  auto r = __builtin_amdgcn_permlane16_swap(i, i, false, false);
+  x = fmaxf(__int_as_float(r[0]), __int_as_float(r[1]));
+  const int j = __float_as_int(x);
+  r = __builtin_amdgcn_permlane32_swap(j, j, false, false);
+  return fmaxf(__int_as_float(r[0]), __int_as_float(r[1]));
+}
 
 // A query row: its sequence's position (keys - 1; -1 without a query or keys) and q / out row.
 struct Row {
@@ -736,12 +750,13 @@ __global__ __launch_bounds__(kThreads, 2) void decode_shared_kernel(SharedParams
 // row's own, and they are read without waiting for its length (a part that is not is left out of the
 // sums): one dependent memory round less.
 template <int D, typename Tag>
-__global__ __launch_bounds__(kMergeThreads) void decode_shared_merge_kernel(SharedParams p) {
+__global__ __launch_bounds__(kMergeThreads, 8) void decode_shared_merge_kernel(SharedParams p) {
   using E = Elem<Tag>;
   constexpr int kTeam = D / 4, kTeams = kMergeThreads / kTeam, kAhead = 8;
   constexpr int kMergeWaves = kMergeThreads / 64;
   __shared__ f32x4_t part_o[kTeams][kTeam];
-  __shared__ float weight[kMergeThreads], wave_m[kMergeWaves], wave_l[kMergeWaves];
+  __shared__ float weight[kMergeThreads], weighted[kMergeThreads], wave_m[kMergeWaves];
+  __shared__ float part_l[kTeams];
   const int row = blockIdx.x;
   const int seq = (int)p.by_heads.div((uint32_t)row), head = row - seq * p.n_heads;
   const int tid = threadIdx.x, c = tid % kTeam, team = tid / kTeam;
@@ -759,7 +774,7 @@ __global__ __launch_bounds__(kMergeThreads) void decode_shared_merge_kernel(Shar
   const int n = p.prefix_chunks + p.own_chunks;
   auto counts = [&](int i) { return (i >= skip && i < np) || (i >= p.prefix_chunks && i < p.prefix_chunks + no); };
   auto reads = [&](int i) { return i < n && (!window || counts(i)); };
-  float m = -INFINITY, l = 0.f;  // alike in all threads
+  float m = -INFINITY, l = 0.f;  // m alike in all threads, l over the team's parts
   f32x4_t acc{};
   for (int base = window ? skip / kMergeThreads * kMergeThreads : 0; base < n; base += kMergeThreads) {
     float2 ml{-INFINITY, 0.f};
@@ -773,9 +788,7 @@ __global__ __launch_bounds__(kMergeThreads) void decode_shared_merge_kernel(Shar
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) rows[j] = load(j);
     if (!counts(base + tid)) ml = float2{-INFINITY, 0.f};
-    float mx = ml.x;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) mx = fmaxf(mx, __shfl_xor(mx, off));
+    const float mx = wave_max(ml.x);
     if (base > 0) __syncthreads();  // the weights of the parts before are read
     if ((tid & 63) == 0) wave_m[tid >> 6] = mx;
     __syncthreads();
@@ -785,14 +798,9 @@ __global__ __launch_bounds__(kMergeThreads) void decode_shared_merge_kernel(Shar
     const float mu = mn == -INFINITY ? 0.f : mn;
     const float wgt = fast_exp2((ml.x - mu) * kLog2e), keep = fast_exp2((m - mu) * kLog2e);
     weight[tid] = wgt;
-    float ls = wgt * ml.y;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) ls += __shfl_xor(ls, off);
-    if ((tid & 63) == 0) wave_l[tid >> 6] = ls;
+    weighted[tid] = wgt * ml.y;
     __syncthreads();
     l *= keep;
-#pragma unroll
-    for (int w = 0; w < kMergeWaves; ++w) l += wave_l[w];
     acc *= keep;
     m = mn;
     for (int j0 = 0; base + kTeams * j0 < n && kTeams * j0 < kMergeThreads; j0 += kAhead) {
@@ -803,7 +811,10 @@ __global__ __launch_bounds__(kMergeThreads) void decode_shared_merge_kernel(Shar
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
         const int i = team + kTeams * (j0 + j);
-        if (i < kMergeThreads && counts(base + i)) acc += weight[i] * rows[j];
+        if (i < kMergeThreads && counts(base + i)) {
+          acc += weight[i] * rows[j];
+          l += weighted[i];
+        }
       }
     }
   }
@@ -818,10 +829,14 @@ __global__ __launch_bounds__(kMergeThreads) void decode_shared_merge_kernel(Shar
     return;
   }
   part_o[team][c] = acc;
+  if (c == 0) part_l[team] = l;
   __syncthreads();
   if (team != 0) return;
 #pragma unroll
-  for (int t = 1; t < kTeams; ++t) acc += part_o[t][c];
+  for (int t = 1; t < kTeams; ++t) {
+    acc += part_o[t][c];
+    l += part_l[t];
+  }
   const float inv = l > 0.f ? p.v_scale / l : 0.f;
   uint16_t* dst = static_cast<uint16_t*>(p.out) + (int64_t)bq.start * p.o_st +
                   (int64_t)head * p.o_sh + 4 * c;
