@@ -348,6 +348,18 @@ at::Tensor kv_append_paged(const at::Tensor& k, const at::Tensor& v, const at::T
   return q_out;
 }
 
+// The append has no gradient: whatever its inputs ask for, its output never requires one.
+at::Tensor kv_append_paged_autograd(
+    const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache, const at::Tensor& v_cache,
+    const at::Tensor& cu_seqlens, const at::Tensor& seqused_k, const at::Tensor& block_table,
+    const OptTensor& q, const OptTensor& q_weight, const OptTensor& k_weight, const OptTensor& cos,
+    const OptTensor& sin, double eps, bool interleaved, double k_scale, double v_scale) {
+  static const auto op = operator_named<decltype(kv_append_paged)>("inkling_fa4::kv_append_paged");
+  const at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(k, v, k_cache, v_cache, cu_seqlens, seqused_k, block_table, q, q_weight, k_weight,
+                 cos, sin, eps, interleaved, k_scale, v_scale);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(inkling_fa4, m) {
@@ -374,4 +386,5 @@ TORCH_LIBRARY_IMPL(inkling_fa4, CUDA, m) {
 TORCH_LIBRARY_IMPL(inkling_fa4, Autograd, m) {
   m.impl("qk_norm_rope", &qk_norm_rope_autograd);
   m.impl("qk_norm_rope_bwd", torch::autograd::autogradNotImplementedFallback());
+  m.impl("kv_append_paged", &kv_append_paged_autograd);
 }

@@ -16,8 +16,6 @@ cos=None: no rotation.  head_dim 64 or 128, bf16 or fp16.  Contents of positions
 cu_seqlens, seqused_k and block tables stay on the device and are not checked against
 the contract; what they hold never leads to an access outside the tensors.
 """
-import torch
-
 from ._native import ops as _ops
 
 _overloads = {}
@@ -28,10 +26,6 @@ def _op(name):
     if op is None:
         op = _overloads[name] = getattr(_ops(), name).default
     return op
-
-
-def _wants_grad(*tensors):
-    return any(getattr(t, "requires_grad", False) for t in tensors)
 
 
 def inkling_fa4_qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=None,
@@ -73,13 +67,7 @@ def inkling_fa4_kv_append_paged(k, v, k_cache, v_cache, cu_seqlens_q, seqused_k,
     scales).  A token with p < 0, past the table or whose table entry lies outside the
     pool is not written; two tokens sent to one row leave one of the two.
     """
-    def call():
-        return _op("kv_append_paged")(k, v, k_cache, v_cache, cu_seqlens_q, seqused_k, block_table,
-                                      q, q_weight, k_weight, cos, sin, float(eps),
-                                      bool(interleaved), float(k_scale), float(v_scale))
-    if torch.is_grad_enabled() and _wants_grad(k, v, q, q_weight, k_weight, k_cache, v_cache):
-        with torch.no_grad():  # no backward: the outputs never require one
-            out = call()
-    else:
-        out = call()
+    out = _op("kv_append_paged")(k, v, k_cache, v_cache, cu_seqlens_q, seqused_k, block_table, q,
+                                 q_weight, k_weight, cos, sin, float(eps), bool(interleaved),
+                                 float(k_scale), float(v_scale))
     return out if q is not None else None
