@@ -147,7 +147,7 @@ struct NormRopeGrad {
   int64_t gq_st, gq_sh, gk_st, gk_sh, dq_st, dq_sh, dk_st, dk_sh;
   void* dq_weight;
   void* dk_weight;
-  float* partial;  // [norm_rope_bwd_rows][2][head_dim], or NULL without weights
+  float* partial;  // [workgroups of the backward pass][2][head_dim], or NULL without weights
 };
 
 // n / d for 32-bit n by a multiplication: magic = floor(2^32 / d) gives the quotient or one less.
@@ -203,9 +203,13 @@ constexpr int kSharedSlots = 512;  // resident workgroups, two a CU
 hipError_t launch_decode_shared(const SharedParams& p, int head_dim, int qkv_dtype,
                                 hipStream_t stream);
 
-// Workgroups of the backward pass at most, each with a row of partial weight gradients.
-constexpr int64_t kNormRopeBwdBlocks = 1024;
-int64_t norm_rope_bwd_rows(int64_t total, int head_dim);
+// Workgroups of the backward pass, over tokens (x) and chunks of heads_per heads (y), each with a
+// row of partial weight gradients.
+struct NormRopeBwdGrid {
+  unsigned x, y;
+  int heads_per;
+};
+NormRopeBwdGrid norm_rope_bwd_grid(int64_t total, int heads, int head_dim);
 // cache: 0 none, 1 of the inputs' type, 2 e4m3
 hipError_t launch_norm_rope(const NormRopeParams& p, const AppendParams& a, int cache, int head_dim,
                             int dtype, hipStream_t stream);

@@ -356,7 +356,7 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(NormRopeParams p, A
 }
 
 // ---- backward -------------------------------------------------------------------------------
-// A workgroup walks over tokens and leaves its sums of the weight gradients in one row of the
+// A workgroup walks over tokens and a chunk of their heads, and leaves its sums of the weight gradients in one row of the
 // workspace, [q or k][D]; the second kernel adds the rows in a fixed order.
 template <int D, typename Tag, bool kPairs>
 __global__ __launch_bounds__(kThreads) void norm_rope_bwd_kernel(NormRopeParams p, NormRopeGrad g) {
@@ -369,7 +369,8 @@ __global__ __launch_bounds__(kThreads) void norm_rope_bwd_kernel(NormRopeParams 
   weights8(p.q_weight, p.w_dtype, 8 * c, wq);
   weights8(p.k_weight, p.w_dtype, 8 * c, wk);
   const int hq = p.n_heads;
-  const int h_beg = g.gq != nullptr ? 0 : hq, h_all = g.gk != nullptr ? hq + p.kv_heads : hq;
+  const int h_beg = max(g.gq != nullptr ? 0 : hq, (int)blockIdx.y * p.heads_per);
+  const int h_all = min(g.gk != nullptr ? hq + p.kv_heads : hq, (int)(blockIdx.y + 1) * p.heads_per);
   for (int64_t t0 = (int64_t)blockIdx.x * S::kPerBlock; t0 < p.total;
        t0 += (int64_t)gridDim.x * S::kPerBlock) {
     const bool in = t0 + grp < p.total;
@@ -440,26 +441,29 @@ __global__ __launch_bounds__(kThreads) void norm_rope_bwd_kernel(NormRopeParams 
     float s = 0.f;
 #pragma unroll
     for (int k = 0; k < S::kPerBlock; ++k) s += sums[k][i / D][i % D];
-    g.partial[(int64_t)blockIdx.x * 2 * D + i] = s;
+    g.partial[((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 * D + i] = s;
   }
 }
 
-// dw of 32 columns of [q or k][D]: 32 threads a column over the partial rows, then in LDS.
+// dw of 32 columns of [q or k][D]: 32 threads a column over the partial rows, then a tree in LDS.
 constexpr int kSumCols = 32, kSumRows = 32;
 __global__ __launch_bounds__(kSumCols * kSumRows) void norm_rope_dw_kernel(NormRopeGrad g,
                                                                            int head_dim, int rows,
                                                                            int w_dtype) {
-  __shared__ float part[kSumRows][kSumCols + 1];
+  __shared__ float part[kSumRows / 2][kSumCols + 1];
   const int col = threadIdx.x % kSumCols, rg = threadIdx.x / kSumCols;
   const int i = blockIdx.x * kSumCols + col;
   float s = 0.f;
 #pragma unroll 8
   for (int r = rg; r < rows; r += kSumRows) s += g.partial[(int64_t)r * 2 * head_dim + i];
-  part[rg][col] = s;
-  __syncthreads();
-  if (rg != 0) return;
 #pragma unroll
-  for (int r = 1; r < kSumRows; ++r) s += part[r][col];
+  for (int n = kSumRows / 2; n > 0; n /= 2) {
+    if (rg >= n && rg < 2 * n) part[rg - n][col] = s;
+    __syncthreads();
+    if (rg < n) s += part[rg][col];
+    __syncthreads();
+  }
+  if (rg != 0) return;
   void* dst = i < head_dim ? g.dq_weight : g.dk_weight;
   if (dst == nullptr) return;
   const int e = i % head_dim;
@@ -471,16 +475,28 @@ __global__ __launch_bounds__(kSumCols * kSumRows) void norm_rope_dw_kernel(NormR
     static_cast<_Float16*>(dst)[e] = (_Float16)s;
 }
 
+// Workgroups from which on a token's heads stay together.  Forward, bf16, d 128, heads split for
+// 256 / 512 / 1024 / 2048 workgroups: 512 tokens of 64 + 8 heads 6.9 / 6.0 / 5.6 / 6.8 us, 2048 of
+// them 19.3 / 15.8 / 14.9 / 18.2, 2048 of 8 + 2 5.1 / 4.5 / 4.6 / 4.5, 8192 of 8 + 2 alike.
+constexpr int64_t kFill = 1024;
+// Backward: workgroups over tokens at most, and those up to which heads are split; each leaves a
+// row of partial sums for the second kernel.  Both kernels, heads split / together: 512 tokens of
+// 64 + 8 heads 11.4 / 46.4 us, 2048 of them 23.8 / 53.7, one token of 8 + 2 6.1 / 10.1.
+constexpr int64_t kBwdTokenBlocks = 1024, kBwdFill = 896;
+int heads_per(int heads, int64_t fill, int64_t blocks) {
+  int64_t chunks = fill / blocks;
+  if (chunks > (heads + 1) / 2) chunks = (heads + 1) / 2;
+  return chunks > 1 ? (int)((heads + chunks - 1) / chunks) : heads;
+}
+
 template <int D, typename Tag, bool kPairs>
 hipError_t launch_fwd(NormRopeParams p, const AppendParams& a, int cache, hipStream_t stream) {
   using S = RowShape<D>;
   const int heads = p.n_heads + (cache != 0 ? 2 : 1) * p.kv_heads;
   const int64_t blocks = (p.total + S::kPerBlock - 1) / S::kPerBlock;
-  // Heads a lane group walks over: all of a token's where the tokens fill the chip, fewer
-  // for fewer tokens.
-  int64_t chunks = (2048 + blocks - 1) / blocks;
-  if (chunks > (heads + 1) / 2) chunks = (heads + 1) / 2;
-  p.heads_per = (int)((heads + chunks - 1) / chunks);
+  // Heads a lane group walks over: all of a token's where the tokens alone make kFill
+  // workgroups, fewer, but two or more, for fewer tokens.
+  p.heads_per = heads_per(heads, kFill, blocks);
   const dim3 grid((unsigned)blocks, (unsigned)((heads + p.heads_per - 1) / p.heads_per));
   if (cache == 0)
     hipLaunchKernelGGL((norm_rope_kernel<D, Tag, kPairs, 0>), grid, dim3(kThreads), 0, stream, p, a);
@@ -492,9 +508,11 @@ hipError_t launch_fwd(NormRopeParams p, const AppendParams& a, int cache, hipStr
 }
 
 template <int D, typename Tag, bool kPairs>
-hipError_t launch_bwd(const NormRopeParams& p, const NormRopeGrad& g, hipStream_t stream) {
-  const int64_t rows = norm_rope_bwd_rows(p.total, D);
-  hipLaunchKernelGGL((norm_rope_bwd_kernel<D, Tag, kPairs>), dim3((unsigned)rows), dim3(kThreads), 0,
+hipError_t launch_bwd(NormRopeParams p, const NormRopeGrad& g, hipStream_t stream) {
+  const NormRopeBwdGrid grid = norm_rope_bwd_grid(p.total, p.n_heads + p.kv_heads, D);
+  const int64_t rows = (int64_t)grid.x * grid.y;
+  p.heads_per = grid.heads_per;
+  hipLaunchKernelGGL((norm_rope_bwd_kernel<D, Tag, kPairs>), dim3(grid.x, grid.y), dim3(kThreads), 0,
                      stream, p, g);
   if (g.partial != nullptr) {
     const hipError_t e = hipGetLastError();
@@ -520,10 +538,15 @@ hipError_t dispatch(const NormRopeParams& p, int head_dim, int dtype, F f) {
 
 }  // namespace
 
-int64_t norm_rope_bwd_rows(int64_t total, int head_dim) {
+NormRopeBwdGrid norm_rope_bwd_grid(int64_t total, int heads, int head_dim) {
   const int64_t per = kThreads / (head_dim / 8);
-  const int64_t blocks = (total + per - 1) / per;
-  return blocks < kNormRopeBwdBlocks ? blocks : kNormRopeBwdBlocks;
+  int64_t blocks = (total + per - 1) / per;
+  if (blocks > kBwdTokenBlocks) blocks = kBwdTokenBlocks;
+  NormRopeBwdGrid g;
+  g.x = (unsigned)blocks;
+  g.heads_per = heads_per(heads, kBwdFill, blocks);
+  g.y = (unsigned)((heads + g.heads_per - 1) / g.heads_per);
+  return g;
 }
 
 hipError_t launch_norm_rope(const NormRopeParams& p, const AppendParams& a, int cache, int head_dim,

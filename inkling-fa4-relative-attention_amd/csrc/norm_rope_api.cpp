@@ -150,7 +150,9 @@ size_t ifa4_qk_norm_rope_bwd_workspace_bytes(const ifa4_norm_rope* a) {
   if (check_norm_rope(a) != IFA4_OK || a->total == 0 ||
       (a->q_weight == nullptr && a->k_weight == nullptr))
     return 0;
-  return (size_t)ifa4::norm_rope_bwd_rows(a->total, a->head_dim) * 2 * a->head_dim * sizeof(float);
+  const ifa4::NormRopeBwdGrid grid =
+      ifa4::norm_rope_bwd_grid(a->total, a->n_heads + a->kv_heads, a->head_dim);
+  return (size_t)grid.x * grid.y * 2 * a->head_dim * sizeof(float);
 }
 
 int32_t ifa4_qk_norm_rope_bwd(const ifa4_norm_rope* a, const ifa4_norm_rope_grad* gr,

@@ -124,6 +124,13 @@ def test_more_rows_than_backward_workgroups(cuda):
     _check(cuda, 1024 * 16 + 5, 3, 1, 128, torch.bfloat16, torch.float32, 128, False)
 
 
+@pytest.mark.parametrize("tokens,hq,hkv,d", [(1, 64, 8, 128), (40, 33, 11, 64), (900, 16, 1, 128),
+                                             (5000, 5, 5, 64)])
+def test_heads_split_over_workgroups(cuda, tokens, hq, hkv, d):
+    """Chunks of heads that hold both kinds, odd counts, and the last chunk short."""
+    _check(cuda, tokens, hq, hkv, d, torch.bfloat16, torch.float32, d, False, seed=31)
+
+
 def test_one_weight_only(cuda):
     q, k, qw, kw, cos, sin, pos, _, _ = _inputs(9, 4, 2, 64, torch.bfloat16, torch.float32, 32, 4)
     args = [x.to(cuda) for x in (q, k)], [x.to(cuda) for x in (cos, sin, pos)]

@@ -113,13 +113,16 @@ def test_backward_checks(kw, grad, want):
 
 def test_backward_workspace():
     size = _abi.lib().ifa4_qk_norm_rope_bwd_workspace_bytes
-    assert size(ctypes.byref(_args(total=1))) == 2 * 128 * 4
-    assert size(ctypes.byref(_args(total=33))) == 3 * 2 * 128 * 4  # 16 rows a workgroup at d 128
+    row = 2 * 128 * 4  # of a workgroup: 16 tokens at d 128, and two of the ten heads
+    assert size(ctypes.byref(_args(total=1))) == 5 * row
+    assert size(ctypes.byref(_args(total=33))) == 3 * 5 * row
+    assert size(ctypes.byref(_args(total=16 * 300))) == 300 * 2 * row  # five heads
+    assert size(ctypes.byref(_args(total=16 * 500))) == 500 * row      # all heads
     assert size(ctypes.byref(_args(total=1, q_weight=0, k_weight=0))) == 0
     most = size(ctypes.byref(_args(total=(1 << 31) - 1)))
     assert most == size(ctypes.byref(_args(total=1 << 24)))
     short = ctypes.c_void_p(_P)
-    for ws, n in ((short, 2 * 128 * 4 - 1), (ctypes.c_void_p(_P + 64), 1 << 20)):
+    for ws, n in ((short, 5 * row - 1), (ctypes.c_void_p(_P + 64), 1 << 20)):
         assert _abi.lib().ifa4_qk_norm_rope_bwd(ctypes.byref(_args(total=1)), ctypes.byref(_grad()),
                                                 ws, n, None) == EWORKSPACE
 
