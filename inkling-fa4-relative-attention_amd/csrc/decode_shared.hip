@@ -676,30 +676,43 @@ __global__ __launch_bounds__(kThreads, 2) void decode_shared_kernel(SharedParams
     const int stride = kOwnStep * kWaves * p.own_chunks;
     const int s0 = key0 + kOwnStep * (chunk * kWaves + wave);
     if (moved) pg = pages_of(p, table, p.max_blocks, s0);
+    // e4m3: the next step's rows are on their way, in registers, while a step is computed (128
+    // sequences behind 8192 keys 22.0 -> 21.5 us).  The twice as many of a 16-bit cache would spill
+    // at d 128 (64 behind 16384 19.9 -> 24.4 us) and lose at d 64 (24.5 -> 25.3 a call): their rows go
+    // to LDS by DMA ahead of each step.
+    constexpr bool kFetch = Eb == 1;
+    u32x4_t kr[kFetch ? kLoads32 : 1], vr[kFetch ? kLoads32 : 1];
+    auto fetch = [&](int k0) {
+      load32(p, tk, pg, k0, key_end, kr);
+      load32(p, tv, pg, k0, key_end, vr);
+      pg = pages_of(p, table, p.max_blocks, k0 + stride);
+    };
+    if constexpr (kFetch) {
+      if (s0 < key_end) fetch(s0);
+    }
     for (int k0 = s0; k0 < key_end; k0 += stride) {
       const bool biased = tile_biased(p, k0, kOwnStep);
       Bias raw;
+      if constexpr (kFetch) {
+        put32(kr, 0, kown);
+        put32(vr, 0, vown);
+      }
       if (biased) bias_issue(p, pos - k0 - 16 * half, raw);
-      if constexpr (Eb == 2) {
-        asm volatile("" ::: "memory");
+      asm volatile("" ::: "memory");
+      if constexpr (kFetch) {
+        if (k0 + stride < key_end) fetch(k0 + stride);
+      } else {
         const uint32_t dst = lds0 + (uint32_t)(wave * 2 * L::kOwn) * 2;
         dma32(p, tk, pg, k0, key_end, 0, dst);
         dma32(p, tv, pg, k0, key_end, 0, dst + L::kOwn * 2);
         pg = pages_of(p, table, p.max_blocks, k0 + stride);
         __builtin_amdgcn_s_waitcnt(kVm0);
         asm volatile("" ::: "memory");
-      } else {
-        u32x4_t kr[kLoads32], vr[kLoads32];
-        load32(p, tk, pg, k0, key_end, kr);
-        load32(p, tv, pg, k0, key_end, vr);
-        pg = pages_of(p, table, p.max_blocks, k0 + stride);
-        put32(kr, 0, kown);
-        put32(vr, 0, vown);
       }
       wave_lds_sync();
       compute(p, std::integral_constant<int, 1>{}, k0, kown, vown, biased, &raw, [] {});
       wave_lds_sync();  // the step's reads come before the next step's rows
-      if constexpr (Eb == 2) __builtin_amdgcn_s_waitcnt(kLgkm0);
+      if constexpr (!kFetch) __builtin_amdgcn_s_waitcnt(kLgkm0);
     }
     // the waves' sums meet: each leaves its O [head][D] in its own rows
     static_assert(16 * D * 4 <= 2 * L::kOwn * 2, "a wave's O fits its rows");
