@@ -18,9 +18,16 @@
 //
 // Layout.  A row is held by D / 8 neighbouring lanes, 16 bytes each; such a lane group
 // takes a token and walks over a chunk of its heads (q heads, then k heads, then for
-// the cache v heads), two rows' loads in flight at a time, with the token's A and B in
-// registers.  Row sums meet by DPP adds, partners by lane exchange of the packed 16-bit
-// row (half-split) or inside the lane (interleaved).
+// the cache v heads) with the token's A and B in registers.  The forward has kAhead rows' loads
+// in flight and asks for the first ahead of the token's position, whose search is the longest
+// chain of a small append; the backward has two rows' x and g.  Row sums meet by DPP adds,
+// partners by lane exchange of the packed 16-bit row (half-split) or inside the lane
+// (interleaved).
+//
+// Bound: memory, and for small calls the launch.  bf16, d 128: 32768 tokens of 8 + 2 heads forward
+// 28.8 us (168 MB at 5.8 TB/s; 45.5 with two rows in flight and none ahead of the position),
+// backward 47.0 us (252 MB at 5.4 TB/s) and 4 us for the weights; into a cache, with values,
+// 34.6 us; 64 decode tokens into a cache 4.5 us.
 #include <type_traits>
 
 #include "ifa4_device.hpp"
@@ -30,7 +37,8 @@ namespace ifa4 {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kAhead = 4;  // rows a lane group has in flight
+constexpr int kAhead = 4;  // rows a lane group has in flight: 2 / 4 / 6 take 29.1 / 28.3 / 28.9 us for
+                           // 32768 tokens of 8 + 2 heads, 3.1 / 3.1 / 3.2 for 64
 
 template <int D>
 struct RowShape {
@@ -356,8 +364,9 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(NormRopeParams p, A
 }
 
 // ---- backward -------------------------------------------------------------------------------
-// A workgroup walks over tokens and a chunk of their heads, and leaves its sums of the weight gradients in one row of the
-// workspace, [q or k][D]; the second kernel adds the rows in a fixed order.
+// A workgroup walks over tokens and a chunk of their heads, and leaves its sums of the weight
+// gradients in one row of the workspace, [q or k][D]; the second kernel adds the rows in a fixed
+// order.
 template <int D, typename Tag, bool kPairs>
 __global__ __launch_bounds__(kThreads) void norm_rope_bwd_kernel(NormRopeParams p, NormRopeGrad g) {
   using S = RowShape<D>;
