@@ -116,6 +116,7 @@ struct NormRopeParams {
   const int32_t* positions;  // [total] (rot > 0; a cache append has its own)
   int64_t angle_stride;
   int64_t total;             // tokens
+  int64_t first_token;       // of this launch (set by the launch)
   int32_t n_heads, kv_heads;
   int32_t w_dtype;           // 0 bf16, 1 fp16, 2 fp32
   int32_t rot;               // leading elements of a head that turn

@@ -262,7 +262,7 @@ __global__ __launch_bounds__(kThreads) void norm_rope_kernel(NormRopeParams p, A
   using S = RowShape<D>;
   constexpr int kLpr = S::kLpr;
   const int lane = threadIdx.x & 63, c = lane % kLpr;
-  const int64_t t64 = (int64_t)blockIdx.x * S::kPerBlock + threadIdx.x / kLpr;
+  const int64_t t64 = p.first_token + (int64_t)blockIdx.x * S::kPerBlock + threadIdx.x / kLpr;
   const bool in = t64 < p.total;
   const int t = in ? (int)t64 : (int)p.total - 1;  // idle groups follow the last token, and store nothing
   const Turn turn = turn_of<kPairs>(p, c);
@@ -492,6 +492,8 @@ constexpr int64_t kFill = 1024;
 // row of partial sums for the second kernel.  Both kernels, heads split / together: 512 tokens of
 // 64 + 8 heads 11.4 / 46.4 us, 2048 of them 23.8 / 53.7, one token of 8 + 2 6.1 / 10.1.
 constexpr int64_t kBwdTokenBlocks = 1024, kBwdFill = 896;
+// Workgroups of one launch along the tokens: a launch holds less than 2^32 threads.
+constexpr int64_t kMostBlocks = 1 << 20;
 int heads_per(int heads, int64_t fill, int64_t blocks) {
   int64_t chunks = fill / blocks;
   if (chunks > (heads + 1) / 2) chunks = (heads + 1) / 2;
@@ -506,14 +508,20 @@ hipError_t launch_fwd(NormRopeParams p, const AppendParams& a, int cache, hipStr
   // Heads a lane group walks over: all of a token's where the tokens alone make kFill
   // workgroups, fewer, but two or more, for fewer tokens.
   p.heads_per = heads_per(heads, kFill, blocks);
-  const dim3 grid((unsigned)blocks, (unsigned)((heads + p.heads_per - 1) / p.heads_per));
-  if (cache == 0)
-    hipLaunchKernelGGL((norm_rope_kernel<D, Tag, kPairs, 0>), grid, dim3(kThreads), 0, stream, p, a);
-  else if (cache == 1)
-    hipLaunchKernelGGL((norm_rope_kernel<D, Tag, kPairs, 1>), grid, dim3(kThreads), 0, stream, p, a);
-  else
-    hipLaunchKernelGGL((norm_rope_kernel<D, Tag, kPairs, 2>), grid, dim3(kThreads), 0, stream, p, a);
-  return hipGetLastError();
+  const unsigned chunks = (unsigned)((heads + p.heads_per - 1) / p.heads_per);
+  for (int64_t at = 0; at < blocks; at += kMostBlocks) {
+    const dim3 grid((unsigned)(blocks - at < kMostBlocks ? blocks - at : kMostBlocks), chunks);
+    p.first_token = at * S::kPerBlock;
+    if (cache == 0)
+      hipLaunchKernelGGL((norm_rope_kernel<D, Tag, kPairs, 0>), grid, dim3(kThreads), 0, stream, p, a);
+    else if (cache == 1)
+      hipLaunchKernelGGL((norm_rope_kernel<D, Tag, kPairs, 1>), grid, dim3(kThreads), 0, stream, p, a);
+    else
+      hipLaunchKernelGGL((norm_rope_kernel<D, Tag, kPairs, 2>), grid, dim3(kThreads), 0, stream, p, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 template <int D, typename Tag, bool kPairs>

@@ -35,6 +35,7 @@ int32_t check_norm_rope(const ifa4_norm_rope* a) {
   if (a->head_dim != 64 && a->head_dim != 128) return IFA4_EUNSUPPORTED;
   if (a->dtype == IFA4_FP32 || a->rot_dim % 16 != 0) return IFA4_EUNSUPPORTED;
   if (a->total > INT32_MAX) return IFA4_EUNSUPPORTED;
+  if ((int64_t)a->n_heads + 2 * (int64_t)a->kv_heads > (1 << 20)) return IFA4_EUNSUPPORTED;
   if (a->q_weight != nullptr || a->k_weight != nullptr) {
     if (a->w_dtype < IFA4_BF16 || a->w_dtype > IFA4_FP32) return IFA4_EINVAL;
     const uintptr_t esize = a->w_dtype == IFA4_FP32 ? 4 : 2;
@@ -147,7 +148,7 @@ int32_t ifa4_qk_norm_rope_fwd(const ifa4_norm_rope* a, void* stream) {
 }
 
 size_t ifa4_qk_norm_rope_bwd_workspace_bytes(const ifa4_norm_rope* a) {
-  if (check_norm_rope(a) != IFA4_OK || a->total == 0 ||
+  if (check_norm_rope(a) != IFA4_OK || a->total == 0 || a->n_heads < 1 || a->kv_heads < 1 ||
       (a->q_weight == nullptr && a->k_weight == nullptr))
     return 0;
   const ifa4::NormRopeBwdGrid grid =

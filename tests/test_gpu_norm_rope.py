@@ -131,6 +131,23 @@ def test_heads_split_over_workgroups(cuda, tokens, hq, hkv, d):
     _check(cuda, tokens, hq, hkv, d, torch.bfloat16, torch.float32, d, False, seed=31)
 
 
+def test_more_tokens_than_one_launch_takes(cuda):
+    """2^25 tokens and some, past 2^31 elements: each row of the outputs is that of its position
+    (one input row for all tokens)."""
+    tokens, rows = (1 << 25) + 37, 8
+    q, k, qw, kw, cos, sin, _, _, _ = _inputs(1, 1, 1, 64, torch.bfloat16, torch.float32, 64, 41)
+    x = [t.to(cuda).expand(tokens, 1, 64) for t in (q, k)]
+    tables = [_dev(t[:rows], cuda).contiguous() for t in (cos, sin)]
+    pos = torch.arange(tokens, device=cuda, dtype=torch.int32) % rows
+    out = inkling_fa4_qk_norm_rope(*x, _dev(qw, cuda), _dev(kw, cuda), *tables, pos, eps=EPS)
+    few = inkling_fa4_qk_norm_rope(*(t[:rows] for t in x), _dev(qw, cuda), _dev(kw, cuda), *tables,
+                                   pos[:rows], eps=EPS)
+    for a, b in zip(out, few):
+        whole = tokens // rows * rows
+        same = (a[:whole].view(-1, rows, 64) == b.view(1, rows, 64)).all(-1).all(0)
+        assert same.all() and torch.equal(a[whole:], b[:tokens - whole])
+
+
 def test_one_weight_only(cuda):
     q, k, qw, kw, cos, sin, pos, _, _ = _inputs(9, 4, 2, 64, torch.bfloat16, torch.float32, 32, 4)
     args = [x.to(cuda) for x in (q, k)], [x.to(cuda) for x in (cos, sin, pos)]

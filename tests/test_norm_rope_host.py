@@ -111,6 +111,16 @@ def test_backward_checks(kw, grad, want):
                                             None) == want
 
 
+@pytest.mark.parametrize("kw", [dict(n_heads=(1 << 31) - 1), dict(kv_heads=(1 << 31) - 1),
+                                dict(n_heads=(1 << 31) - 1, kv_heads=(1 << 31) - 1)])
+def test_more_heads_than_the_launch_counts(kw):
+    a, g = _args(total=1, **kw), _grad()
+    lib = _abi.lib()
+    assert lib.ifa4_qk_norm_rope_fwd(ctypes.byref(a), None) == EUNSUPPORTED
+    assert lib.ifa4_qk_norm_rope_bwd_workspace_bytes(ctypes.byref(a)) == 0
+    assert lib.ifa4_qk_norm_rope_bwd(ctypes.byref(a), ctypes.byref(g), None, 0, None) == EUNSUPPORTED
+
+
 def test_backward_workspace():
     size = _abi.lib().ifa4_qk_norm_rope_bwd_workspace_bytes
     row = 2 * 128 * 4  # of a workgroup: 16 tokens at d 128, and two of the ten heads
@@ -119,6 +129,8 @@ def test_backward_workspace():
     assert size(ctypes.byref(_args(total=16 * 300))) == 300 * 2 * row  # five heads
     assert size(ctypes.byref(_args(total=16 * 500))) == 500 * row      # all heads
     assert size(ctypes.byref(_args(total=1, q_weight=0, k_weight=0))) == 0
+    assert size(ctypes.byref(_args(total=9, n_heads=0, kv_heads=0))) == 0
+    assert size(ctypes.byref(_args(total=9, n_heads=0))) == 0
     most = size(ctypes.byref(_args(total=(1 << 31) - 1)))
     assert most == size(ctypes.byref(_args(total=1 << 24)))
     short = ctypes.c_void_p(_P)
