@@ -203,11 +203,42 @@ def test_batches(cuda, batch):
     c.check(c.run(cuda))
 
 
+@pytest.mark.parametrize("batch,hq,prefix,own,kv", [
+    (256, 8, 4096, 128, None), (200, 8, 4096, 300, None), (200, 8, 4096, 300, F8),
+    (80, 4, 9000, 700, None), (24, 16, 2500, 1500, None)])
+def test_own_keys_shared_out_over_idle_workgroups(cuda, batch, hq, prefix, own, kv):
+    """Workgroups without a prefix piece take several pieces of own keys each, some pieces go to
+    the others, and some workgroups of the prefix's range have no piece of it."""
+    g = torch.Generator().manual_seed(batch)
+    lens = [prefix + int(x) for x in torch.randint(1, own + 1, (batch,), generator=g)]
+    lens[3], lens[-1] = prefix + own, 0
+    c = Case(lens, prefix, hq, 2, extent=512, kv=kv, seed=batch)
+    c.check(c.run(cuda))
+
+
 @pytest.mark.parametrize("kv", [None, F8])
 def test_a_long_prefix_over_small_blocks(cuda, kv):
     """70000 keys in blocks of 16: the window of table entries moves on within a chunk."""
     c = Case([70000 + 5, 70400, 69000], 70000, 2, 1, kv=kv, seed=3)
     c.check(c.run(cuda))
+
+
+def test_blocks_past_32_bits_of_elements(cuda):
+    """The same blocks at the end of a pool of 2^32 elements and more: the same bits."""
+    c = Case([700, 650, 1300], 600, block=16, extent=64, seed=18)
+    want = c.run(cuda)
+    few = c.kc.shape[0]
+    shift = (1 << 32) // c.kc[0].numel() + 1000 - few
+    pools = []
+    for x in (c.kc, c.vc):
+        big = torch.empty(shift + few, *x.shape[1:], dtype=x.dtype, device=cuda)
+        big[shift:] = x.to(cuda)
+        pools.append(big)
+    q, _, _, rel, cu, used, table, prefix = c.on(cuda)
+    table = torch.where(table < few, table + shift, table)
+    out, lse = inkling_fa4_rel_attention_decode_shared_prefix(
+        q, *pools, rel, cu, used, table, prefix + shift, c.prefix, 1, c.max_k, c.extent, **c.settings())
+    assert torch.equal(out.cpu(), want[0]) and torch.equal(lse.cpu(), want[1])
 
 
 def test_large_scores(cuda):

@@ -195,6 +195,27 @@ def test_fp8_rounding_saturation_and_nan(cuda):
     assert torch.equal(got.nan_to_num(99.0), want.nan_to_num(99.0)) and got[37].isnan()
 
 
+def test_blocks_past_32_bits_of_elements(cuda):
+    """The same blocks at the end of a pool of 2^32 elements and more: the same rows there."""
+    c = Call([20, 1, 33], [5, 70, 0], d=128, seed=19)
+    want = c.run(cuda)
+    few = c.kc.shape[0]
+    shift = (1 << 32) // c.kc[0].numel() + 1000 - few
+    pools = []
+    for x in (c.kc, c.vc):
+        big = torch.empty(shift + few, *x.shape[1:], dtype=x.dtype, device=cuda)
+        big[shift:] = x.to(cuda)
+        pools.append(big)
+    table = torch.where(c.table < few, c.table + shift, c.table).to(cuda)
+    on = [x.to(cuda) for x in (c.cu, c.used)]
+    q = inkling_fa4_kv_append_paged(
+        c.k.to(cuda), c.v.to(cuda), *pools, *on, table, q=c.q.to(cuda), q_weight=c.qw.to(cuda),
+        k_weight=c.kw.to(cuda), cos=c.cos.to(cuda), sin=c.sin.to(cuda), eps=EPS)
+    assert torch.equal(q, want[0])
+    for big, x in zip(pools, want[1:]):
+        assert torch.equal(big[shift:].cpu(), x)
+
+
 def test_strided_caches(cuda):
     """A pool that keeps k and v of a block side by side, and one with the heads outermost."""
     c = Call([3, 18], [14, 2], seed=10)
