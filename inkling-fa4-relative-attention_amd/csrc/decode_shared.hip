@@ -138,11 +138,14 @@ __device__ __forceinline__ int first_key(const SharedParams& p, int pos) {
   return p.window_left >= 0 ? max(0, pos - p.window_left) : 0;
 }
 
+struct Whole {};  // every row of a group is there
+
 // Table entry of key k0 (wave-uniform), by a scalar load: a load through the vector memory
 // counter would have to wait for the K and V rows in flight before it.
 __device__ __forceinline__ int page_at(const int32_t* table, int i) {
-  typedef const __attribute__((address_space(4))) int32_t* scalar_ptr;
-  return ((scalar_ptr)(uintptr_t)table)[i];
+  typedef const __attribute__((address_space(4))) char* scalar_ptr;
+  typedef const __attribute__((address_space(4))) int32_t* entry_ptr;
+  return *(entry_ptr)((scalar_ptr)(uintptr_t)table + 4u * (uint32_t)i);  // an offset of 32 bits
 }
 
 template <int D, typename Tag, typename Rel, int Eb>
@@ -223,17 +226,21 @@ __global__ __launch_bounds__(kThreads, 2) void decode_shared_kernel(SharedParams
   };
   // Resource over the group's rows [k0, min(k0 + kGroupRows, stop)): what lies past it, and a
   // whole group whose entry lies outside the pool, reads as zero.
-  // (stop < 0: whole groups only)
-  auto group_rsrc = [&](const SharedParams& p, const Tensor& t, int ent, int k0, int stop) {
-    const int n = stop < 0 ? kGroupRows : min(kGroupRows, stop - k0);
-    const bool good = (unsigned)ent < (unsigned)p.num_blocks && n > 0;
-    const uint32_t at = good ? (uint32_t)ent : 0u;
-    const char* base = t.pool + (int64_t)at * t.block + (uint32_t)(k0 & ((1 << p.block_shift) - 1)) * t.row;
-    return make_rsrc_uniform(base, good ? (uint32_t)(n - 1) * t.row + D * Eb : 0u);
+  auto group_rsrc = [&](const SharedParams& p, const Tensor& t, int ent, int k0, auto stop) {
+    uint32_t seen = (uint32_t)(kGroupRows - 1) * t.row + D * Eb;
+    if constexpr (!std::is_same<decltype(stop), Whole>::value) {
+      const int n = min(kGroupRows, stop - k0);
+      seen = n > 0 ? (uint32_t)(n - 1) * t.row + D * Eb : 0u;
+    }
+    seen = (uint32_t)ent < (uint32_t)p.num_blocks ? seen : 0u;
+    // (no address is formed from the base of an empty resource)
+    const uint64_t base = reinterpret_cast<uint64_t>(t.pool) + (uint64_t)(uint32_t)ent * (uint64_t)t.block +
+                          (uint32_t)(k0 & ((1 << p.block_shift) - 1)) * t.row;
+    return make_rsrc_uniform(reinterpret_cast<const void*>(base), seen);
   };
   const uint32_t lds0 = lds_addr(stages);
   // 16-bit: rows k0 .. k0 + 31 by DMA to LDS rows tile_row .. of the tensor at LDS address dst
-  auto dma32 = [&](const SharedParams& p, const Tensor& t, const Pages& pg, int k0, int stop, int tile_row,
+  auto dma32 = [&](const SharedParams& p, const Tensor& t, const Pages& pg, int k0, auto stop, int tile_row,
                    uint32_t dst) {
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
@@ -249,7 +256,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_shared_kernel(SharedParams
     }
   };
   // e4m3: the same rows into registers, and from there to LDS in the 16-bit type
-  auto load32 = [&](const SharedParams& p, const Tensor& t, const Pages& pg, int k0, int stop, u32x4_t* reg) {
+  auto load32 = [&](const SharedParams& p, const Tensor& t, const Pages& pg, int k0, auto stop, u32x4_t* reg) {
 #pragma unroll
     for (int i = 0; i < kGroups; ++i) {
       const rsrc_t rs = group_rsrc(p, t, pg.ent[i], k0 + kGroupRows * i, stop);
@@ -551,10 +558,10 @@ __global__ __launch_bounds__(kThreads, 2) void decode_shared_kernel(SharedParams
     };
     auto fetch = [&](int kt, int stage) {
       if constexpr (Eb == 2)
-        dma32(p, kv, pg, kt * kTile + my_row, -1, my_row,
+        dma32(p, kv, pg, kt * kTile + my_row, Whole{}, my_row,
               lds0 + (uint32_t)(stage * L::kStage + (is_v ? L::kTensor : 0)) * 2);
       else
-        load32(p, kv, pg, kt * kTile + my_row, -1, reg);
+        load32(p, kv, pg, kt * kTile + my_row, Whole{}, reg);
       pages(kt + 1);
     };
     // the first tile's rows go out ahead of everything that they do not depend on
