@@ -36,7 +36,7 @@
 // and the vector instructions (180, 32 of them exp2) nearly all the rest, with little overlap; 5000
 // where it meets a bias.  One common barrier for eight waves with the K and V of both halves cost
 // 4700 to 5400.  Measured, bf16, d 128, Hq 8 / Hkv 2, bias extent 1024: 256 sequences behind 32768 keys
-// 54 us (570 TFLOP/s of the whole call, 60 us); the merge 9 us, of which 4 are a launch over nothing
+// 56 us traced (a whole call 60, 570 TFLOP/s); the merge 9 us, of which 4 are a launch over nothing
 // and the rest the parts at 5.6 TB/s.  64 sequences behind 16384 keys 20 + 7 us: there a
 // workgroup's four tiles take less than its first rows, its parts and its launch.
 #include <type_traits>
