@@ -21,6 +21,15 @@ using OptTensor = std::optional<at::Tensor>;
 
 bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
 
+// A tangent (forward-mode differentiation) is refused: below autograd it would vanish.
+bool has_tangent(const at::Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+bool has_tangent(const OptTensor& t) { return t.has_value() && has_tangent(*t); }
+template <typename... T>
+void check_no_tangent(const char* op, const T&... inputs) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(inputs) || ...), "inkling_fa4.", op,
+                              ": no forward-mode derivative");
+}
+
 void check_heads(const at::Tensor& x, const at::Tensor& like, const char* op, const char* name) {
   TORCH_CHECK(x.is_cuda() && x.device() == like.device(), "inkling_fa4.", op, ": ", name,
               " must be on k's GPU");
@@ -259,6 +268,7 @@ std::tuple<at::Tensor, at::Tensor> qk_norm_rope_autograd(
     const OptTensor& cos, const OptTensor& sin, const OptTensor& positions, double eps,
     bool interleaved) {
   auto wants = [](const OptTensor& t) { return given(t) && t->requires_grad(); };
+  check_no_tangent("qk_norm_rope", q, k, q_weight, k_weight, cos, sin);
   if (at::GradMode::is_enabled()) {
     TORCH_CHECK_VALUE(!wants(cos) && !wants(sin),
                       "inkling_fa4.qk_norm_rope: cos and sin have no gradient");
@@ -348,13 +358,15 @@ at::Tensor kv_append_paged(const at::Tensor& k, const at::Tensor& v, const at::T
   return q_out;
 }
 
-// The append has no gradient: whatever its inputs ask for, its output never requires one.
+// The append has no gradient: whatever its inputs ask for, its output never requires one.  A
+// tangent is refused.
 at::Tensor kv_append_paged_autograd(
     const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache, const at::Tensor& v_cache,
     const at::Tensor& cu_seqlens, const at::Tensor& seqused_k, const at::Tensor& block_table,
     const OptTensor& q, const OptTensor& q_weight, const OptTensor& k_weight, const OptTensor& cos,
     const OptTensor& sin, double eps, bool interleaved, double k_scale, double v_scale) {
   static const auto op = operator_named<decltype(kv_append_paged)>("inkling_fa4::kv_append_paged");
+  check_no_tangent("kv_append_paged", k, v, k_cache, v_cache, q, q_weight, k_weight, cos, sin);
   const at::AutoDispatchBelowADInplaceOrView below;
   return op.call(k, v, k_cache, v_cache, cu_seqlens, seqused_k, block_table, q, q_weight, k_weight,
                  cos, sin, eps, interleaved, k_scale, v_scale);

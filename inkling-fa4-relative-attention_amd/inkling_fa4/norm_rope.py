@@ -38,8 +38,8 @@ def inkling_fa4_qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=N
     or None, positions int32 [tokens] (needed with cos; outside the table: results
     unspecified).  Returns (q, k), contiguous, in the inputs' dtype.
 
-    Differentiable in q, k and the weights (once); the backward pass reads the inputs
-    again and keeps nothing else.  The weights' gradients are summed over tokens and
+    Differentiable in q, k and the weights (once, in reverse mode; tangents are refused);
+    the backward pass reads the inputs again and keeps nothing else.  The weights' gradients are summed over tokens and
     heads in fp32, in a fixed order.
     """
     if q_weight is None and k_weight is None and cos is None:
@@ -67,6 +67,8 @@ def inkling_fa4_kv_append_paged(k, v, k_cache, v_cache, cu_seqlens_q, seqused_k,
     v / v_scale (saturating; a 16-bit cache ignores the scales).  A token with p < 0, past
     the table or whose table entry lies outside the pool is not written; two tokens sent
     to one row leave one of the two.
+
+    There is no gradient: the result never requires one, and tangents are refused.
     """
     out = _op("kv_append_paged")(k, v, k_cache, v_cache, cu_seqlens_q, seqused_k, block_table, q,
                                  q_weight, k_weight, cos, sin, float(eps), bool(interleaved),
