@@ -12,7 +12,9 @@
 // on q or k alone, so a token's heads share them.
 // Backward, with g the gradient of y: the rotation's transpose is the rotation by -p, so
 //   gz_e = g_e c_e - g_e' s_e;   dw = sum over rows of gz x r;
-//   dx = r gz w - x (r^3 / D) sum_e(gz_e w_e x_e).
+//   dx = r gz w - x (r^3 / D) sum_e(gz_e w_e x_e),
+// taken as r (gz w - (x r) (r / D) sum): r^3 leaves fp32 for rows of rms 1e13 and more, and for
+// tiny ones next to a tiny eps, where the outputs and gradients are ordinary numbers.
 // r is computed again from x, which the backward pass reads anyway: nothing but the
 // inputs is kept between the passes.  All of it is in fp32 with one rounding at the end.
 //
@@ -413,16 +415,16 @@ __global__ __launch_bounds__(kThreads) void norm_rope_bwd_kernel(NormRopeParams 
       dot = row_sum<kLpr>(dot);
       if ((is_q ? p.q_weight : p.k_weight) != nullptr) {
         const float r = rsqrtf(ss * (1.f / D) + p.eps);
-        const float f = r * r * r * (1.f / D) * dot;
-        const float keep = in ? r : 0.f;
+        const float mean = r * dot * (1.f / D);  // of the gradient along x r
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float dw = gy[e] * x[e] * keep;
+          const float xr = x[e] * r;
+          const float dw = in ? gy[e] * xr : 0.f;
           if (is_q)
             dwq[e] += dw;
           else
             dwk[e] += dw;
-          gw[e] = fmaf(-x[e], f, r * gw[e]);
+          gw[e] = r * fmaf(-xr, mean, gw[e]);
         }
       }
       if (!in) return;

@@ -351,3 +351,27 @@ def test_refusals(cuda):
     odd = torch.zeros(3 * 4 * 64 + 1, dtype=torch.bfloat16, device=cuda)[1:].view(3, 4, 64)
     with pytest.raises(RuntimeError, match="EUNSUPPORTED"):
         inkling_fa4_qk_norm_rope(**dict(ok, q=odd))
+
+
+@pytest.mark.parametrize("rms,eps", [(1e13, EPS), (1e14, EPS), (1e16, EPS), (1e18, EPS), (1e-6, 0.0),
+                                     (1e-14, 0.0), (1e-16, 0.0), (1e-16, 1e-30)])
+def test_backward_of_large_and_small_rows(cuda, rms, eps):
+    """Rows whose r^3 leaves fp32 have the gradients of the formula, as the forward its values."""
+    d, dtype = 128, torch.bfloat16
+    q, k, qw, kw, cos, sin, pos, gq, gk = _inputs(33, 4, 2, d, dtype, torch.float32, 64, 51)
+    q, k = ((x.float() * (rms / 3)).to(dtype) for x in (q, k))
+    if eps > 0:
+        q[2, 1] = 0
+    x = [_dev(t, cuda) for t in (q, k, qw, kw, cos, sin, pos, gq, gk)]
+    leaves = [t.clone().requires_grad_() for t in x[:4]]
+    print(f"norm_rope: rows of rms {rms}, eps {eps}", flush=True)
+    out = inkling_fa4_qk_norm_rope(*leaves, *x[4:7], eps=eps)
+    grads = torch.autograd.grad(out, leaves, x[7:])
+    cs, sn = _per_token(cos, sin, pos)
+    eps = float(torch.tensor(eps, dtype=torch.float32))
+    for n, (t, w, y, g, heads) in enumerate(((q, qw, out[0], gq, 4), (k, kw, out[1], gk, 2))):
+        want, size = norm_rope(t, w, cs, sn, eps)
+        _close(y, want, 40 * U * size, ("y", n))
+        wx, ww, xs, ws = norm_rope_bwd(t, w, cs, sn, eps, g)
+        _close(grads[n], wx, 80 * U * xs, ("dx", n))
+        _close(grads[2 + n], ww, (40 + _adds(33, heads, d)) * U * ws, ("dw", n))
