@@ -358,18 +358,37 @@ at::Tensor kv_append_paged(const at::Tensor& k, const at::Tensor& v, const at::T
   return q_out;
 }
 
-// The append has no gradient: whatever its inputs ask for, its output never requires one.  A
-// tangent is refused.
-at::Tensor kv_append_paged_autograd(
+// The append as a change in place: a graph that has saved a cache finds it changed.
+at::Tensor kv_append_paged_in_place(
     const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache, const at::Tensor& v_cache,
     const at::Tensor& cu_seqlens, const at::Tensor& seqused_k, const at::Tensor& block_table,
     const OptTensor& q, const OptTensor& q_weight, const OptTensor& k_weight, const OptTensor& cos,
     const OptTensor& sin, double eps, bool interleaved, double k_scale, double v_scale) {
   static const auto op = operator_named<decltype(kv_append_paged)>("inkling_fa4::kv_append_paged");
+  at::Tensor out;
+  {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    out = op.call(k, v, k_cache, v_cache, cu_seqlens, seqused_k, block_table, q, q_weight, k_weight,
+                  cos, sin, eps, interleaved, k_scale, v_scale);
+  }
+  for (const at::Tensor* cache : {&k_cache, &v_cache})
+    if (!cache->is_inference()) cache->unsafeGetTensorImpl()->bump_version();
+  return out;
+}
+
+// The append has no gradient: whatever its inputs ask for, its output never requires one.  A
+// tangent is refused, and so is a cache that requires a gradient, which would go on as if it had
+// not been written.
+at::Tensor kv_append_paged_autograd(
+    const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache, const at::Tensor& v_cache,
+    const at::Tensor& cu_seqlens, const at::Tensor& seqused_k, const at::Tensor& block_table,
+    const OptTensor& q, const OptTensor& q_weight, const OptTensor& k_weight, const OptTensor& cos,
+    const OptTensor& sin, double eps, bool interleaved, double k_scale, double v_scale) {
   check_no_tangent("kv_append_paged", k, v, k_cache, v_cache, q, q_weight, k_weight, cos, sin);
-  const at::AutoDispatchBelowADInplaceOrView below;
-  return op.call(k, v, k_cache, v_cache, cu_seqlens, seqused_k, block_table, q, q_weight, k_weight,
-                 cos, sin, eps, interleaved, k_scale, v_scale);
+  TORCH_CHECK(!at::GradMode::is_enabled() || !(k_cache.requires_grad() || v_cache.requires_grad()),
+              "inkling_fa4.kv_append_paged: a cache that requires a gradient is written in place");
+  return kv_append_paged_in_place(k, v, k_cache, v_cache, cu_seqlens, seqused_k, block_table, q,
+                                  q_weight, k_weight, cos, sin, eps, interleaved, k_scale, v_scale);
 }
 
 }  // namespace
@@ -393,6 +412,11 @@ TORCH_LIBRARY_IMPL(inkling_fa4, CUDA, m) {
   m.impl("qk_norm_rope", &qk_norm_rope);
   m.impl("qk_norm_rope_bwd", &qk_norm_rope_bwd);
   m.impl("kv_append_paged", &kv_append_paged);
+}
+
+// where there is no autograd above it (inference mode)
+TORCH_LIBRARY_IMPL(inkling_fa4, ADInplaceOrView, m) {
+  m.impl("kv_append_paged", &kv_append_paged_in_place);
 }
 
 TORCH_LIBRARY_IMPL(inkling_fa4, Autograd, m) {

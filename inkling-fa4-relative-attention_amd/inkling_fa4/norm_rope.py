@@ -68,7 +68,8 @@ def inkling_fa4_kv_append_paged(k, v, k_cache, v_cache, cu_seqlens_q, seqused_k,
     the table or whose table entry lies outside the pool is not written; two tokens sent
     to one row leave one of the two.
 
-    There is no gradient: the result never requires one, and tangents are refused.
+    There is no gradient: the result never requires one, tangents are refused, and so are
+    caches that require a gradient (outside torch.no_grad()).
     """
     out = _op("kv_append_paged")(k, v, k_cache, v_cache, cu_seqlens_q, seqused_k, block_table, q,
                                  q_weight, k_weight, cos, sin, float(eps), bool(interleaved),
