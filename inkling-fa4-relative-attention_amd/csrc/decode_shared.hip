@@ -706,6 +706,11 @@ __global__ __launch_bounds__(kThreads, 2) void decode_shared_kernel(SharedParams
     if constexpr (kFetch) {
       if (s0 < key_end) fetch(s0);
     }
+    // The first step under a window begins up to 31 keys left of it.  Their weights are 0, and 0
+    // times an infinite or NaN value would reach the sum: those rows of V are cleared.
+    auto clear_rows = [&](uint16_t* rows, int n) {
+      for (int e = 8 * lane; e < n * D; e += 8 * 64) *reinterpret_cast<u32x4_t*>(rows + e) = u32x4_t{};
+    };
     for (int k0 = s0; k0 < key_end; k0 += stride) {
       const bool biased = tile_biased(p, k0, kOwnStep);
       Bias raw;
@@ -725,6 +730,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_shared_kernel(SharedParams
         __builtin_amdgcn_s_waitcnt(kVm0);
         asm volatile("" ::: "memory");
       }
+      if (k0 < lo_min) clear_rows(vown, lo_min - k0);
       wave_lds_sync();
       compute(p, std::integral_constant<int, 1>{}, k0, kown, vown, biased, &raw, [] {});
       wave_lds_sync();  // the step's reads come before the next step's rows

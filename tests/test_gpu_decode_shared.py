@@ -465,3 +465,22 @@ def test_refusals(cuda):
         call(**dict(ok, k_cache=kc[0]))
     with pytest.raises(ValueError):
         call(**dict(ok, q=q[:, :7]))
+
+
+@pytest.mark.parametrize("kv", [None, F8])
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (4, 4, 64), (16, 1, 128)])
+@pytest.mark.parametrize("window", [0, 5, 40, 130])
+def test_own_keys_left_of_the_window_may_hold_anything(cuda, window, hq, hkv, d, kv):
+    """NaN and infinite keys and values of a sequence's own that its window hides, the ones next
+    to the first visible key among them, reach no result."""
+    lens = [640 + n for n in (60, 161, 192, 193, 223, 500, 777)]
+    c = Case(lens, 640, hq, hkv, d, kv=kv, window=window, seed=window + d)
+    want = c.run(cuda)
+    for b, lk in enumerate(lens):
+        for j in range(640, lk - 1 - window):
+            at = int(c.table[b, j // 16]), j % 16
+            c.kc[at] = math.nan
+            c.vc[at] = math.nan if j % 2 else (448.0 if kv else math.inf)
+    got = c.run(cuda)
+    c.check(got)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
