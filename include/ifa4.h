@@ -364,7 +364,7 @@ int32_t ifa4_decode_fwd_noalloc(const ifa4_args* args, void* stream);
  * fp32 throughout, one rounding to `dtype` at the end.
  * Layouts (element strides, last dim contiguous): q, q_out [total, n_heads,
  * head_dim], k, k_out [total, kv_heads, head_dim] in dtype (rows 16-byte aligned,
- * strides multiples of 8); weights [head_dim] in w_dtype; cos, sin
+ * strides multiples of 8, of a dimension of one any); weights [head_dim] in w_dtype; cos, sin
  * [max_position, rot_dim / 2] fp32 (rows 16-byte aligned, angle_stride elements
  * apart); positions int32 [total], read on the device: one outside
  * [0, max_position) takes the nearest row of the table (results unspecified).
@@ -438,7 +438,8 @@ int32_t ifa4_qk_norm_rope_bwd(const ifa4_norm_rope* args, const ifa4_norm_rope_g
  * even, magnitudes past 448 as 448).  Tokens of no sequence, with p < 0 or past the
  * table, or whose table entry lies outside the pool are not written (q_out of a token of
  * no sequence neither).  Two tokens sent to one row leave one of them.
- * Cache strides are in cache elements, multiples of 16 bytes, as for decode.
+ * Cache strides are in cache elements, multiples of 16 bytes, as for decode (of one
+ * head or block any).
  */
 typedef struct ifa4_kv_append {
   uint32_t struct_size;    /* sizeof(ifa4_kv_append) */

@@ -13,13 +13,15 @@ namespace {
 
 bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
-// 16-byte rows of `heads` heads; written rows must not overlap.
+// 16-byte rows of `heads` heads; written rows must not overlap.  The stride of a dimension of one
+// is never stepped along: it says nothing.
 int32_t check_rows(const void* p, int64_t total, int64_t heads, int64_t st, int64_t sh, int d,
                    bool written) {
   if (st < 0 || sh < 0) return IFA4_EINVAL;
   if (total == 0 || heads == 0) return IFA4_OK;
   if (p == nullptr) return IFA4_EINVAL;
-  if (!aligned(p, 16) || (st | sh) % 8 != 0) return IFA4_EUNSUPPORTED;
+  if (!aligned(p, 16) || ((total > 1 ? st : 0) | (heads > 1 ? sh : 0)) % 8 != 0)
+    return IFA4_EUNSUPPORTED;
   if (written && ((heads > 1 && sh < d) || (total > 1 && st < d))) return IFA4_EUNSUPPORTED;
   return IFA4_OK;
 }
@@ -115,9 +117,10 @@ int32_t check_cache(const ifa4_norm_rope* a, const ifa4_kv_append* ap, const ifa
   if (kv->num_blocks < 1 || kv->max_blocks_per_seq < 1) return IFA4_EINVAL;
   if ((int64_t)kv->max_blocks_per_seq * bs > (int64_t(1) << 30)) return IFA4_EUNSUPPORTED;
   const int64_t unit = fp8 ? 16 : 8;
-  if ((ap->k_cache_stride_t | ap->k_cache_stride_h | ap->v_cache_stride_t | ap->v_cache_stride_h |
-       kv->k_stride_block | kv->v_stride_block) % unit != 0 ||
-      !aligned(ap->k_cache, 16) || !aligned(ap->v_cache, 16))
+  int64_t steps = ap->k_cache_stride_t | ap->v_cache_stride_t;
+  if (a->kv_heads > 1) steps |= ap->k_cache_stride_h | ap->v_cache_stride_h;
+  if (kv->num_blocks > 1) steps |= kv->k_stride_block | kv->v_stride_block;
+  if (steps % unit != 0 || !aligned(ap->k_cache, 16) || !aligned(ap->v_cache, 16))
     return IFA4_EUNSUPPORTED;
   // rows of the cache must not overlap
   const int64_t d = a->head_dim;

@@ -341,3 +341,18 @@ def test_no_gradient_is_asked_of_the_result(cuda):
                                       c.cu.to(cuda), c.used.to(cuda), c.table.to(cuda), q=q,
                                       q_weight=c.qw.to(cuda))
     assert not out.requires_grad
+
+
+def test_strides_of_dimensions_of_one(cuda):
+    """One token, one head, one block: their strides are never stepped along and say nothing."""
+    c = Call([1], [3], 1, 1, seed=20)
+    c.kc, c.vc = c.kc[:1], c.vc[:1]
+    c.table[:] = 0
+    want = c.run(cuda)
+    q, k, v = (t.contiguous().to(cuda).as_strided((1, 1, 64), (67, 3, 1)) for t in (c.q, c.k, c.v))
+    kc, vc = (t.clone().to(cuda).as_strided((1, 16, 1, 64), (7, 64, 3, 1)) for t in (c.kc, c.vc))
+    out = inkling_fa4_kv_append_paged(k, v, kc, vc, c.cu.to(cuda), c.used.to(cuda), c.table.to(cuda),
+                                      q=q, q_weight=c.qw.to(cuda), k_weight=c.kw.to(cuda),
+                                      cos=c.cos.to(cuda), sin=c.sin.to(cuda), eps=EPS)
+    assert torch.equal(out, want[0])
+    assert torch.equal(kc.cpu(), want[1]) and torch.equal(vc.cpu(), want[2])

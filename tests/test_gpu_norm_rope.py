@@ -375,3 +375,22 @@ def test_backward_of_large_and_small_rows(cuda, rms, eps):
         wx, ww, xs, ws = norm_rope_bwd(t, w, cs, sn, eps, g)
         _close(grads[n], wx, 80 * U * xs, ("dx", n))
         _close(grads[2 + n], ww, (40 + _adds(33, heads, d)) * U * ws, ("dw", n))
+
+
+def test_strides_of_dimensions_of_one(cuda):
+    """The stride of a dimension that holds one row is never stepped along and says nothing."""
+    x = _inputs(1, 1, 1, 64, torch.bfloat16, torch.float32, 64, 52)
+    q, k, qw, kw, cos, sin, pos, gq, gk = (_dev(t, cuda) for t in x)
+    q, k = (t.contiguous().as_strided((1, 1, 64), (64, 64, 1)) for t in (q, k))
+
+    def run(*x):
+        leaves = [t.detach().requires_grad_() for t in x] + [w.clone().requires_grad_() for w in (qw, kw)]
+        out = inkling_fa4_qk_norm_rope(*leaves, cos, sin, pos)
+        return list(out) + list(torch.autograd.grad(out, leaves, (gq, gk)))
+    want = run(q, k)
+    for st, sh in ((67, 64), (64, 3), (5, 1)):
+        got = run(*(t.as_strided((1, 1, 64), (st, sh, 1)) for t in (q, k)))
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+    with pytest.raises(RuntimeError, match="EUNSUPPORTED"):  # two rows: stepped along
+        inkling_fa4_qk_norm_rope(torch.zeros(134, dtype=torch.bfloat16, device=cuda).as_strided(
+            (2, 1, 64), (67, 64, 1)), k.expand(2, 1, 64), qw)

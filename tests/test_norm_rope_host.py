@@ -204,3 +204,31 @@ def test_python_refusals_without_a_gpu():
     ints = torch.zeros(2, dtype=torch.int32)
     with pytest.raises(NotImplementedError):
         inkling_fa4_kv_append_paged(k, k, cache, cache.clone(), ints, ints[:1], ints[None])
+
+
+ODD = dict(q_stride_t=67, k_stride_t=67, q_stride_h=3, k_stride_h=3)
+
+
+@pytest.mark.parametrize("kw,want", [
+    ({"total": 1, "n_heads": 1, "kv_heads": 1}, EWORKSPACE),  # every check passed
+    ({"total": 2, "n_heads": 1, "kv_heads": 1}, EUNSUPPORTED),
+    ({"total": 1, "n_heads": 2, "kv_heads": 1}, EUNSUPPORTED),
+    ({"total": 1, "n_heads": 1, "kv_heads": 2}, EUNSUPPORTED),
+])
+def test_strides_of_dimensions_of_one(kw, want):
+    """They are not looked at (the backward pass asks for its workspace last); others are."""
+    a, g = _args(**kw, **ODD), _grad(gq_stride_t=5, gk_stride_t=5, dq_stride_t=9, dk_stride_t=9,
+                                     gq_stride_h=128 + 3 * (kw["n_heads"] == 1))
+    assert _abi.lib().ifa4_qk_norm_rope_bwd(ctypes.byref(a), ctypes.byref(g), None, 0, None) == want
+
+
+@pytest.mark.parametrize("kw,append,kv", [
+    ({"kv_heads": 2}, dict(k_cache_stride_h=132), {}),
+    ({"kv_heads": 1}, {}, dict(num_blocks=2, k_stride_block=4100)),
+    ({"kv_heads": 1}, dict(k_cache_stride_t=132), {}),
+])
+def test_cache_strides_that_are_stepped_along(kw, append, kv):
+    a = _args(total=1, n_heads=1, **kw)
+    ap, pk = _append(**append), _kv(**dict(dict(num_blocks=1), **kv))
+    assert _abi.lib().ifa4_kv_append_paged(ctypes.byref(a), ctypes.byref(ap), ctypes.byref(pk),
+                                           None) == EUNSUPPORTED
