@@ -434,8 +434,8 @@ int32_t ifa4_qk_norm_rope_bwd(const ifa4_norm_rope* args, const ifa4_norm_rope_g
  * (kv->seqused_k counts the new keys: it is what the attention call after this one
  * takes); its k, normed and turned by position p, and its v go to row p % block_size of
  * block kv->block_table[b, p / block_size], in the type kv_dtype: args.dtype, or
- * IFA4_FP8_E4M3, which stores the e4m3 value nearest to k * (1 / k_scale) (ties to
- * even, magnitudes past 448 as 448).  Tokens of no sequence, with p < 0 or past the
+ * IFA4_FP8_E4M3, which stores the e4m3 value nearest to the fp32 quotient k / k_scale
+ * (ties to even, magnitudes past 448 as 448).  Tokens of no sequence, with p < 0 or past the
  * table, or whose table entry lies outside the pool are not written (q_out of a token of
  * no sequence neither).  Two tokens sent to one row leave one of them.
  * Cache strides are in cache elements, multiples of 16 bytes, as for decode (of one

@@ -136,7 +136,7 @@ struct AppendParams {
   const int32_t* block_table;
   int64_t v_st, v_sh, kc_st, kc_sh, kc_sblk, vc_st, vc_sh, vc_sblk, bt_stride;
   int32_t batch, block_shift, num_blocks, max_blocks;
-  float inv_k_scale, inv_v_scale;
+  float k_scale, v_scale, inv_k_scale, inv_v_scale;
 };
 
 // Gradients of the norm and rotation; gq or gk NULL: that output has none.

@@ -243,6 +243,8 @@ int32_t ifa4_kv_append_paged(const ifa4_norm_rope* a, const ifa4_kv_append* ap,
   p.block_shift = __builtin_ctz((unsigned)kv->block_size);
   p.num_blocks = kv->num_blocks;
   p.max_blocks = kv->max_blocks_per_seq;
+  p.k_scale = ap->k_scale;
+  p.v_scale = ap->v_scale;
   p.inv_k_scale = 1.f / ap->k_scale;
   p.inv_v_scale = 1.f / ap->v_scale;
   return status_of(ifa4::launch_norm_rope(make_params(a), p, ap->kv_dtype == IFA4_FP8_E4M3 ? 2 : 1,

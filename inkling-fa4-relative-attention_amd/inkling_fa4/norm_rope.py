@@ -63,8 +63,8 @@ def inkling_fa4_kv_append_paged(k, v, k_cache, v_cache, cu_seqlens_q, seqused_k,
 
     With q [tokens, Hq, D] the queries are normed and turned by the same positions in the
     same launch and returned (else None); rows of tokens that no sequence holds are not
-    written.  A float8_e4m3fn cache stores the e4m3 value nearest to k / k_scale and
-    v / v_scale (saturating; a 16-bit cache ignores the scales).  A token with p < 0, past
+    written.  A float8_e4m3fn cache stores the e4m3 values nearest to the fp32 quotients
+    k / k_scale and v / v_scale (ties to even, saturating; a 16-bit cache ignores the scales).  A token with p < 0, past
     the table or whose table entry lies outside the pool is not written; two tokens sent
     to one row leave one of the two.
 

@@ -356,3 +356,22 @@ def test_strides_of_dimensions_of_one(cuda):
                                       cos=c.cos.to(cuda), sin=c.sin.to(cuda), eps=EPS)
     assert torch.equal(out, want[0])
     assert torch.equal(kc.cpu(), want[1]) and torch.equal(vc.cpu(), want[2])
+
+
+@pytest.mark.parametrize("scale", [7.0, 13.0, 0.03, 0.3, 1 / 64])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_fp8_of_every_16_bit_value(cuda, dtype, scale):
+    """The e4m3 values of the fp32 quotients k / k_scale and v / v_scale, ties to even, whatever
+    the scale (no norm, no rotation: rows go into the cache as they are)."""
+    x = torch.arange(1 << 16, dtype=torch.int32).to(torch.int16).view(dtype)
+    n = x.numel() // 64
+    c = Call([n], [0], 0 + 1, 1, 64, dtype, kv=F8, rot=0, normed=False, seed=1)
+    c.k = c.v = x.view(n, 1, 64).clone()
+    _, kc, vc = c.run(cuda, k_scale=scale, v_scale=scale)
+    want = (x.float() / torch.tensor(scale)).clamp(-448, 448).to(F8).float().view(n, 64)
+    pages = c.table[0].long()
+    for cache in (kc, vc):
+        got = cache[pages].reshape(-1, 64)[:n].float()
+        assert torch.equal(got.isnan(), want.isnan())
+        off = (got != want) & ~want.isnan()
+        assert not off.any(), (int(off.sum()), x.view(n, 64)[off][:3], got[off][:3], want[off][:3])
