@@ -92,8 +92,8 @@ ifa4_norm_rope make_args(const char* op, const OptTensor& q, const at::Tensor& k
     TORCH_CHECK(cos->is_cuda() && cos->device() == k.device() && sin->is_cuda() &&
                     sin->device() == k.device() && cos->scalar_type() == at::kFloat &&
                     sin->scalar_type() == at::kFloat && cos->dim() == 2 &&
-                    cos->sizes() == sin->sizes() && cos->strides() == sin->strides() &&
-                    cos->stride(1) == 1,
+                    cos->sizes() == sin->sizes() && cos->stride(1) == 1 && sin->stride(1) == 1 &&
+                    (cos->size(0) <= 1 || cos->stride(0) == sin->stride(0)),
                 "inkling_fa4.", op,
                 ": cos and sin must be fp32 [positions, rot_dim / 2] with contiguous rows, alike, "
                 "on k's GPU");

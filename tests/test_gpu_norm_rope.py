@@ -394,3 +394,15 @@ def test_strides_of_dimensions_of_one(cuda):
     with pytest.raises(RuntimeError, match="EUNSUPPORTED"):  # two rows: stepped along
         inkling_fa4_qk_norm_rope(torch.zeros(134, dtype=torch.bfloat16, device=cuda).as_strided(
             (2, 1, 64), (67, 64, 1)), k.expand(2, 1, 64), qw)
+
+
+def test_a_table_of_one_row(cuda):
+    """cos and sin of one position: the stride between rows says nothing, alike or not."""
+    q, k, qw, kw, cos, sin, _, _, _ = (_dev(t, cuda) for t in _inputs(
+        5, 2, 1, 64, torch.bfloat16, torch.float32, 32, 53))
+    pos = torch.zeros(5, dtype=torch.int32, device=cuda)
+    want = inkling_fa4_qk_norm_rope(q, k, qw, kw, cos, sin, pos)
+    wide = torch.cat([cos, cos, sin], 1)
+    for c in (cos[:1], wide[:1, 16:32], cos[:1].as_strided((1, 16), (3, 1))):
+        got = inkling_fa4_qk_norm_rope(q, k, qw, kw, c, sin[:1].clone(), pos)
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
