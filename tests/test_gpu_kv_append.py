@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from inkling_fa4 import (inkling_fa4_kv_append_paged, inkling_fa4_qk_norm_rope,
-                         inkling_fa4_rel_attention_decode_paged)
+                         inkling_fa4_rel_attention, inkling_fa4_rel_attention_decode_paged)
 from oracle import ref_rel_attn_paged_with_lse
 from oracle.norm_rope import append_positions, norm_rope
 
@@ -375,3 +375,36 @@ def test_fp8_of_every_16_bit_value(cuda, dtype, scale):
         assert torch.equal(got.isnan(), want.isnan())
         off = (got != want) & ~want.isnan()
         assert not off.any(), (int(off.sum()), x.view(n, 64)[off][:3], got[off][:3], want[off][:3])
+
+
+@pytest.mark.parametrize("kv", [None, F8])
+def test_a_prompt_through_norm_attention_and_append(cuda, kv):
+    """A prompt's three calls: norm and rotation, attention over what comes back, an append of that
+    k as it is.  The cache holds, bit by bit, what the append's own norm and rotation write in
+    16 bits; an e4m3 row is then the nearest of a 16-bit value.  A prompt's last row is that of a
+    decode over the cache: 2e-2 apart at most, as in the decode tests (16-bit weights and outputs of
+    two kernels), where the cache holds the same keys."""
+    lens, hq, hkv, d = [40, 7, 129], 8, 2, 128
+    c = Call(lens, [0, 0, 0], hq, hkv, d, kv=kv, rot=64, seed=21)
+    q, k, v, qw, kw, cos, sin, cu, used, table = (x.to(cuda) for x in (
+        c.q, c.k, c.v, c.qw, c.kw, c.cos, c.sin, c.cu, c.used, c.table))
+    pos = torch.cat([torch.arange(n, dtype=torch.int32) for n in lens]).to(cuda)
+    kc, vc = c.kc.to(cuda), c.vc.to(cuda)
+    q, k = inkling_fa4_qk_norm_rope(q, k, qw, kw, cos, sin, pos, eps=EPS)
+    rel = (0.5 * torch.randn(sum(lens), hq, 64, generator=torch.Generator().manual_seed(22))).to(cuda)
+    out = inkling_fa4_rel_attention(q, k, v, rel, cu, cu, max(lens), max(lens), 64, softmax_scale=0.1)
+    scales = dict(k_scale=0.03, v_scale=0.02) if kv else {}
+    assert inkling_fa4_kv_append_paged(k, v, kc, vc, cu, used, table, **scales) is None
+    if kv:
+        for cache, x, s in ((kc, k, 0.03), (vc, v, 0.02)):
+            want = (x.float() / torch.tensor(s, device=cuda)).clamp(-448, 448).to(F8)
+            for t, _, blk, row in c.slots():
+                assert torch.equal(cache[blk, row].float(), want[t].float())
+        return
+    _, k2, v2 = c.run(cuda)
+    assert torch.equal(kc.cpu(), k2) and torch.equal(vc.cpu(), v2)
+    last = (cu[1:] - 1).long()
+    got = inkling_fa4_rel_attention_decode_paged(
+        q[last], kc, vc, rel[last].contiguous(), torch.arange(4, dtype=torch.int32, device=cuda), used,
+        table, 1, max(lens), 64, softmax_scale=0.1, bottom_right=True)
+    torch.testing.assert_close(got.float(), out[last].float(), atol=2e-2, rtol=2e-2)
