@@ -26,10 +26,11 @@
 // partners by lane exchange of the packed 16-bit row (half-split) or inside the lane
 // (interleaved).
 //
-// Bound: memory, and for small calls the launch.  bf16, d 128: 32768 tokens of 8 + 2 heads forward
-// 28.8 us (168 MB at 5.8 TB/s; 45.5 with two rows in flight and none ahead of the position),
-// backward 47.0 us (252 MB at 5.4 TB/s) and 4 us for the weights; into a cache, with values,
-// 34.6 us; 64 decode tokens into a cache 4.5 us.
+// Bound: memory, and for small calls the launch.  bf16, d 128, 32768 tokens of 8 + 2 heads on fresh
+// inputs: forward 37.0 us (168 MB at 4.5 TB/s), backward 47.6 us (252 MB at 5.3 TB/s, the rate of a
+// copy) and 4 us for the weights, into a cache with values 45.4 us (203 MB at 4.5 TB/s).  Where
+// the caches hold part of the inputs forward takes 29 us (45.5 with two rows in flight and none ahead
+// of the position), into a cache 34.5; 64 decode tokens into a cache take 4.7 us.
 #include <type_traits>
 
 #include "ifa4_device.hpp"

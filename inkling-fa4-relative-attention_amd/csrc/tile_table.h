@@ -451,7 +451,8 @@ struct SharedPlan {
 // Cycles, measured inside the kernel (d 128, two workgroups on a CU): a prefix piece without its
 // tiles (rows, first tile, the part's way out), a tile (a quarter more with a bias), a part's share
 // of the merge, a piece that a window hides; an own piece without its rounds, and a round of its
-// waves (128 keys).
+// waves (128 keys).  Taken on a 16-bit cache with 16-bit biases; d 64, e4m3 and fp32 biases are planned
+// with the same.
 constexpr int64_t kSharedPiece = 13000, kSharedTileCost = 4000, kSharedPart = 70;
 constexpr int64_t kSharedHidden = 8000;
 constexpr int64_t kSharedOwnPiece = 7000, kSharedOwnRoundCost = 7000;

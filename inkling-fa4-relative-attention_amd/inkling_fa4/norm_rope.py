@@ -60,6 +60,7 @@ def inkling_fa4_kv_append_paged(k, v, k_cache, v_cache, cu_seqlens_q, seqused_k,
     so token i of n new ones has position p = seqused_k[b] - n + i and goes to row
     p % block_size of block block_table[b, p // block_size].  The caches change in place;
     rows that no token goes to stay as they are.
+    cos and sin need a row for every position p (past them: that row's values unspecified).
 
     With q [tokens, Hq, D] the queries are normed and turned by the same positions in the
     same launch and returned (else None); rows of tokens that no sequence holds are not

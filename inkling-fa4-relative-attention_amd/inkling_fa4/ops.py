@@ -195,7 +195,10 @@ def inkling_fa4_rel_attention_decode_shared_prefix(q, k_cache, v_cache, rel_logi
                                                    k_scale=1.0, v_scale=1.0):
     """Paged decode of a batch whose sequences begin with the same keys: the result of
     inkling_fa4_rel_attention_decode_paged(..., bottom_right=True), with the keys and values
-    of the prefix read and multiplied once for the whole batch.
+    of the prefix read and multiplied once for the whole batch.  Faster than that call behind
+    prefixes of more than 256 keys, a few sequences included (4 behind 1024 keys 12.4 against
+    16.0 us, 64 behind 8192 21 against 78), unless a window shows less than an eighth of the
+    prefix (64 behind 8192 under a window of 511: 17.9 against 14.3).
 
     The caller states that the first prefix_len keys of every sequence are those of
     prefix_table, int32 [>= ceil(prefix_len / block_size)] (any sequence's row of
