@@ -31,17 +31,17 @@
 // exp2((s - m) log2 e), so that biases down to the lowest finite fp32 stay finite: a row that
 // has nothing else gives the softmax over them.
 //
-// Bounds.  The tiles of a long prefix are bound by what two waves of a SIMD issue: a tile takes 4000 cycles for
-// two workgroups of a CU, of which the matrix products are 2048 (32 products of 32 cycles a wave)
-// and the vector instructions (180, 32 of them exp2) nearly all the rest, with little overlap; 5000
-// where it meets a bias.  One common barrier for eight waves with the K and V of both halves cost
-// 4700 to 5400.  Measured, bf16, d 128, Hq 8 / Hkv 2, bias extent 1024: 256 sequences behind 32768 keys
-// 57 us traced (a whole call 59, 580 TFLOP/s), the matrix cores busy for 0.35 of it: of a
-// workgroup's 98000 cycles 80000 are its 20 tiles and 13000 its start and exit, and 96 of the 512
-// workgroups hold own keys only, whose rounds wait for their rows.  The merge takes 9 us, of which 4
-// are a launch over nothing and the rest the 28 MB of parts at 5.6 TB/s.  64 sequences behind 16384
-// keys 21 + 7 us: there a workgroup's four tiles take less than its first rows, its parts and its
-// launch.
+// Bounds.  The tiles of a long prefix are bound by what two waves of a SIMD issue: a tile takes 4000
+// cycles for two workgroups of a CU, of which the matrix products are 2048 (32 products of 32 cycles
+// a wave) and the vector instructions (180, 32 of them exp2) nearly all the rest, with little
+// overlap; 5000 where it meets a bias.  One common barrier for eight waves with the K and V of both
+// halves cost 4700 to 5400.  Measured, bf16, d 128, Hq 8 / Hkv 2, bias extent 1024: 256 sequences
+// behind 32768 keys 57 us traced (a whole call 59, 580 TFLOP/s), the matrix cores busy for 0.35 of
+// it: by the plan's cycles 80000 of a workgroup's 98000 are its 20 tiles and 13000 its start and
+// exit, and 96 of the 512 workgroups hold own keys only, whose rounds wait for their rows.  The merge
+// takes 9 us, of which 4 are a launch over nothing and the rest the 28 MB of parts at 5.6 TB/s.  64
+// sequences behind 16384 keys 21 + 7 us: there a workgroup's four tiles take less than its first
+// rows, its parts and its launch.
 #include <type_traits>
 
 #include "ifa4_device.hpp"

@@ -39,8 +39,8 @@ def inkling_fa4_qk_norm_rope(q, k, q_weight=None, k_weight=None, cos=None, sin=N
     unspecified).  Returns (q, k), contiguous, in the inputs' dtype.
 
     Differentiable in q, k and the weights (once, in reverse mode; tangents are refused);
-    the backward pass reads the inputs again and keeps nothing else.  The weights' gradients are summed over tokens and
-    heads in fp32, in a fixed order.
+    the backward pass reads the inputs again and keeps nothing else.  The weights' gradients
+    are summed over tokens and heads in fp32, in a fixed order.
     """
     if q_weight is None and k_weight is None and cos is None:
         raise ValueError("nothing to do: give a weight, or cos and sin")
@@ -59,15 +59,15 @@ def inkling_fa4_kv_append_paged(k, v, k_cache, v_cache, cu_seqlens_q, seqused_k,
     inkling_fa4_rel_attention_decode_paged takes afterwards: seqused_k counts the new keys,
     so token i of n new ones has position p = seqused_k[b] - n + i and goes to row
     p % block_size of block block_table[b, p // block_size].  The caches change in place;
-    rows that no token goes to stay as they are.
-    cos and sin need a row for every position p (past them: that row's values unspecified).
+    rows that no token goes to stay as they are.  cos and sin need a row for every position
+    p (a token past them gets unspecified values).
 
     With q [tokens, Hq, D] the queries are normed and turned by the same positions in the
     same launch and returned (else None); rows of tokens that no sequence holds are not
     written.  A float8_e4m3fn cache stores the e4m3 values nearest to the fp32 quotients
-    k / k_scale and v / v_scale (ties to even, saturating; a 16-bit cache ignores the scales).  A token with p < 0, past
-    the table or whose table entry lies outside the pool is not written; two tokens sent
-    to one row leave one of the two.
+    k / k_scale and v / v_scale (ties to even, saturating; a 16-bit cache ignores the
+    scales).  A token with p < 0, past the table or whose table entry lies outside the pool
+    is not written; two tokens sent to one row leave one of the two.
 
     There is no gradient: the result never requires one, tangents are refused, and so are
     caches that require a gradient (outside torch.no_grad()).
