@@ -303,6 +303,26 @@ int32_t ifa4_decode_quant_fwd(const ifa4_args* args, const ifa4_paged_kv* kv,
                               size_t workspace_bytes, void* stream);
 
 /*
+ * Prefill over a paged cache: the newest tokens of every sequence attend to its cache, their
+ * own keys (already in it) included: a chunk of a long prompt, a new turn of a conversation,
+ * draft tokens to be verified.  Sequence b has n = cu_seqlens_q[b+1] - cu_seqlens_q[b]
+ * queries and seqused_k[b] keys; query i sits at key position seqused_k[b] - n + i
+ * (bottom-right alignment; args.flags must hold IFA4_FLAG_BOTTOM_RIGHT) for the causal mask,
+ * the window and the bias distance.  quant: NULL for a 16-bit cache, else an e4m3 one; any GQA
+ * group.  The result is that of ifa4_prefill_fwd on the same keys stored contiguously, up to
+ * the order of a split's merge.  Rows left of the first key that a tile of queries (128 at
+ * most) sees and rows past the last may hold anything; of a key that one query of a tile sees
+ * and another does not, key and value must be finite.  The workspace
+ * (ifa4_prefill_paged_workspace_bytes, 0 for a call that does not split) as in
+ * ifa4_prefill_fwd_ws.  The reference has no kernel for it.
+ */
+size_t ifa4_prefill_paged_workspace_bytes(const ifa4_args* args, const ifa4_paged_kv* kv,
+                                          const ifa4_kv_quant* quant);
+int32_t ifa4_prefill_paged_fwd(const ifa4_args* args, const ifa4_paged_kv* kv,
+                               const ifa4_kv_quant* quant, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
+/*
  * Decode of a batch whose sequences begin with the same keys (a shared prompt): the
  * result of paged decode with bottom-right alignment (args.flags must hold
  * IFA4_FLAG_BOTTOM_RIGHT), computed with the prefix read and multiplied once for the

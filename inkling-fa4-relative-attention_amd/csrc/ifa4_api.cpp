@@ -54,7 +54,8 @@ int32_t check_args(const ifa4_args* a, const ifa4_paged_kv* kv = nullptr, int kv
   if ((a->q == nullptr || a->out == nullptr) && a->total_q > 0) return IFA4_EINVAL;
   if ((a->k == nullptr || a->v == nullptr) && (kv != nullptr || a->total_k > 0))
     return IFA4_EINVAL;
-  if (a->rel_extent > 0 && a->rel == nullptr) return IFA4_EINVAL;
+  if (a->rel_extent > 0 && a->rel == nullptr && (kv == nullptr || a->total_q > 0))
+    return IFA4_EINVAL;
   if (a->lse != nullptr) {
     if (!aligned(a->lse, 4)) return IFA4_EINVAL;
     if (a->n_heads > 1 && a->lse_stride_h < a->total_q) return IFA4_EINVAL;
@@ -129,6 +130,16 @@ int32_t check_paged(const ifa4_args* a, const ifa4_paged_kv* kv, int kv_esize = 
   if (((int64_t)(bs - 1) * a->k_stride_t + a->head_dim) * kv_esize >= kLimit ||
       ((int64_t)(bs - 1) * a->v_stride_t + a->head_dim) * kv_esize >= kLimit)
     return IFA4_EUNSUPPORTED;
+  return IFA4_OK;
+}
+
+// Quantised K/V description (include/ifa4.h, ifa4_kv_quant).
+int32_t check_quant(const ifa4_kv_quant* qt) {
+  if (qt->struct_size != sizeof(ifa4_kv_quant)) return IFA4_EINVAL;
+  if (qt->kv_dtype != IFA4_FP8_E4M3) return IFA4_EUNSUPPORTED;
+  if (!std::isfinite(qt->k_scale) || !std::isfinite(qt->v_scale) || !(qt->k_scale > 0.f) ||
+      !(qt->v_scale > 0.f))
+    return IFA4_EINVAL;
   return IFA4_OK;
 }
 
@@ -335,6 +346,50 @@ int32_t run_rproj(const ifa4_args* args, const ifa4_rel_proj* pr, bool split, vo
   return e == hipSuccess ? IFA4_OK : IFA4_ELAUNCH;
 }
 
+// Checks of a prefill call over a paged cache.
+int32_t check_prefill_paged(const ifa4_args* a, const ifa4_paged_kv* kv, const ifa4_kv_quant* qt) {
+  int32_t st = IFA4_OK;
+  if (kv == nullptr) return IFA4_EINVAL;
+  if (qt != nullptr && (st = check_quant(qt)) != IFA4_OK) return st;
+  const int esize = qt != nullptr ? 1 : 2;
+  if ((st = check_args(a, kv, esize)) != IFA4_OK) return st;
+  if ((a->flags & IFA4_FLAG_BOTTOM_RIGHT) == 0) return IFA4_EUNSUPPORTED;
+  return check_paged(a, kv, esize);
+}
+
+// No query token at all (an empty tensor's rel may be null): nothing to do.
+bool no_queries(const ifa4_args* a) {
+  return a->batch == 0 || a->max_seqlen_q == 0 || a->total_q == 0;
+}
+
+int32_t run_prefill_paged(const ifa4_args* a, const ifa4_paged_kv* kv, const ifa4_kv_quant* qt,
+                          void* workspace, size_t workspace_bytes, void* stream) {
+  const int32_t st = check_prefill_paged(a, kv, qt);
+  if (st != IFA4_OK || no_queries(a)) return st;
+  ifa4_args b = *a;
+  b.total_k = (int64_t)a->batch * a->max_seqlen_k;  // the lengths are on the device only
+  ifa4::PrefillParams p = make_prefill_params(&b);
+  const PrefillWorkspace w = prefill_workspace(a);
+  set_tiles(p, a, ifa4::prefill_block_q(), w.pack);
+  if (!set_split(p, w, workspace, workspace_bytes)) return IFA4_EWORKSPACE;
+  p.block_table = kv->block_table;
+  p.seqused_k = kv->seqused_k;
+  p.bt_stride = kv->block_table_stride;
+  p.k_sblk = kv->k_stride_block;
+  p.v_sblk = kv->v_stride_block;
+  p.block_shift = __builtin_ctz((unsigned)kv->block_size);
+  p.num_blocks = kv->num_blocks;
+  p.max_blocks = kv->max_blocks_per_seq;
+  p.v_scale = 1.f;
+  if (qt != nullptr) {
+    p.scale_log2 = a->softmax_scale * qt->k_scale * kLog2eHost;
+    p.v_scale = qt->v_scale;
+  }
+  const auto launch = qt != nullptr ? ifa4::launch_prefill_paged_fp8 : ifa4::launch_prefill_paged;
+  const hipError_t e = launch(p, a->head_dim, a->qkv_dtype, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? IFA4_OK : IFA4_ELAUNCH;
+}
+
 // Top-left causal decode (Lq = 1) sees key 0 only.
 bool key0_only(const ifa4_args* a) {
   return a->causal != 0 && (a->flags & IFA4_FLAG_BOTTOM_RIGHT) == 0;
@@ -393,16 +448,6 @@ DecodeLayout decode_layout(const ifa4_args* a, bool fp8 = false, bool paged = fa
   l.lse_bytes = (l.slots * group * 4 + 255) / 256 * 256;
   l.meta_bytes = segs * 2 * 4;
   return l;
-}
-
-// Quantised K/V description (include/ifa4.h, ifa4_kv_quant).
-int32_t check_quant(const ifa4_kv_quant* qt) {
-  if (qt->struct_size != sizeof(ifa4_kv_quant)) return IFA4_EINVAL;
-  if (qt->kv_dtype != IFA4_FP8_E4M3) return IFA4_EUNSUPPORTED;
-  if (!std::isfinite(qt->k_scale) || !std::isfinite(qt->v_scale) || !(qt->k_scale > 0.f) ||
-      !(qt->v_scale > 0.f))
-    return IFA4_EINVAL;
-  return IFA4_OK;
 }
 
 int32_t check_decode(const ifa4_args* a, const ifa4_paged_kv* kv = nullptr,
@@ -699,6 +744,18 @@ size_t ifa4_prefill_rproj_workspace_bytes(const ifa4_args* args, const ifa4_rel_
 int32_t ifa4_prefill_rproj_fwd_ws(const ifa4_args* args, const ifa4_rel_proj* pr, void* workspace,
                                   size_t workspace_bytes, void* stream) {
   return run_rproj(args, pr, true, workspace, workspace_bytes, stream);
+}
+
+size_t ifa4_prefill_paged_workspace_bytes(const ifa4_args* args, const ifa4_paged_kv* kv,
+                                          const ifa4_kv_quant* quant) {
+  if (check_prefill_paged(args, kv, quant) != IFA4_OK || no_queries(args)) return 0;
+  return (size_t)prefill_workspace(args).total();
+}
+
+int32_t ifa4_prefill_paged_fwd(const ifa4_args* args, const ifa4_paged_kv* kv,
+                               const ifa4_kv_quant* quant, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+  return run_prefill_paged(args, kv, quant, workspace, workspace_bytes, stream);
 }
 
 int32_t ifa4_prefill_count_tiles(const ifa4_args* args, const int32_t* cu_q, const int32_t* cu_k,

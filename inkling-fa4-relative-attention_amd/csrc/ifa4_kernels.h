@@ -57,6 +57,13 @@ struct PrefillParams {
   // rel_dtype describe r [Tq, Hq, 16]; wt is W^T [rel_width, 16] fp32, rows
   // contiguous; bias(i, dist) = sum_c r[i, c] * wt[dist, c].
   const float* wt;
+  // Paged KV cache (block_table != nullptr): k/v are block pools, as in DecodeParams; k_st,
+  // k_sh, k_sblk (and v's) count elements of the cache's type.
+  const int32_t* block_table;
+  const int32_t* seqused_k;
+  int64_t bt_stride, k_sblk, v_sblk;
+  int32_t block_shift, num_blocks, max_blocks;
+  float v_scale;  // of an e4m3 cache: multiplies the output (the K scale is in scale_log2)
 };
 
 struct DecodeParams {
@@ -224,6 +231,10 @@ bool prefill_tab(const PrefillParams& p);  // the shared bias table is staged in
 bool prefill_tab_packs(int rel_extent, int pack);  // ... and holds the tables of `pack` heads
 int prefill_waves();
 hipError_t launch_prefill(const PrefillParams& p, int head_dim, int qkv_dtype, hipStream_t stream);
+hipError_t launch_prefill_paged(const PrefillParams& p, int head_dim, int qkv_dtype,
+                                hipStream_t stream);
+hipError_t launch_prefill_paged_fp8(const PrefillParams& p, int head_dim, int qkv_dtype,
+                                    hipStream_t stream);
 
 int decode_max_group();
 int decode_fp8_max_group();

@@ -2,7 +2,8 @@
 
 Same export names as the reference package (src/inkling_fa4/__init__.py:1-11),
 minus `ref_rel_attn`: the fp32 oracle is test infrastructure and lives in the
-repository's `oracle/` package, outside the product.  Added: the paged-KV
+repository's `oracle/` package, outside the product.  Added: prefill over a paged KV
+cache, `inkling_fa4_rel_attention_paged`; the paged-KV
 decode entry points `inkling_fa4_rel_attention_decode_paged` and
 `inkling_fa4_rel_attention_decode_shared_prefix`; the fused
 relative-logit projection `inkling_fa4_rel_attention_rproj`; and the steps before
@@ -17,6 +18,7 @@ from .ops import (
     inkling_fa4_rel_attention_decode_shared_prefix,
     inkling_fa4_rel_attention_decode_triton,
     inkling_fa4_rel_attention_kv_pruned_triton,
+    inkling_fa4_rel_attention_paged,
     inkling_fa4_rel_attention_rproj,
     inkling_fa4_rel_attention_triton,
     prefill_tile_counts,
@@ -27,6 +29,7 @@ __all__ = [
     "inkling_fa4_rel_attention_decode",
     "inkling_fa4_rel_attention_decode_paged",
     "inkling_fa4_rel_attention_decode_shared_prefix",
+    "inkling_fa4_rel_attention_paged",
     "inkling_fa4_rel_attention_triton",
     "inkling_fa4_rel_attention_decode_triton",
     "inkling_fa4_rel_attention_kv_pruned_triton",

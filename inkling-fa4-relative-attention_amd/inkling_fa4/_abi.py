@@ -162,6 +162,9 @@ SIGNATURES = {
                                                              _P_QUANT]),
     "ifa4_decode_shared_fwd": (_c_int32, [_P_ARGS, _P_PAGED, _P_SHARED, _P_QUANT, _vp,
                                           ctypes.c_size_t, _vp]),
+    "ifa4_prefill_paged_workspace_bytes": (ctypes.c_size_t, [_P_ARGS, _P_PAGED, _P_QUANT]),
+    "ifa4_prefill_paged_fwd": (_c_int32, [_P_ARGS, _P_PAGED, _P_QUANT, _vp, ctypes.c_size_t,
+                                          _vp]),
     "ifa4_qk_norm_rope_fwd": (_c_int32, [_P_NORM, _vp]),
     "ifa4_qk_norm_rope_bwd_workspace_bytes": (ctypes.c_size_t, [_P_NORM]),
     "ifa4_qk_norm_rope_bwd": (_c_int32, [_P_NORM, ctypes.POINTER(Ifa4NormRopeGrad), _vp,

@@ -187,6 +187,34 @@ def inkling_fa4_rel_attention_decode_paged(q, k_cache, v_cache, rel_logits, cu_s
     return (out, lse) if return_lse else out
 
 
+def inkling_fa4_rel_attention_paged(q, k_cache, v_cache, rel_logits, cu_seqlens_q, seqused_k,
+                                    block_table, max_seqlen_q, max_seqlen_k, rel_extent,
+                                    causal=True, window_size=(-1, -1), *, softmax_scale=None,
+                                    return_lse=False, k_scale=1.0, v_scale=1.0):
+    """Prefill over a paged KV cache: the newest tokens of every sequence attend to its cache,
+    their own keys included (inkling_fa4_kv_append_paged put them there): a chunk of a long
+    prompt, a new turn of a conversation, draft tokens to be verified.
+
+    q [total_q, Hq, D] and rel_logits [total_q, Hq, R' >= rel_extent] as in
+    inkling_fa4_rel_attention, the cache, seqused_k (which counts the new tokens) and
+    block_table as in inkling_fa4_rel_attention_decode_paged; any GQA group, any number of
+    queries a sequence.  Query i of a sequence's n sits at key position seqused_k[b] - n + i
+    for the causal mask, the window and the bias distance (bottom-right alignment); causal=False
+    lets it see every key.  A row with no visible key: out 0, lse -inf; rows of tokens that no
+    sequence holds are not written.  max_seqlen_q and max_seqlen_k must bound the lengths.
+    Keys and values that one of a tile's queries (128 at most) sees and another does not must
+    be finite; what lies past the last key, or left of every query's window, may be anything.
+    """
+    if k_cache.dim() != 4:
+        raise ValueError("k_cache must be [num_blocks, block_size, kv_heads, head_dim]")
+    scale = _resolve(q, k_cache.shape[1:], None, None, None, softmax_scale)
+    out, lse = _call("fwd_paged", q, k_cache, v_cache, rel_logits, cu_seqlens_q, seqused_k,
+                     block_table, int(max_seqlen_q), int(max_seqlen_k), int(rel_extent),
+                     bool(causal), _window_left(window_size), scale, bool(return_lse),
+                     float(k_scale), float(v_scale))
+    return (out, lse) if return_lse else out
+
+
 def inkling_fa4_rel_attention_decode_shared_prefix(q, k_cache, v_cache, rel_logits, cu_seqlens_q,
                                                    seqused_k, block_table, prefix_table,
                                                    prefix_len, max_seqlen_q, max_seqlen_k,
