@@ -478,6 +478,98 @@ typedef struct ifa4_kv_append {
 int32_t ifa4_kv_append_paged(const ifa4_norm_rope* args, const ifa4_kv_append* append,
                              const ifa4_paged_kv* kv, void* stream);
 
+/*
+ * Bounds of the keys of a paged cache's blocks: for the blocks that new tokens went to
+ * (positions seqused_k[b] - n .. seqused_k[b] - 1 of sequence b, n = cu_seqlens[b+1] -
+ * cu_seqlens[b], as in the append before it), the least and the greatest element of their
+ * keys below seqused_k[b], by kv head and dimension, in the cache's type (exact; NaN where a
+ * key is NaN):
+ *   bounds[blk, h, 0, d] = min over rows, bounds[blk, h, 1, d] = max.
+ * Other blocks' bounds stay as they are, and so do those behind table entries outside the pool.
+ * Two sequences that hold one block at unequal lengths leave the bounds of one of them.
+ * max_seqlen_q must bound n.  Of kv the fields v_stride_block is not read.  The reference has
+ * no kernel for it.
+ */
+typedef struct ifa4_key_bounds {
+  uint32_t struct_size;    /* sizeof(ifa4_key_bounds) */
+  int32_t kv_dtype;        /* IFA4_BF16, IFA4_FP16 or IFA4_FP8_E4M3: of cache and bounds */
+  int32_t head_dim;        /* 64 or 128 */
+  int32_t kv_heads;
+  int32_t batch;
+  int32_t max_seqlen_q;
+  const void* k_cache;
+  int64_t k_stride_t, k_stride_h;      /* elements, multiples of 16 bytes */
+  void* bounds;            /* [num_blocks, kv_heads, 2, head_dim], 16-byte aligned */
+  int64_t bounds_stride_block, bounds_stride_h;  /* of [2, head_dim], which is contiguous */
+  const int32_t* cu_seqlens;           /* device int32 [batch + 1] */
+} ifa4_key_bounds;
+
+int32_t ifa4_key_bounds_paged(const ifa4_key_bounds* args, const ifa4_paged_kv* kv, void* stream);
+
+/*
+ * The blocks that each token and kv head attends to, by those bounds.  Token i of n of sequence
+ * b sits at pos = seqused_k[b] - n + i and may read the blocks 0 .. pos / block_size.  With no
+ * more than n_select of them it reads all; else the first sink_blocks, the last recent_blocks
+ * and the best of those between by
+ *   score(blk) = sum over the kv head's query heads g and d of max(q_gd lo_d, q_gd hi_d),
+ * summed in 64 bits (NaN counts as infinity; equal scores: the lower block; a table entry outside
+ * the pool has bounds of zero).  blocks [total_q, kv_heads, n_select] (contiguous) gets the block
+ * indexes ascending, then -1; a token of no sequence gets -1 throughout.  n_select >=
+ * sink_blocks + recent_blocks, recent_blocks >= 1.  max_seqlen_q and max_seqlen_k must bound the
+ * lengths.  The workspace (256-byte aligned, contents on entry irrelevant) is scratch for one
+ * call.  Of kv the fields k_stride_block and v_stride_block are not read.  The reference has no
+ * kernel for it.
+ */
+typedef struct ifa4_block_select {
+  uint32_t struct_size;    /* sizeof(ifa4_block_select) */
+  int32_t dtype;           /* of q: IFA4_BF16 or IFA4_FP16 */
+  int32_t kv_dtype;        /* of bounds: dtype or IFA4_FP8_E4M3 */
+  int32_t head_dim;        /* 64 or 128 */
+  int32_t n_heads;
+  int32_t kv_heads;
+  int32_t batch;
+  int32_t max_seqlen_q;
+  int32_t max_seqlen_k;
+  int32_t n_select;
+  int32_t sink_blocks;
+  int32_t recent_blocks;
+  int64_t total_q;
+  const void* q;           /* [total_q, n_heads, head_dim], rows 16-byte aligned */
+  int64_t q_stride_t, q_stride_h;
+  const void* bounds;      /* as in ifa4_key_bounds */
+  int64_t bounds_stride_block, bounds_stride_h;
+  const int32_t* cu_seqlens;
+  int32_t* blocks;
+} ifa4_block_select;
+
+size_t ifa4_select_blocks_workspace_bytes(const ifa4_block_select* args, const ifa4_paged_kv* kv);
+int32_t ifa4_select_blocks_paged(const ifa4_block_select* args, const ifa4_paged_kv* kv,
+                                 void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Attention of each token and kv head over the listed blocks of its sequence (one token a
+ * sequence or many), causal, bottom-right alignment (args.causal 1, args.flags must hold
+ * IFA4_FLAG_BOTTOM_RIGHT): the keys j of the blocks blocks[t, h, :] with j <= pos and, with a
+ * window, j >= pos - window_left; the bias by pos - j.  An entry outside the sequence's table
+ * (-1), a block past pos, and a block whose table entry lies outside the pool are passed over; a
+ * block named twice counts twice.  A list that names all blocks gives ifa4_prefill_paged_fwd's
+ * result up to rounding.  GQA groups up to 16; quant: NULL for a 16-bit cache.  The workspace
+ * (ifa4_sparse_paged_workspace_bytes, 0 where one pass takes the call) is scratch for one
+ * call, 256-byte aligned.  The reference has no kernel for it.
+ */
+typedef struct ifa4_block_list {
+  uint32_t struct_size;    /* sizeof(ifa4_block_list) */
+  int32_t n_select;        /* entries of a list, >= 1 */
+  const int32_t* blocks;   /* device int32 [total_q, kv_heads, n_select], last dim contiguous */
+  int64_t stride_t, stride_h;
+} ifa4_block_list;
+
+size_t ifa4_sparse_paged_workspace_bytes(const ifa4_args* args, const ifa4_paged_kv* kv,
+                                         const ifa4_block_list* list, const ifa4_kv_quant* quant);
+int32_t ifa4_sparse_paged_fwd(const ifa4_args* args, const ifa4_paged_kv* kv,
+                              const ifa4_block_list* list, const ifa4_kv_quant* quant,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif

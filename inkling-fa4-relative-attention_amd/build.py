@@ -23,9 +23,9 @@ ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 HIPCC = os.path.join(ROCM, "bin", "hipcc")
 
 LIB_SOURCES = ["prefill_fwd.hip", "prefill_paged.hip", "prefill_paged_fp8.hip", "decode_fwd.hip",
-               "decode_noalloc.hip", "decode_shared.hip", "norm_rope.hip", "ifa4_api.cpp",
-               "norm_rope_api.cpp"]
-EXT_SOURCES = ["torch_ext.cpp", "torch_norm_rope.cpp"]
+               "decode_noalloc.hip", "decode_shared.hip", "norm_rope.hip", "block_select.hip",
+               "sparse_fwd.hip", "ifa4_api.cpp", "norm_rope_api.cpp", "block_select_api.cpp"]
+EXT_SOURCES = ["torch_ext.cpp", "torch_norm_rope.cpp", "torch_block_select.cpp"]
 LIB_NAME = "libifa4.so"
 EXT_NAME = "_ifa4_torch.so"
 

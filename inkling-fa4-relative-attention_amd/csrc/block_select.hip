@@ -1,0 +1,413 @@
+// Which blocks of a paged cache a token's attention reads, for gfx950 (MI355X): bounds of the
+// keys of every block, scores of the blocks by them, and the choice.  The reference has none.
+//
+//   lo, hi[blk, h, d] = least and greatest key element of the block's rows (the type holds them
+//     exactly; NaN where a key is NaN)
+//   score[t, h, b] = sum over the query heads g of kv head h and d of max(q_gd lo_d, q_gd hi_d)
+//                  = sum_d qn_d lo_d + qp_d hi_d,  qn = sum_g min(q_g, 0), qp = sum_g max(q_g, 0):
+//     no key of the block has a greater sum of its group's dot products.
+//   list[t, h] = the first `sink` blocks, the last `recent` ones up to the token's own, and the
+//     best by score of those between (a score of NaN as infinity, equal ones the lower block
+//     first), ascending; all blocks where there are no more than the list holds.
+//
+// The choice is whole numbers, so it should not hang on the order of a sum: scores are summed in
+// 64 bits, where the products are exact to 2^-53 (in 32 bits about one list in a few hundred of
+// 2000 blocks changed with the summation order).  The chip multiplies 64-bit floats at 74 TFLOP/s
+// on the matrix cores and converts and adds 17e12 elements a second on the vector unit, so a
+// decode step is bound by the bounds' bytes all the same.
+#include "ifa4_device.hpp"
+#include "ifa4_kernels.h"
+
+namespace ifa4 {
+namespace {
+
+typedef double f64x4_t __attribute__((ext_vector_type(4)));
+
+// Elements of a cache: 16 bytes of them as fp32.
+template <typename Tag, int Eb>
+__device__ __forceinline__ void unpack16(u32x4_t w, float* f) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (Eb == 2) {
+      f[2 * i] = Elem<Tag>::lo(w[i]);
+      f[2 * i + 1] = Elem<Tag>::hi(w[i]);
+    } else {
+      typedef float f32x2_t __attribute__((ext_vector_type(2)));
+      const f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], false);
+      const f32x2_t b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[i], true);
+      f[4 * i] = a[0];
+      f[4 * i + 1] = a[1];
+      f[4 * i + 2] = b[0];
+      f[4 * i + 3] = b[1];
+    }
+  }
+}
+template <typename Tag, int Eb>
+__device__ __forceinline__ u32x4_t pack16(const float* f) {
+  u32x4_t w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (Eb == 2) {
+      w[i] = Elem<Tag>::pack2(f[2 * i], f[2 * i + 1]);
+    } else {  // exact: the values are e4m3 values
+      int x = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i], f[4 * i + 1], 0, false);
+      w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[4 * i + 2], f[4 * i + 3], x, true);
+    }
+  }
+  return w;
+}
+
+__device__ __forceinline__ float lower(float x, float m) { return x < m || x != x ? x : m; }
+__device__ __forceinline__ float higher(float x, float m) { return x > m || x != x ? x : m; }
+
+// ---- bounds ----------------------------------------------------------------------------------
+// A wave takes one (block, kv head) whose rows new tokens changed: D * Eb / 16 lanes a row, as
+// many rows at a time as fit, then the row groups meet by lane exchange.  Blocks of 64 rows and
+// more: the four waves of the workgroup share one.
+constexpr int kBoundWaves = 4;
+template <int D, typename Tag, int Eb>
+__global__ __launch_bounds__(64 * kBoundWaves) void key_bounds_kernel(KeyBoundsParams p) {
+  constexpr int kLpr = D * Eb / 16, kRpi = 64 / kLpr, kEpl = 16 / Eb;
+  __shared__ float part[kBoundWaves][2][D];
+  const int seq = blockIdx.y;
+  const int wave = (int)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int bs = 1 << p.block_shift;
+  const int team = bs >= 64 ? kBoundWaves : 1;  // waves a block
+  const int item = (int)blockIdx.x * (kBoundWaves / team) + (team > 1 ? 0 : wave);
+  const int slot = item / p.kv_heads, h = item - slot * p.kv_heads;
+  const int64_t cap = (int64_t)p.max_blocks << p.block_shift;
+  const int64_t used = min(max((int64_t)p.seqused_k[seq], (int64_t)0), cap);
+  const int64_t n = min(max((int64_t)p.cu_q[seq + 1] - p.cu_q[seq], (int64_t)0), used);
+  const int64_t blk = ((used - n) >> p.block_shift) + slot;
+  const bool on = n > 0 && slot < p.slots && (blk << p.block_shift) < used;  // team: uniform
+  const int ent = on ? p.block_table[seq * p.bt_stride + blk] : -1;
+  const bool good = (uint32_t)ent < (uint32_t)p.num_blocks;
+  if (team == 1 && !good) return;
+  const int rows = good ? (int)min(used - (blk << p.block_shift), (int64_t)bs) : 0;
+  const int r = lane / kLpr, c = lane % kLpr;
+  const char* const base = static_cast<const char*>(p.k) +
+                           ((int64_t)(good ? ent : 0) * p.k_sblk + (int64_t)h * p.k_sh) * Eb + 16 * c;
+  float lo[kEpl], hi[kEpl];
+#pragma unroll
+  for (int e = 0; e < kEpl; ++e) {
+    lo[e] = INFINITY;
+    hi[e] = -INFINITY;
+  }
+  const int first = team > 1 ? wave * kRpi : 0, step = team * kRpi;
+#pragma unroll 4
+  for (int row = first + r; row < rows; row += step) {
+    float f[kEpl];
+    unpack16<Tag, Eb>(ld_global_16(base + (int64_t)row * p.k_st * Eb), f);
+#pragma unroll
+    for (int e = 0; e < kEpl; ++e) {
+      lo[e] = lower(f[e], lo[e]);
+      hi[e] = higher(f[e], hi[e]);
+    }
+  }
+#pragma unroll
+  for (int off = kLpr; off < 64; off <<= 1) {
+#pragma unroll
+    for (int e = 0; e < kEpl; ++e) {
+      lo[e] = lower(__shfl_xor(lo[e], off), lo[e]);
+      hi[e] = higher(__shfl_xor(hi[e], off), hi[e]);
+    }
+  }
+  if (team > 1) {
+    if (r == 0) {
+#pragma unroll
+      for (int e = 0; e < kEpl; ++e) {
+        part[wave][0][kEpl * c + e] = lo[e];
+        part[wave][1][kEpl * c + e] = hi[e];
+      }
+    }
+    __syncthreads();
+    if (wave != 0 || !good) return;
+#pragma unroll
+    for (int w = 1; w < kBoundWaves; ++w) {
+#pragma unroll
+      for (int e = 0; e < kEpl; ++e) {
+        lo[e] = lower(part[w][0][kEpl * c + e], lo[e]);
+        hi[e] = higher(part[w][1][kEpl * c + e], hi[e]);
+      }
+    }
+  }
+  if (r > 1) return;
+  char* const dst = static_cast<char*>(p.bounds) +
+                    ((int64_t)ent * p.b_sblk + (int64_t)h * p.b_sh) * Eb + 16 * c;
+  // row group 0 writes the lower bounds, row group 1 the upper (a wave holds two rows at least)
+  *reinterpret_cast<u32x4_t*>(dst + r * D * Eb) = pack16<Tag, Eb>(r == 0 ? lo : hi);
+}
+
+// ---- scores ----------------------------------------------------------------------------------
+// Keys that order as the scores do: greater score, greater key; NaN as the greatest of all with
+// infinity's key (+0 and -0 alike).
+__device__ __forceinline__ uint64_t score_key(double x) {
+  x = x != x ? (double)INFINITY : x + 0.0;
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  return b >> 63 ? ~b : b | (uint64_t(1) << 63);
+}
+
+// Blocks that token t of sequence seq may read: those up to its own.
+struct TokenSpan {
+  int start, len;  // tokens of the sequence
+  int past;        // keys before its first token
+};
+__device__ __forceinline__ TokenSpan token_span(const SelectParams& p, int seq) {
+  const SeqBounds b = seq_bounds(p.cu_q, seq, p.total_q);
+  const int lk = min(max(p.seqused_k[seq], 0), p.max_blocks << p.block_shift);
+  return TokenSpan{b.start, b.len, lk - b.len};
+}
+__device__ __forceinline__ int token_blocks(const SelectParams& p, const TokenSpan& s, int i) {
+  const int pos = s.past + i;
+  return pos < 0 ? 0 : min((pos >> p.block_shift) + 1, p.cols);
+}
+
+// 16 tokens of a sequence against 16 blocks a step, on v_mfma_f64_16x16x4: A = bounds (lane l:
+// block l % 16, elements of the chunks l / 16 modulo 4), B = qn, qp of the same elements (token
+// l % 16), held in registers over the blocks; C (lane l, register r) = block 4 r + l / 16, token
+// l % 16.
+constexpr int kScoreWaves = 4;
+template <int D, typename Tag, int Eb>
+__global__ __launch_bounds__(64 * kScoreWaves) void score_tile_kernel(SelectParams p) {
+  constexpr int kEpc = 16 / Eb;                // elements of a 16-byte chunk
+  constexpr int kChunks = 2 * D / kEpc / 4;    // chunks a lane holds of a block's bounds
+  const int seq = blockIdx.y;
+  const int part0 = blockIdx.x % p.score_parts, rest = blockIdx.x / p.score_parts;
+  const int h = rest % p.kv_heads, i0 = rest / p.kv_heads * 16;
+  const TokenSpan s = token_span(p, seq);
+  if (i0 >= s.len) return;
+  const int most = token_blocks(p, s, min(i0 + 16, s.len) - 1);  // of the tile's last token
+  const int lane = threadIdx.x & 63, wave = (int)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int m = lane & 15, g = lane >> 4;
+  // a list that takes every block needs no scores; nor do the sink and recent blocks
+  if (most <= p.n_select) return;
+  const int last = most - p.recent;  // blocks [sink, last) compete for the tile's last token
+  int tile = (p.sink >> 4) + part0 * kScoreWaves + wave;
+  if (tile * 16 >= last) return;
+
+  double q[kChunks][kEpc];
+#pragma unroll
+  for (int i = 0; i < kChunks; ++i)
+#pragma unroll
+    for (int e = 0; e < kEpc; ++e) q[i][e] = 0.0;
+  const int64_t tok = s.start + min(i0 + m, s.len - 1);
+  const char* const q_row = static_cast<const char*>(p.q) +
+                            (tok * p.q_st + (int64_t)h * p.group * p.q_sh) * 2;
+  for (int head = 0; head < p.group; ++head) {
+#pragma unroll
+    for (int i = 0; i < kChunks / 2; ++i) {
+      const int d = kEpc * (4 * i + g);
+#pragma unroll
+      for (int part = 0; part < kEpc / 8; ++part) {
+        float f[8];
+        unpack16<Tag, 2>(ld_global_16(q_row + (head * p.q_sh + d + 8 * part) * 2), f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          q[i][8 * part + e] += (double)(f[e] > 0.f ? 0.f : f[e]);  // a NaN in both
+          q[i + kChunks / 2][8 * part + e] += (double)(f[e] < 0.f ? 0.f : f[e]);
+        }
+      }
+    }
+  }
+
+  const int32_t* const table = p.block_table + seq * p.bt_stride;
+  auto load = [&](int t, u32x4_t* w) {
+    const int blk = min(16 * t + m, most - 1);
+    const int ent = table[blk];
+    const bool good = (uint32_t)ent < (uint32_t)p.num_blocks;
+    const char* src = static_cast<const char*>(p.bounds) +
+                      ((int64_t)(good ? ent : 0) * p.b_sblk + (int64_t)h * p.b_sh) * Eb + 16 * g;
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      w[i] = ld_global_16(src + 64 * i);
+      if (!good) w[i] = u32x4_t{0u, 0u, 0u, 0u};
+    }
+  };
+  const int step = p.score_parts * kScoreWaves;
+  u32x4_t w[kChunks], next[kChunks];
+  load(tile, w);
+  for (; tile * 16 < last; tile += step) {
+    if ((tile + step) * 16 < last) load(tile + step, next);
+    f64x4_t acc = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      float f[kEpc];
+      unpack16<Tag, Eb>(w[i], f);
+#pragma unroll
+      for (int e = 0; e < kEpc; ++e)
+        acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)f[e], q[i][e], acc, 0, 0, 0);
+    }
+    if (i0 + m < s.len) {
+      uint64_t* const dst = p.scores + ((tok * p.kv_heads + h) * (int64_t)p.cols + 16 * tile + g);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (16 * tile + g + 4 * r < p.cols) dst[4 * r] = score_key(acc[r]);
+    }
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) w[i] = next[i];
+  }
+}
+
+// ---- choice ----------------------------------------------------------------------------------
+// One workgroup per (token, kv head): the n_free best of the competing blocks by a radix select
+// over their keys, 8 bits at a time from the top until the keys that share the border's digits
+// are all taken or all digits are used; then the list in ascending order, by a prefix sum over
+// the blocks.
+constexpr int kPickThreads = 256;
+__global__ __launch_bounds__(kPickThreads) void pick_blocks_kernel(SelectParams p) {
+  __shared__ int hist[256];
+  __shared__ int sums[2][kPickThreads / 64 + 1];
+  __shared__ int border[2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t row = blockIdx.x;
+  const int t = (int)(row / p.kv_heads);
+  int32_t* const list = p.out + row * p.n_select;
+
+  // the token's sequence: the first whose tokens end past it
+  int nb = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += 64) {
+    const int b = b0 + lane;
+    const uint64_t past = __builtin_amdgcn_ballot_w64(b < p.batch && p.cu_q[min(b, p.batch - 1) + 1] > t);
+    if (past != 0) {
+      const TokenSpan s = token_span(p, b0 + __builtin_ctzll(past));
+      if (t >= s.start && t < s.start + s.len) nb = token_blocks(p, s, t - s.start);
+      break;
+    }
+  }
+  if (nb <= p.n_select) {
+    for (int i = tid; i < p.n_select; i += kPickThreads) list[i] = i < nb ? i : -1;
+    return;
+  }
+  const int first = p.sink, last = nb - p.recent;
+  int need = p.n_select - p.sink - p.recent;  // of the competing blocks [first, last)
+  const uint64_t* const keys = p.scores + row * (int64_t)p.cols;
+  uint64_t prefix = 0;  // the border's digits found so far, shifted down
+  int shift = 64;       // by so much
+  while (shift > 0 && need > 0) {
+    shift -= 8;
+    hist[tid] = 0;
+    __syncthreads();
+    for (int b = first + tid; b < last; b += kPickThreads) {
+      const uint64_t k = keys[b];
+      if (shift == 56 || (k >> (shift + 8)) == prefix) atomicAdd(&hist[(int)(k >> shift) & 255], 1);
+    }
+    __syncthreads();
+    // digit of the border: greater digits hold fewer than need, with it as many or more
+    const int mine = hist[255 - tid];
+    int incl = mine;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int up = __shfl_up(incl, off);
+      if (lane >= off) incl += up;
+    }
+    if (lane == 63) sums[0][wave] = incl;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) incl += sums[0][w];
+    if (incl - mine < need && incl >= need) {
+      border[0] = 255 - tid;
+      border[1] = need - (incl - mine);
+    }
+    __syncthreads();
+    const int digit = border[0];
+    const int all = hist[digit];
+    need = border[1];
+    prefix = prefix << 8 | (uint64_t)digit;
+    __syncthreads();
+    if (need == all) break;  // every key with these digits is taken
+  }
+  // taken: digits above the border's, and of the border's the first `need`
+  for (int i = tid; i < p.sink; i += kPickThreads) list[i] = i;
+  for (int i = tid; i < p.recent; i += kPickThreads) list[p.n_select - p.recent + i] = last + i;
+  int at = p.sink, equal = 0;  // places filled and border keys met before this round
+  for (int b0 = first; b0 < last; b0 += kPickThreads) {
+    const int b = b0 + tid;
+    bool above = false, same = false;
+    if (b < last && shift < 64) {
+      const uint64_t k = keys[b] >> shift;
+      above = k > prefix;
+      same = k == prefix;
+    }
+    const uint64_t ma = __builtin_amdgcn_ballot_w64(above), ms = __builtin_amdgcn_ballot_w64(same);
+    __syncthreads();
+    if (lane == 0) {
+      sums[0][wave] = __builtin_popcountll(ma);
+      sums[1][wave] = __builtin_popcountll(ms);
+    }
+    __syncthreads();
+    int a = 0, e = 0, a_all = 0, e_all = 0;
+#pragma unroll
+    for (int w = 0; w < kPickThreads / 64; ++w) {
+      if (w < wave) {
+        a += sums[0][w];
+        e += sums[1][w];
+      }
+      a_all += sums[0][w];
+      e_all += sums[1][w];
+    }
+    const uint64_t below = (uint64_t(1) << lane) - 1;
+    a += __builtin_popcountll(ma & below);
+    e += equal + __builtin_popcountll(ms & below);
+    if (above || (same && e < need)) list[at + a + min(e, need) - min(equal, need)] = b;
+    at += a_all + min(equal + e_all, need) - min(equal, need);
+    equal += e_all;
+  }
+}
+
+template <int D, typename Tag, int Eb>
+hipError_t launch_select_t(const SelectParams& p_in, hipStream_t stream) {
+  SelectParams p = p_in;
+  if (p.cols > p.n_select) {
+    const int tiles = (p.cols + 15) / 16, q_tiles = (p.max_q + 15) / 16;
+    // waves take one tile of 16 blocks each, more where there are many tokens
+    const int per = (tiles + kScoreWaves - 1) / kScoreWaves;
+    const int64_t others = (int64_t)q_tiles * p.kv_heads * p.batch;
+    p.score_parts = (int)max(int64_t(1), min((int64_t)per, 4096 / max(int64_t(1), others)));
+    hipLaunchKernelGGL((score_tile_kernel<D, Tag, Eb>),
+                       dim3((unsigned)((int64_t)p.score_parts * q_tiles * p.kv_heads), p.batch),
+                       dim3(64 * kScoreWaves), 0, stream, p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL(pick_blocks_kernel, dim3((unsigned)((int64_t)p.total_q * p.kv_heads)),
+                     dim3(kPickThreads), 0, stream, p);
+  return hipGetLastError();
+}
+
+template <int D, typename Tag>
+hipError_t launch_select_d(const SelectParams& p, bool fp8, hipStream_t stream) {
+  return fp8 ? launch_select_t<D, Tag, 1>(p, stream) : launch_select_t<D, Tag, 2>(p, stream);
+}
+
+template <int D, typename Tag, int Eb>
+hipError_t launch_bounds_t(const KeyBoundsParams& p, hipStream_t stream) {
+  const int per = (1 << p.block_shift) >= 64 ? 1 : kBoundWaves;
+  const int64_t items = (int64_t)p.slots * p.kv_heads;
+  hipLaunchKernelGGL((key_bounds_kernel<D, Tag, Eb>), dim3((unsigned)((items + per - 1) / per), p.batch),
+                     dim3(64 * kBoundWaves), 0, stream, p);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_key_bounds(const KeyBoundsParams& p, int head_dim, int dtype, bool fp8,
+                             hipStream_t stream) {
+  if (fp8)
+    return head_dim == 128 ? launch_bounds_t<128, Bf16Tag, 1>(p, stream)
+                           : launch_bounds_t<64, Bf16Tag, 1>(p, stream);
+  if (head_dim == 128)
+    return dtype == 0 ? launch_bounds_t<128, Bf16Tag, 2>(p, stream)
+                      : launch_bounds_t<128, F16Tag, 2>(p, stream);
+  return dtype == 0 ? launch_bounds_t<64, Bf16Tag, 2>(p, stream)
+                    : launch_bounds_t<64, F16Tag, 2>(p, stream);
+}
+
+hipError_t launch_select_blocks(const SelectParams& p, int head_dim, int dtype, bool fp8,
+                                hipStream_t stream) {
+  if (head_dim == 128)
+    return dtype == 0 ? launch_select_d<128, Bf16Tag>(p, fp8, stream)
+                      : launch_select_d<128, F16Tag>(p, fp8, stream);
+  return dtype == 0 ? launch_select_d<64, Bf16Tag>(p, fp8, stream)
+                    : launch_select_d<64, F16Tag>(p, fp8, stream);
+}
+
+}  // namespace ifa4

@@ -390,6 +390,98 @@ int32_t run_prefill_paged(const ifa4_args* a, const ifa4_paged_kv* kv, const ifa
   return e == hipSuccess ? IFA4_OK : IFA4_ELAUNCH;
 }
 
+// Checks of a call over listed blocks.
+int32_t check_sparse(const ifa4_args* a, const ifa4_paged_kv* kv, const ifa4_block_list* ls,
+                     const ifa4_kv_quant* qt) {
+  const int32_t st = check_prefill_paged(a, kv, qt);
+  if (st != IFA4_OK) return st;
+  if (ls == nullptr || ls->struct_size != sizeof(ifa4_block_list) || ls->n_select < 1 ||
+      ls->stride_t < 0 || ls->stride_h < 0)
+    return IFA4_EINVAL;
+  if (a->causal != 1 || a->n_heads / a->kv_heads > ifa4::decode_max_group())
+    return IFA4_EUNSUPPORTED;
+  if (no_queries(a)) return IFA4_OK;
+  if (ls->blocks == nullptr || !aligned(ls->blocks, 4)) return IFA4_EINVAL;
+  // rows of a list and workgroups are counted in 32 bits
+  if ((int64_t)ls->n_select * kv->block_size > (int64_t(1) << 30) ||
+      a->total_q * a->n_heads > (int64_t(1) << 28))
+    return IFA4_EUNSUPPORTED;
+  return IFA4_OK;
+}
+
+// Shares of a list, and the workspace of their partials: O, then maxima and sums.
+struct SparseLayout {
+  int32_t splits;
+  int64_t o_bytes, ml_bytes;
+  int64_t total() const { return splits > 1 ? o_bytes + ml_bytes : 0; }
+};
+SparseLayout sparse_layout(const ifa4_args* a, const ifa4_paged_kv* kv, const ifa4_block_list* ls) {
+  SparseLayout l;
+  l.splits = ifa4::sparse_splits(a->total_q * a->kv_heads, (int64_t)ls->n_select * kv->block_size);
+  const int64_t rows = l.splits * a->total_q * a->n_heads;
+  l.o_bytes = (rows * a->head_dim * 4 + 255) / 256 * 256;
+  l.ml_bytes = (rows * 8 + 255) / 256 * 256;
+  return l;
+}
+
+int32_t run_sparse(const ifa4_args* a, const ifa4_paged_kv* kv, const ifa4_block_list* ls,
+                   const ifa4_kv_quant* qt, void* workspace, size_t workspace_bytes, void* stream) {
+  const int32_t st = check_sparse(a, kv, ls, qt);
+  if (st != IFA4_OK || no_queries(a)) return st;
+  const SparseLayout l = sparse_layout(a, kv, ls);
+  if (l.total() > 0 && (workspace == nullptr || workspace_bytes < (size_t)l.total() ||
+                        !aligned(workspace, 256)))
+    return IFA4_EWORKSPACE;
+  ifa4::SparseParams p{};
+  p.q = a->q;
+  p.k = a->k;
+  p.v = a->v;
+  p.rel = a->rel;
+  p.out = a->out;
+  p.lse = a->lse;
+  p.cu_q = a->cu_seqlens_q;
+  p.seqused_k = kv->seqused_k;
+  p.block_table = kv->block_table;
+  p.blocks = ls->blocks;
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + l.o_bytes);
+  p.q_st = a->q_stride_t;
+  p.q_sh = a->q_stride_h;
+  p.k_st = a->k_stride_t;
+  p.k_sh = a->k_stride_h;
+  p.k_sblk = kv->k_stride_block;
+  p.v_st = a->v_stride_t;
+  p.v_sh = a->v_stride_h;
+  p.v_sblk = kv->v_stride_block;
+  p.rel_st = a->rel_stride_t;
+  p.rel_sh = a->rel_stride_h;
+  p.o_st = a->out_stride_t;
+  p.o_sh = a->out_stride_h;
+  p.lse_sh = a->lse_stride_h;
+  p.bt_stride = kv->block_table_stride;
+  p.ls_st = ls->stride_t;
+  p.ls_sh = ls->stride_h;
+  p.total_q = clamp_rows(a->total_q);
+  p.batch = a->batch;
+  p.n_heads = a->n_heads;
+  p.kv_heads = a->kv_heads;
+  p.group = a->n_heads / a->kv_heads;
+  p.rel_extent = a->rel_extent;
+  p.rel_dtype = a->rel_dtype;
+  p.window_left = a->window_left < (1 << 30) ? a->window_left : (1 << 30);
+  p.block_shift = __builtin_ctz((unsigned)kv->block_size);
+  p.num_blocks = kv->num_blocks;
+  p.max_blocks = kv->max_blocks_per_seq;
+  p.n_select = ls->n_select;
+  p.splits = l.splits;
+  p.kv_fp8 = qt != nullptr ? 1 : 0;
+  p.scale_log2 = a->softmax_scale * (qt != nullptr ? qt->k_scale : 1.f) * kLog2eHost;
+  p.v_scale = qt != nullptr ? qt->v_scale : 1.f;
+  const hipError_t e = ifa4::launch_sparse(p, a->head_dim, a->qkv_dtype,
+                                           static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? IFA4_OK : IFA4_ELAUNCH;
+}
+
 // Top-left causal decode (Lq = 1) sees key 0 only.
 bool key0_only(const ifa4_args* a) {
   return a->causal != 0 && (a->flags & IFA4_FLAG_BOTTOM_RIGHT) == 0;
@@ -756,6 +848,18 @@ int32_t ifa4_prefill_paged_fwd(const ifa4_args* args, const ifa4_paged_kv* kv,
                                const ifa4_kv_quant* quant, void* workspace,
                                size_t workspace_bytes, void* stream) {
   return run_prefill_paged(args, kv, quant, workspace, workspace_bytes, stream);
+}
+
+size_t ifa4_sparse_paged_workspace_bytes(const ifa4_args* args, const ifa4_paged_kv* kv,
+                                         const ifa4_block_list* list, const ifa4_kv_quant* quant) {
+  if (check_sparse(args, kv, list, quant) != IFA4_OK || no_queries(args)) return 0;
+  return (size_t)sparse_layout(args, kv, list).total();
+}
+
+int32_t ifa4_sparse_paged_fwd(const ifa4_args* args, const ifa4_paged_kv* kv,
+                              const ifa4_block_list* list, const ifa4_kv_quant* quant,
+                              void* workspace, size_t workspace_bytes, void* stream) {
+  return run_sparse(args, kv, list, quant, workspace, workspace_bytes, stream);
 }
 
 int32_t ifa4_prefill_count_tiles(const ifa4_args* args, const int32_t* cu_q, const int32_t* cu_k,

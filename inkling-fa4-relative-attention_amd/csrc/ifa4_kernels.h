@@ -211,6 +211,74 @@ constexpr int kSharedSlots = 512;  // resident workgroups, two a CU
 hipError_t launch_decode_shared(const SharedParams& p, int head_dim, int qkv_dtype,
                                 hipStream_t stream);
 
+// Bounds of the keys of a paged cache's blocks (block_select.hip).
+struct KeyBoundsParams {
+  const void* k;
+  void* bounds;              // [blocks][kv_heads][2][head_dim], of the cache's type
+  const int32_t* cu_q;
+  const int32_t* seqused_k;
+  const int32_t* block_table;
+  int64_t k_st, k_sh, k_sblk, b_sh, b_sblk, bt_stride;
+  int32_t batch, kv_heads, block_shift, num_blocks, max_blocks;
+  int32_t slots;             // blocks of a sequence that new tokens can have changed
+};
+hipError_t launch_key_bounds(const KeyBoundsParams& p, int head_dim, int dtype, bool fp8,
+                             hipStream_t stream);
+
+// The blocks that each token and kv head reads, by those bounds.
+struct SelectParams {
+  const void* q;
+  const void* bounds;
+  const int32_t* cu_q;
+  const int32_t* seqused_k;
+  const int32_t* block_table;
+  int32_t* out;              // [total_q][kv_heads][n_select]
+  uint64_t* scores;          // [total_q][kv_heads][cols] keys of the scores
+  int64_t q_st, q_sh, b_sh, b_sblk, bt_stride;
+  int32_t total_q, max_q, batch, kv_heads, group, block_shift, num_blocks, max_blocks;
+  int32_t cols;              // blocks of the longest sequence
+  int32_t n_select, sink, recent;
+  int32_t score_parts;       // workgroups that share the blocks of 16 tokens (set by the launch)
+};
+hipError_t launch_select_blocks(const SelectParams& p, int head_dim, int dtype, bool fp8,
+                                hipStream_t stream);
+
+// Attention of each token and kv head over the blocks its list names (sparse_fwd.hip).
+struct SparseParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* rel;
+  void* out;
+  float* lse;
+  const int32_t* cu_q;
+  const int32_t* seqused_k;
+  const int32_t* block_table;
+  const int32_t* blocks;     // lists, ls_st elements between tokens, ls_sh between kv heads
+  float* part_o;             // [splits][total_q][n_heads][head_dim], splits > 1
+  float2* part_ml;           // [splits][total_q][n_heads]: maximum (log2 units), sum
+  int64_t q_st, q_sh, k_st, k_sh, k_sblk, v_st, v_sh, v_sblk, rel_st, rel_sh, o_st, o_sh, lse_sh;
+  int64_t bt_stride, ls_st, ls_sh;
+  int32_t total_q, batch, n_heads, kv_heads, group;
+  int32_t rel_extent, rel_dtype, window_left;
+  int32_t block_shift, num_blocks, max_blocks;
+  int32_t n_select;
+  int32_t splits;            // workgroups that share a list
+  int32_t kv_fp8;
+  float scale_log2;          // with the K scale of an e4m3 cache
+  float v_scale;
+};
+constexpr int kSparseWaves = 4, kSparseStep = 32;
+// Workgroups that share a list of `rows` rows, for `items` (token, kv head) pairs: enough for
+// two workgroups a CU, each wave two steps at least.
+inline int32_t sparse_splits(int64_t items, int64_t rows) {
+  const int64_t most = rows / (2 * kSparseStep * kSparseWaves);
+  int64_t s = items > 0 ? 512 / items : 1;
+  if (s > most) s = most;
+  return (int32_t)(s < 1 ? 1 : s);
+}
+hipError_t launch_sparse(const SparseParams& p, int head_dim, int qkv_dtype, hipStream_t stream);
+
 // Workgroups of the backward pass, over tokens (x) and chunks of heads_per heads (y), each with a
 // row of partial weight gradients.
 struct NormRopeBwdGrid {

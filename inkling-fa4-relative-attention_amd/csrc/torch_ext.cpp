@@ -1,7 +1,7 @@
 // Thin PyTorch-ROCm binding over the C ABI (include/ifa4.h).
 //
 // Registers torch.ops.inkling_fa4.fwd / .fwd_rproj / .fwd_paged / .decode / .decode_paged /
-// .decode_shared_prefix.  The binding checks tensor
+// .decode_shared_prefix / .sparse_paged.  The binding checks tensor
 // devices, dtypes and shapes, allocates out / lse / the decode workspace from
 // torch's caching allocator, fills an ifa4_args and calls the library on the
 // current HIP stream.  No math happens here, and there is no fallback: a
@@ -336,6 +336,43 @@ std::tuple<at::Tensor, at::Tensor> fwd_paged(
   return {out, lse};
 }
 
+// Attention over the listed blocks of a paged KV cache: blocks int32 [total_q, kv_heads,
+// n_select].
+std::tuple<at::Tensor, at::Tensor> sparse_paged(
+    const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+    const at::Tensor& rel, const at::Tensor& cu_q, const at::Tensor& seqused_k,
+    const at::Tensor& block_table, const at::Tensor& blocks, int64_t max_q, int64_t max_k,
+    int64_t rel_extent, int64_t window_left, double softmax_scale, bool return_lse, double k_scale,
+    double v_scale) {
+  constexpr const char* op = "sparse_paged";
+  ifa4_paged_kv kv;
+  ifa4_args a = paged_args(op, q, k_cache, v_cache, rel, cu_q, seqused_k, block_table, max_q, max_k,
+                           rel_extent, true, window_left, softmax_scale, IFA4_FLAG_BOTTOM_RIGHT, &kv);
+  TORCH_CHECK(blocks.is_cuda() && blocks.device() == q.device() &&
+                  blocks.scalar_type() == at::kInt && blocks.dim() == 3 &&
+                  blocks.size(0) == q.size(0) && blocks.size(1) == k_cache.size(2) &&
+                  (blocks.size(2) <= 1 || blocks.stride(2) == 1) && blocks.size(2) <= INT32_MAX,
+              "inkling_fa4.", op,
+              ": blocks must be int32 [total_q, kv_heads, n_select] with contiguous lists, on q's GPU");
+  const c10::DeviceGuard guard(q.device());
+  ifa4_block_list ls{};
+  ls.struct_size = sizeof(ifa4_block_list);
+  ls.n_select = static_cast<int32_t>(blocks.size(2));
+  ls.blocks = blocks.data_ptr<int32_t>();
+  ls.stride_t = blocks.stride(0);
+  ls.stride_h = blocks.stride(1);
+  const auto [out, lse] = make_outputs(q, return_lse, &a);
+  const ifa4_kv_quant qt = kv_quant(k_scale, v_scale);
+  const ifa4_kv_quant* quant = k_cache.scalar_type() == at::kFloat8_e4m3fn ? &qt : nullptr;
+  // 0 bytes: one pass takes the call, or invalid arguments, which the call reports
+  const size_t ws_bytes = ifa4_sparse_paged_workspace_bytes(&a, &kv, &ls, quant);
+  const at::Tensor ws = ws_bytes > 0 ? empty_on(q, {(int64_t)ws_bytes}, at::kByte) : at::Tensor();
+  check_status(ifa4_sparse_paged_fwd(&a, &kv, &ls, quant, ws_bytes > 0 ? ws.data_ptr() : nullptr,
+                                     ws_bytes, c10::hip::getCurrentHIPStream(q.device().index()).stream()),
+               op);
+  return {out, lse};
+}
+
 // Decode over a paged KV cache whose first prefix_len keys are those of prefix_table for
 // every sequence; bottom-right alignment.  Same outputs as decode_paged().
 std::tuple<at::Tensor, at::Tensor> decode_shared_prefix(
@@ -399,6 +436,11 @@ TORCH_LIBRARY(inkling_fa4, m) {
       "int max_seqlen_k, int rel_extent, bool causal, int window_left, float softmax_scale, "
       "bool return_lse, float k_scale, float v_scale) -> (Tensor, Tensor)");
   m.def(
+      "sparse_paged(Tensor q, Tensor k_cache, Tensor v_cache, Tensor rel_logits, "
+      "Tensor cu_seqlens_q, Tensor seqused_k, Tensor block_table, Tensor blocks, "
+      "int max_seqlen_q, int max_seqlen_k, int rel_extent, int window_left, float softmax_scale, "
+      "bool return_lse, float k_scale, float v_scale) -> (Tensor, Tensor)");
+  m.def(
       "decode_shared_prefix(Tensor q, Tensor k_cache, Tensor v_cache, Tensor rel_logits, "
       "Tensor cu_seqlens_q, Tensor seqused_k, Tensor block_table, Tensor prefix_table, "
       "int prefix_len, int max_seqlen_q, int max_seqlen_k, int rel_extent, int window_left, "
@@ -411,5 +453,6 @@ TORCH_LIBRARY_IMPL(inkling_fa4, CUDA, m) {
   m.impl("decode", &decode);
   m.impl("decode_paged", &decode_paged);
   m.impl("fwd_paged", &fwd_paged);
+  m.impl("sparse_paged", &sparse_paged);
   m.impl("decode_shared_prefix", &decode_shared_prefix);
 }

@@ -126,12 +126,42 @@ class Ifa4KvAppend(ctypes.Structure):
     ]
 
 
+class Ifa4KeyBounds(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32), ("kv_dtype", _c_int32), ("head_dim", _c_int32),
+        ("kv_heads", _c_int32), ("batch", _c_int32), ("max_seqlen_q", _c_int32),
+        ("k_cache", _vp), ("k_stride_t", _c_int64), ("k_stride_h", _c_int64),
+        ("bounds", _vp), ("bounds_stride_block", _c_int64), ("bounds_stride_h", _c_int64),
+        ("cu_seqlens", _vp),
+    ]
+
+
+class Ifa4BlockSelect(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32), ("dtype", _c_int32), ("kv_dtype", _c_int32),
+        ("head_dim", _c_int32), ("n_heads", _c_int32), ("kv_heads", _c_int32), ("batch", _c_int32),
+        ("max_seqlen_q", _c_int32), ("max_seqlen_k", _c_int32), ("n_select", _c_int32),
+        ("sink_blocks", _c_int32), ("recent_blocks", _c_int32), ("total_q", _c_int64),
+        ("q", _vp), ("q_stride_t", _c_int64), ("q_stride_h", _c_int64),
+        ("bounds", _vp), ("bounds_stride_block", _c_int64), ("bounds_stride_h", _c_int64),
+        ("cu_seqlens", _vp), ("blocks", _vp),
+    ]
+
+
+class Ifa4BlockList(ctypes.Structure):
+    _fields_ = [("struct_size", ctypes.c_uint32), ("n_select", _c_int32), ("blocks", _vp),
+                ("stride_t", _c_int64), ("stride_h", _c_int64)]
+
+
 _P_ARGS = ctypes.POINTER(Ifa4Args)
 _P_PAGED = ctypes.POINTER(Ifa4PagedKV)
 _P_QUANT = ctypes.POINTER(Ifa4KvQuant)
 _P_TILE = ctypes.POINTER(Ifa4Tile)
 _P_SHARED = ctypes.POINTER(Ifa4SharedPrefix)
 _P_NORM = ctypes.POINTER(Ifa4NormRope)
+_P_BOUNDS = ctypes.POINTER(Ifa4KeyBounds)
+_P_SELECT = ctypes.POINTER(Ifa4BlockSelect)
+_P_LIST = ctypes.POINTER(Ifa4BlockList)
 _P_I32 = ctypes.POINTER(ctypes.c_int32)
 _P_I64 = ctypes.POINTER(ctypes.c_int64)
 
@@ -165,6 +195,12 @@ SIGNATURES = {
     "ifa4_prefill_paged_workspace_bytes": (ctypes.c_size_t, [_P_ARGS, _P_PAGED, _P_QUANT]),
     "ifa4_prefill_paged_fwd": (_c_int32, [_P_ARGS, _P_PAGED, _P_QUANT, _vp, ctypes.c_size_t,
                                           _vp]),
+    "ifa4_key_bounds_paged": (_c_int32, [_P_BOUNDS, _P_PAGED, _vp]),
+    "ifa4_select_blocks_workspace_bytes": (ctypes.c_size_t, [_P_SELECT, _P_PAGED]),
+    "ifa4_select_blocks_paged": (_c_int32, [_P_SELECT, _P_PAGED, _vp, ctypes.c_size_t, _vp]),
+    "ifa4_sparse_paged_workspace_bytes": (ctypes.c_size_t, [_P_ARGS, _P_PAGED, _P_LIST, _P_QUANT]),
+    "ifa4_sparse_paged_fwd": (_c_int32, [_P_ARGS, _P_PAGED, _P_LIST, _P_QUANT, _vp,
+                                         ctypes.c_size_t, _vp]),
     "ifa4_qk_norm_rope_fwd": (_c_int32, [_P_NORM, _vp]),
     "ifa4_qk_norm_rope_bwd_workspace_bytes": (ctypes.c_size_t, [_P_NORM]),
     "ifa4_qk_norm_rope_bwd": (_c_int32, [_P_NORM, ctypes.POINTER(Ifa4NormRopeGrad), _vp,
@@ -254,6 +290,21 @@ def make_norm_rope_grad(**kw):
 def make_kv_append(**kw):
     """Ifa4KvAppend with struct_size filled and scales 1, fields from kw."""
     return _filled(Ifa4KvAppend, dict({"k_scale": 1.0, "v_scale": 1.0}, **kw))
+
+
+def make_key_bounds(**kw):
+    """Ifa4KeyBounds with struct_size filled, fields from kw."""
+    return _filled(Ifa4KeyBounds, kw)
+
+
+def make_block_select(**kw):
+    """Ifa4BlockSelect with struct_size filled and one recent block, fields from kw."""
+    return _filled(Ifa4BlockSelect, dict({"recent_blocks": 1}, **kw))
+
+
+def make_block_list(**kw):
+    """Ifa4BlockList with struct_size filled, fields from kw."""
+    return _filled(Ifa4BlockList, kw)
 
 
 def prefill_tile(head_dim, batch=0, n_heads=1, seq_len=0, causal=True):

@@ -70,15 +70,20 @@ _is_grad_enabled = torch.is_grad_enabled
 _overloads = {}
 
 
+def _op(name):
+    op = _overloads.get(name)
+    if op is None:
+        op = _overloads[name] = getattr(_ops(), name).default
+    return op
+
+
 def _call(name, *args):
     """torch.ops.inkling_fa4.<name> with gradients off: the operators have no
     backward, and their outputs never require one.  Small calls are bound by the
     host (a short prompt or cache computes in less time than it takes to issue),
     so the mode is switched, which costs a tenth of such a call, only when one of
     the floating-point inputs (the first five arguments hold them) asks for a gradient."""
-    op = _overloads.get(name)
-    if op is None:
-        op = _overloads[name] = getattr(_ops(), name).default
+    op = _overloads.get(name) or _op(name)
     if _is_grad_enabled():
         q, k, v, rel, w = args[:5]
         try:

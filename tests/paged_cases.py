@@ -103,8 +103,8 @@ class Case:
             see &= dist <= self.window
         return see, dist
 
-    def named(self, b, h):
-        """Keys that the queries of a sequence may see beside the masks (None: all)."""
+    def times(self, b, h):
+        """[queries, keys]: how often a query counts a key that the masks leave it (None: once)."""
         return None
 
     def check(self, got, seqs=None):
@@ -121,8 +121,8 @@ class Case:
             for kvh in range(self.hkv):
                 k, v = (self.rows(c, s, b, kvh)
                         for c, s in zip((self.kc, self.vc), self.scales))
-                named = self.named(b, kvh)
-                sees = see if named is None else see & named
+                times = self.times(b, kvh)
+                sees = see if times is None else see & (times > 0)
                 for head in range(kvh * group, (kvh + 1) * group):
                     o, ls = out[mine, head].double(), lse[head, mine].double()
                     if lk == 0:
@@ -135,6 +135,8 @@ class Case:
                         rel = self.rel[mine, head].double()
                         x = x + torch.where(
                             band, rel.gather(1, dist.clamp(0, self.extent - 1)), 0.0)
+                    if times is not None:
+                        x = x + times.double().clamp(min=1).log()
                     x = x.masked_fill(~sees, -math.inf)
                     want_lse = torch.logsumexp(x, -1)
                     live = want_lse > -math.inf
