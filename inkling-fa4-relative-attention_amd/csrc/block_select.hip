@@ -167,6 +167,14 @@ __device__ __forceinline__ int token_blocks(const SelectParams& p, const TokenSp
 // l % 16), held in registers over the blocks; C (lane l, register r) = block 4 r + l / 16, token
 // l % 16.
 constexpr int kScoreWaves = 4;
+#ifndef SCORE_GROUPS
+#define SCORE_GROUPS 1024
+#endif
+constexpr int kScoreGroups = SCORE_GROUPS;
+#ifndef STEP_TOKENS
+#define STEP_TOKENS 4
+#endif
+constexpr int kStepTokens = STEP_TOKENS;
 template <int D, typename Tag, int Eb>
 __global__ __launch_bounds__(64 * kScoreWaves) void score_tile_kernel(SelectParams p) {
   constexpr int kEpc = 16 / Eb;                // elements of a 16-byte chunk
@@ -248,16 +256,129 @@ __global__ __launch_bounds__(64 * kScoreWaves) void score_tile_kernel(SelectPara
   }
 }
 
+// One token of a sequence against its blocks, on the vector unit: a lane group of 8 takes a block
+// (lane `sub`: the chunks sub modulo 8), qn and qp of a lane's elements stay in registers, a wave
+// walks over 64 blocks (one load of their table entries), the next 8 blocks' bounds in flight
+// while 8 are summed.
+constexpr int kStepBlocks = 64;  // of a wave
+template <int Ctrl>
+__device__ __forceinline__ double dpp_add(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_mov_dpp((int)b, Ctrl, 0xf, 0xf, true);
+  const uint32_t hi = __builtin_amdgcn_mov_dpp((int)(b >> 32), Ctrl, 0xf, 0xf, true);
+  return x + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+template <int D, typename Tag, int Eb>
+__global__ __launch_bounds__(64 * kScoreWaves) void score_step_kernel(SelectParams p) {
+  constexpr int kEpc = 16 / Eb;              // elements of a 16-byte chunk
+  constexpr int kHalf = D / kEpc;            // chunks of lo, and of hi
+  constexpr int kChunks = 2 * kHalf / 8;     // of a lane
+  const int lane = threadIdx.x & 63, wave = (int)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int seq = blockIdx.y;
+  const int part0 = blockIdx.x % p.score_parts, rest = blockIdx.x / p.score_parts;
+  const int h = rest % p.kv_heads, i0 = rest / p.kv_heads;
+  const TokenSpan s = token_span(p, seq);
+  if (i0 >= s.len) return;
+  const int nb = token_blocks(p, s, i0);
+  if (nb <= p.n_select) return;
+  const int last = nb - p.recent;
+  const int first = p.sink + (part0 * kScoreWaves + wave) * kStepBlocks;
+  if (first >= last) return;
+  const int sub = lane & 7, row = lane >> 3;
+  const int ent_mine = p.block_table[seq * p.bt_stride + min(first + lane, nb - 1)];
+
+  const int64_t tok = s.start + i0;
+  const char* const q_row = static_cast<const char*>(p.q) +
+                            (tok * p.q_st + (int64_t)h * p.group * p.q_sh) * 2;
+  double q[kChunks][kEpc];
+#pragma unroll
+  for (int i = 0; i < kChunks; ++i)
+#pragma unroll
+    for (int e = 0; e < kEpc; ++e) q[i][e] = 0.0;
+  // chunk c: elements d = kEpc (c % kHalf) .., of lo for c < kHalf, else of hi
+  for (int head = 0; head < p.group; ++head) {
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      const int c = sub + 8 * i;
+      const bool up = c >= kHalf;
+      const int d = kEpc * (c & (kHalf - 1));
+#pragma unroll
+      for (int part = 0; part < kEpc / 8; ++part) {
+        float f[8];
+        unpack16<Tag, 2>(ld_global_16(q_row + (head * p.q_sh + d + 8 * part) * 2), f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = up ? f[e] : -f[e];
+          q[i][8 * part + e] += (double)(x < 0.f ? 0.f : f[e]);  // a NaN in both
+        }
+      }
+    }
+  }
+
+  const char* const bounds = static_cast<const char*>(p.bounds) + (int64_t)h * p.b_sh * Eb + 16 * sub;
+  auto load = [&](int it, u32x4_t* w) {
+    const int ent = __shfl(ent_mine, 8 * it + row);
+    const bool good = (uint32_t)ent < (uint32_t)p.num_blocks;
+    const char* src = bounds + (int64_t)(good ? ent : 0) * p.b_sblk * Eb;
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      w[i] = ld_global_16(src + 128 * i);
+      if (!good) w[i] = u32x4_t{0u, 0u, 0u, 0u};
+    }
+  };
+  uint64_t* const dst = p.scores + ((tok * p.kv_heads + h) * (int64_t)p.cols + first);
+  auto sum = [&](int it, const u32x4_t* w) {
+    double acc[2] = {0.0, 0.0};
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      float f[kEpc];
+      unpack16<Tag, Eb>(w[i], f);
+#pragma unroll
+      for (int e = 0; e < kEpc; ++e) acc[e & 1] = fma((double)f[e], q[i][e], acc[e & 1]);
+    }
+    double x = acc[0] + acc[1];
+    x = dpp_add<0xb1>(x);   // lane ^ 1
+    x = dpp_add<0x4e>(x);   // lane ^ 2
+    x = dpp_add<0x141>(x);  // the other four of eight
+    if (sub == 0 && first + 8 * it + row < last) dst[8 * it + row] = score_key(x);
+  };
+  const int its = min(kStepBlocks / 8, (last - first + 7) / 8);
+  u32x4_t a[kChunks], b[kChunks];
+  load(0, a);
+  for (int it = 0; it < its; it += 2) {
+    if (it + 1 < its) load(it + 1, b);
+    sum(it, a);
+    if (it + 1 >= its) break;
+    if (it + 2 < its) load(it + 2, a);
+    sum(it + 1, b);
+  }
+}
+
 // ---- choice ----------------------------------------------------------------------------------
-// One workgroup per (token, kv head): the n_free best of the competing blocks by a radix select
-// over their keys, 8 bits at a time from the top until the keys that share the border's digits
-// are all taken or all digits are used; then the list in ascending order, by a prefix sum over
-// the blocks.
-constexpr int kPickThreads = 256;
+// One workgroup per (token, kv head).  The border of the n_free best competing blocks is found by
+// halving the keys' range by 1024 at a time, from least to greatest: count the keys of each of
+// 1024 equal parts, keep the part that holds the border, until all its keys are taken, they are
+// few enough to rank one against another, or they are all equal.  Scores spread over a range, so
+// one count mostly leaves a handful.  Then the list in ascending order by a prefix sum over the
+// blocks: a thread holds kPer consecutive ones, a workgroup kRound (kOne: they stay in registers
+// from pass to pass; longer rows are read again).
+constexpr int kPickThreads = 256, kPer = 8, kRound = kPickThreads * kPer, kBins = 1024;
+constexpr int kRankMost = 64;
+__device__ __forceinline__ uint64_t shfl_xor64(uint64_t x, int off) {
+  return (uint64_t)(uint32_t)__shfl_xor((int)(x >> 32), off) << 32 | (uint32_t)__shfl_xor((int)x, off);
+}
+template <bool kOne>
 __global__ __launch_bounds__(kPickThreads) void pick_blocks_kernel(SelectParams p) {
-  __shared__ int hist[256];
-  __shared__ int sums[2][kPickThreads / 64 + 1];
+  constexpr int kPickWaves = kPickThreads / 64;
+  __shared__ int hist[kBins];
+  __shared__ uint64_t ends[2][kPickWaves];
+  __shared__ int sums[kPickWaves];
   __shared__ int border[2];
+  __shared__ uint64_t few_key[kRankMost];
+  __shared__ int few_at[kRankMost];
+  __shared__ int few_n;
+  __shared__ uint64_t top_key;
+  __shared__ int top_equal;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = blockIdx.x;
   const int t = (int)(row / p.kv_heads);
@@ -278,78 +399,189 @@ __global__ __launch_bounds__(kPickThreads) void pick_blocks_kernel(SelectParams 
     for (int i = tid; i < p.n_select; i += kPickThreads) list[i] = i < nb ? i : -1;
     return;
   }
-  const int first = p.sink, last = nb - p.recent;
-  int need = p.n_select - p.sink - p.recent;  // of the competing blocks [first, last)
-  const uint64_t* const keys = p.scores + row * (int64_t)p.cols;
-  uint64_t prefix = 0;  // the border's digits found so far, shifted down
-  int shift = 64;       // by so much
-  while (shift > 0 && need > 0) {
-    shift -= 8;
-    hist[tid] = 0;
-    __syncthreads();
-    for (int b = first + tid; b < last; b += kPickThreads) {
-      const uint64_t k = keys[b];
-      if (shift == 56 || (k >> (shift + 8)) == prefix) atomicAdd(&hist[(int)(k >> shift) & 255], 1);
+  for (int i = tid; i < p.sink; i += kPickThreads) list[i] = i;
+  for (int i = tid; i < p.recent; i += kPickThreads)
+    list[p.n_select - p.recent + i] = nb - p.recent + i;
+  const int first = p.sink, n = nb - p.recent - p.sink;  // competing blocks, n > 0
+  int need = p.n_select - p.sink - p.recent;
+  if (need == 0) return;
+  const uint64_t* const keys = p.scores + row * (int64_t)p.cols + first;
+  uint64_t mine[kPer];
+  auto load = [&](int r0) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int b = r0 + tid * kPer + i;
+      mine[i] = b < n ? keys[b] : 0;
     }
+  };
+  const int rounds = kOne ? 1 : (n + kRound - 1) / kRound;
+  if constexpr (kOne) load(0);
+  // every key of the row, in any order
+  auto each = [&](auto&& f) {
+    for (int r = 0; r < rounds; ++r) {
+      if constexpr (!kOne) load(r * kRound);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (r * kRound + tid * kPer + i < n) f(mine[i], r * kRound + tid * kPer + i);
+    }
+  };
+
+  uint64_t lo = ~uint64_t(0), hi = 0;
+  each([&](uint64_t k, int) {
+    lo = k < lo ? k : lo;
+    hi = k > hi ? k : hi;
+  });
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const uint64_t a = shfl_xor64(lo, off), b = shfl_xor64(hi, off);
+    lo = a < lo ? a : lo;
+    hi = b > hi ? b : hi;
+  }
+  if (lane == 0) {
+    ends[0][wave] = lo;
+    ends[1][wave] = hi;
+  }
+  if (tid == 0) few_n = 0;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kPickWaves; ++w) {
+    lo = ends[0][w] < lo ? ends[0][w] : lo;
+    hi = ends[1][w] > hi ? ends[1][w] : hi;
+  }
+
+  uint64_t top;   // keys above it are taken,
+  int equal;      // and so many of those equal to it, the lower blocks
+  while (true) {
+    if (lo == hi) {
+      top = lo;
+      equal = need;
+      break;
+    }
+    const int bits = 64 - __builtin_clzll(hi - lo);
+    const int shift = bits > 10 ? bits - 10 : 0;
+#pragma unroll
+    for (int i = 0; i < kBins / kPickThreads; ++i) hist[tid + i * kPickThreads] = 0;
     __syncthreads();
-    // digit of the border: greater digits hold fewer than need, with it as many or more
-    const int mine = hist[255 - tid];
-    int incl = mine;
+    each([&](uint64_t k, int) {
+      if (k >= lo && k <= hi) atomicAdd(&hist[(int)((k - lo) >> shift)], 1);
+    });
+    __syncthreads();
+    // thread t holds the bins kBins - 4 t - 4 .. + 3: counts from the top
+    constexpr int kMine = kBins / kPickThreads;
+    int c[kMine], total = 0;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      c[i] = hist[kBins - 1 - tid * kMine - i];
+      total += c[i];
+    }
+    int incl = total;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
       const int up = __shfl_up(incl, off);
       if (lane >= off) incl += up;
     }
-    if (lane == 63) sums[0][wave] = incl;
+    if (lane == 63) sums[wave] = incl;
     __syncthreads();
-    for (int w = 0; w < wave; ++w) incl += sums[0][w];
-    if (incl - mine < need && incl >= need) {
-      border[0] = 255 - tid;
-      border[1] = need - (incl - mine);
-    }
-    __syncthreads();
-    const int digit = border[0];
-    const int all = hist[digit];
-    need = border[1];
-    prefix = prefix << 8 | (uint64_t)digit;
-    __syncthreads();
-    if (need == all) break;  // every key with these digits is taken
-  }
-  // taken: digits above the border's, and of the border's the first `need`
-  for (int i = tid; i < p.sink; i += kPickThreads) list[i] = i;
-  for (int i = tid; i < p.recent; i += kPickThreads) list[p.n_select - p.recent + i] = last + i;
-  int at = p.sink, equal = 0;  // places filled and border keys met before this round
-  for (int b0 = first; b0 < last; b0 += kPickThreads) {
-    const int b = b0 + tid;
-    bool above = false, same = false;
-    if (b < last && shift < 64) {
-      const uint64_t k = keys[b] >> shift;
-      above = k > prefix;
-      same = k == prefix;
-    }
-    const uint64_t ma = __builtin_amdgcn_ballot_w64(above), ms = __builtin_amdgcn_ballot_w64(same);
-    __syncthreads();
-    if (lane == 0) {
-      sums[0][wave] = __builtin_popcountll(ma);
-      sums[1][wave] = __builtin_popcountll(ms);
-    }
-    __syncthreads();
-    int a = 0, e = 0, a_all = 0, e_all = 0;
 #pragma unroll
-    for (int w = 0; w < kPickThreads / 64; ++w) {
-      if (w < wave) {
-        a += sums[0][w];
-        e += sums[1][w];
+    for (int w = 0; w < kPickWaves; ++w)
+      if (w < wave) incl += sums[w];
+    int above = incl - total;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      if (above < need && above + c[i] >= need) {
+        border[0] = kBins - 1 - tid * kMine - i;
+        border[1] = above;
       }
-      a_all += sums[0][w];
-      e_all += sums[1][w];
+      above += c[i];
     }
-    const uint64_t below = (uint64_t(1) << lane) - 1;
-    a += __builtin_popcountll(ma & below);
-    e += equal + __builtin_popcountll(ms & below);
-    if (above || (same && e < need)) list[at + a + min(e, need) - min(equal, need)] = b;
-    at += a_all + min(equal + e_all, need) - min(equal, need);
-    equal += e_all;
+    __syncthreads();
+    const int bin = border[0];
+    const int held = hist[bin];
+    need -= border[1];
+    lo += (uint64_t)bin << shift;
+    const uint64_t span = (uint64_t(1) << shift) - 1;  // lo + span may lie past 64 bits
+    hi = hi - lo < span ? hi : lo + span;
+    if (held == need) {  // all of them: keys >= lo
+      top = lo - 1;      // (lo > 0: some key lies below the border's part, or lo is the least key)
+      equal = 0;
+      if (lo == 0) {
+        top = 0;
+        equal = need;
+      }
+      break;
+    }
+    if (held <= kRankMost) {
+      each([&](uint64_t k, int b) {
+        if (k >= lo && k <= hi) {
+          const int i = atomicAdd(&few_n, 1);
+          few_key[i] = k;
+          few_at[i] = b;
+        }
+      });
+      __syncthreads();
+      if (wave == 0) {
+        const uint64_t k = lane < held ? few_key[lane] : 0;
+        const int at = lane < held ? few_at[lane] : 0;
+        int rank = 0, same = 0;  // keys before mine, and of them those equal to it
+        for (int i = 0; i < held; ++i) {
+          const uint64_t o = few_key[i];
+          const bool before = o == k && few_at[i] < at;
+          same += before;
+          rank += before || o > k;
+        }
+        if (lane < held && rank == need - 1) {
+          top_key = k;
+          top_equal = same + 1;
+        }
+      }
+      __syncthreads();
+      top = top_key;
+      equal = top_equal;
+      break;
+    }
+    __syncthreads();  // hist is cleared again
+  }
+
+  // the list: blocks with keys above `top`, and the first `equal` of those equal to it
+  int at = p.sink, met = 0;  // places filled, keys equal to top met
+  for (int r = 0; r < rounds; ++r) {
+    if constexpr (!kOne) load(r * kRound);
+    int a = 0, e = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const bool in = r * kRound + tid * kPer + i < n;
+      a += in && mine[i] > top;
+      e += in && mine[i] == top;
+    }
+    int incl = a | e << 16;  // at most kRound of either
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int up = __shfl_up(incl, off);
+      if (lane >= off) incl += up;
+    }
+    __syncthreads();
+    if (lane == 63) sums[wave] = incl;
+    __syncthreads();
+    int all = 0;
+#pragma unroll
+    for (int w = 0; w < kPickWaves; ++w) {
+      if (w < wave) incl += sums[w];
+      all += sums[w];
+    }
+    int ab = (incl & 0xffff) - a, eb = met + (incl >> 16) - e;  // before this thread's
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int b = r * kRound + tid * kPer + i;
+      if (b < n) {
+        const bool above = mine[i] > top, same = mine[i] == top;
+        if (above || (same && eb < equal))
+          list[at + ab + min(eb, equal) - min(met, equal)] = first + b;
+        ab += above;
+        eb += same;
+      }
+    }
+    at += (all & 0xffff) + min(met + (all >> 16), equal) - min(met, equal);
+    met += all >> 16;
   }
 }
 
@@ -357,19 +589,31 @@ template <int D, typename Tag, int Eb>
 hipError_t launch_select_t(const SelectParams& p_in, hipStream_t stream) {
   SelectParams p = p_in;
   if (p.cols > p.n_select) {
-    const int tiles = (p.cols + 15) / 16, q_tiles = (p.max_q + 15) / 16;
-    // waves take one tile of 16 blocks each, more where there are many tokens
-    const int per = (tiles + kScoreWaves - 1) / kScoreWaves;
-    const int64_t others = (int64_t)q_tiles * p.kv_heads * p.batch;
-    p.score_parts = (int)max(int64_t(1), min((int64_t)per, 4096 / max(int64_t(1), others)));
-    hipLaunchKernelGGL((score_tile_kernel<D, Tag, Eb>),
-                       dim3((unsigned)((int64_t)p.score_parts * q_tiles * p.kv_heads), p.batch),
-                       dim3(64 * kScoreWaves), 0, stream, p);
-    const hipError_t e = hipGetLastError();
+    hipError_t e;
+    if (p.max_q <= kStepTokens) {
+      p.score_parts = (p.cols + kStepBlocks * kScoreWaves - 1) / (kStepBlocks * kScoreWaves);
+      hipLaunchKernelGGL((score_step_kernel<D, Tag, Eb>),
+                         dim3((unsigned)((int64_t)p.score_parts * p.max_q * p.kv_heads), p.batch),
+                         dim3(64 * kScoreWaves), 0, stream, p);
+    } else {
+      const int tiles = (p.cols + 15) / 16, q_tiles = (p.max_q + 15) / 16;
+      // workgroups for every tile of blocks, or two rounds of them where there are many tokens:
+      // each begins with the sums over its query heads
+      const int per = (tiles + kScoreWaves - 1) / kScoreWaves;
+      const int64_t others = (int64_t)q_tiles * p.kv_heads * p.batch;
+      p.score_parts = (int)max(int64_t(1), min((int64_t)per, kScoreGroups / max(int64_t(1), others)));
+      hipLaunchKernelGGL((score_tile_kernel<D, Tag, Eb>),
+                         dim3((unsigned)((int64_t)p.score_parts * q_tiles * p.kv_heads), p.batch),
+                         dim3(64 * kScoreWaves), 0, stream, p);
+    }
+    e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL(pick_blocks_kernel, dim3((unsigned)((int64_t)p.total_q * p.kv_heads)),
-                     dim3(kPickThreads), 0, stream, p);
+  const dim3 grid((unsigned)((int64_t)p.total_q * p.kv_heads));
+  if (p.cols <= kRound)
+    hipLaunchKernelGGL(pick_blocks_kernel<true>, grid, dim3(kPickThreads), 0, stream, p);
+  else
+    hipLaunchKernelGGL(pick_blocks_kernel<false>, grid, dim3(kPickThreads), 0, stream, p);
   return hipGetLastError();
 }
 
