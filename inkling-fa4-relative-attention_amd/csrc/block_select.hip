@@ -168,7 +168,7 @@ __device__ __forceinline__ int token_blocks(const SelectParams& p, const TokenSp
 // l % 16.
 constexpr int kScoreWaves = 4;
 #ifndef SCORE_GROUPS
-#define SCORE_GROUPS 1024
+#define SCORE_GROUPS 512
 #endif
 constexpr int kScoreGroups = SCORE_GROUPS;
 #ifndef STEP_TOKENS
@@ -191,32 +191,42 @@ __global__ __launch_bounds__(64 * kScoreWaves) void score_tile_kernel(SelectPara
   if (most <= p.n_select) return;
   const int last = most - p.recent;  // blocks [sink, last) compete for the tile's last token
   int tile = (p.sink >> 4) + part0 * kScoreWaves + wave;
-  if (tile * 16 >= last) return;
+  if ((tile - wave) * 16 >= last) return;
 
+  // qn and qp of the 16 tokens, summed over the heads by the four waves together (8 elements of
+  // a lane each, in units of 8)
+  constexpr int kUnits = D / 32;
+  __shared__ __align__(16) double q_lds[2 * kUnits][64][8];
+  const int64_t tok = s.start + min(i0 + m, s.len - 1);
+  const char* const q_row = static_cast<const char*>(p.q) +
+                            (tok * p.q_st + (int64_t)h * p.group * p.q_sh) * 2;
+  if (wave < kUnits) {
+    const int d = kEpc * (4 * (wave / (kEpc / 8)) + g) + 8 * (wave % (kEpc / 8));
+    double neg[8], up[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) neg[e] = up[e] = 0.0;
+    for (int head = 0; head < p.group; ++head) {
+      float f[8];
+      unpack16<Tag, 2>(ld_global_16(q_row + (head * p.q_sh + d) * 2), f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        neg[e] += (double)(f[e] > 0.f ? 0.f : f[e]);  // a NaN in both
+        up[e] += (double)(f[e] < 0.f ? 0.f : f[e]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      q_lds[wave][lane][e] = neg[e];
+      q_lds[kUnits + wave][lane][e] = up[e];
+    }
+  }
+  __syncthreads();
+  if (tile * 16 >= last) return;
   double q[kChunks][kEpc];
 #pragma unroll
   for (int i = 0; i < kChunks; ++i)
 #pragma unroll
-    for (int e = 0; e < kEpc; ++e) q[i][e] = 0.0;
-  const int64_t tok = s.start + min(i0 + m, s.len - 1);
-  const char* const q_row = static_cast<const char*>(p.q) +
-                            (tok * p.q_st + (int64_t)h * p.group * p.q_sh) * 2;
-  for (int head = 0; head < p.group; ++head) {
-#pragma unroll
-    for (int i = 0; i < kChunks / 2; ++i) {
-      const int d = kEpc * (4 * i + g);
-#pragma unroll
-      for (int part = 0; part < kEpc / 8; ++part) {
-        float f[8];
-        unpack16<Tag, 2>(ld_global_16(q_row + (head * p.q_sh + d + 8 * part) * 2), f);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          q[i][8 * part + e] += (double)(f[e] > 0.f ? 0.f : f[e]);  // a NaN in both
-          q[i + kChunks / 2][8 * part + e] += (double)(f[e] < 0.f ? 0.f : f[e]);
-        }
-      }
-    }
-  }
+    for (int e = 0; e < kEpc; ++e) q[i][e] = q_lds[i * (kEpc / 8) + e / 8][lane][e % 8];
 
   const int32_t* const table = p.block_table + seq * p.bt_stride;
   auto load = [&](int t, u32x4_t* w) {
@@ -236,15 +246,18 @@ __global__ __launch_bounds__(64 * kScoreWaves) void score_tile_kernel(SelectPara
   load(tile, w);
   for (; tile * 16 < last; tile += step) {
     if ((tile + step) * 16 < last) load(tile + step, next);
-    f64x4_t acc = {0.0, 0.0, 0.0, 0.0};
+    f64x4_t acc = {0.0, 0.0, 0.0, 0.0}, acc1 = acc;
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
       float f[kEpc];
       unpack16<Tag, Eb>(w[i], f);
 #pragma unroll
-      for (int e = 0; e < kEpc; ++e)
+      for (int e = 0; e < kEpc; e += 2) {
         acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)f[e], q[i][e], acc, 0, 0, 0);
+        acc1 = __builtin_amdgcn_mfma_f64_16x16x4f64((double)f[e + 1], q[i][e + 1], acc1, 0, 0, 0);
+      }
     }
+    acc += acc1;
     if (i0 + m < s.len) {
       uint64_t* const dst = p.scores + ((tok * p.kv_heads + h) * (int64_t)p.cols + 16 * tile + g);
 #pragma unroll

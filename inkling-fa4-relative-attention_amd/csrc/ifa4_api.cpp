@@ -411,14 +411,14 @@ int32_t check_sparse(const ifa4_args* a, const ifa4_paged_kv* kv, const ifa4_blo
 
 // Shares of a list, and the workspace of their partials: O, then maxima and sums.
 struct SparseLayout {
-  int32_t splits;
+  ifa4::SparsePlan plan;
   int64_t o_bytes, ml_bytes;
-  int64_t total() const { return splits > 1 ? o_bytes + ml_bytes : 0; }
+  int64_t total() const { return plan.splits > 1 ? o_bytes + ml_bytes : 0; }
 };
 SparseLayout sparse_layout(const ifa4_args* a, const ifa4_paged_kv* kv, const ifa4_block_list* ls) {
   SparseLayout l;
-  l.splits = ifa4::sparse_splits(a->total_q * a->kv_heads, (int64_t)ls->n_select * kv->block_size);
-  const int64_t rows = l.splits * a->total_q * a->n_heads;
+  l.plan = ifa4::sparse_plan(a->total_q * a->kv_heads, (int64_t)ls->n_select * kv->block_size);
+  const int64_t rows = l.plan.splits * a->total_q * a->n_heads;
   l.o_bytes = (rows * a->head_dim * 4 + 255) / 256 * 256;
   l.ml_bytes = (rows * 8 + 255) / 256 * 256;
   return l;
@@ -473,7 +473,8 @@ int32_t run_sparse(const ifa4_args* a, const ifa4_paged_kv* kv, const ifa4_block
   p.num_blocks = kv->num_blocks;
   p.max_blocks = kv->max_blocks_per_seq;
   p.n_select = ls->n_select;
-  p.splits = l.splits;
+  p.waves = l.plan.waves;
+  p.splits = l.plan.splits;
   p.kv_fp8 = qt != nullptr ? 1 : 0;
   p.scale_log2 = a->softmax_scale * (qt != nullptr ? qt->k_scale : 1.f) * kLog2eHost;
   p.v_scale = qt != nullptr ? qt->v_scale : 1.f;

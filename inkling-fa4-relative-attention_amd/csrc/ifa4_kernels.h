@@ -263,19 +263,30 @@ struct SparseParams {
   int32_t rel_extent, rel_dtype, window_left;
   int32_t block_shift, num_blocks, max_blocks;
   int32_t n_select;
-  int32_t splits;            // workgroups that share a list
+  int32_t waves, splits;     // waves of a workgroup, workgroups that share a list
   int32_t kv_fp8;
   float scale_log2;          // with the K scale of an e4m3 cache
   float v_scale;
 };
-constexpr int kSparseWaves = 4, kSparseStep = 32;
-// Workgroups that share a list of `rows` rows, for `items` (token, kv head) pairs: enough for
-// two workgroups a CU, each wave two steps at least.
-inline int32_t sparse_splits(int64_t items, int64_t rows) {
-  const int64_t most = rows / (2 * kSparseStep * kSparseWaves);
-  int64_t s = items > 0 ? 512 / items : 1;
-  if (s > most) s = most;
-  return (int32_t)(s < 1 ? 1 : s);
+constexpr int kSparseStep = 32;
+// Waves that share a list of `rows` rows, for `items` (token, kv head) pairs: enough of them in all
+// to fill the chip (IFA4_SPARSE_WAVES), each with two steps at least; up to 8 in a workgroup, the
+// rest as workgroups whose partials a second pass joins.
+#ifndef IFA4_SPARSE_WAVES
+#define IFA4_SPARSE_WAVES 2048
+#endif
+struct SparsePlan {
+  int32_t waves, splits;
+};
+inline SparsePlan sparse_plan(int64_t items, int64_t rows) {
+  const int64_t steps = (rows + kSparseStep - 1) / kSparseStep;
+  int64_t want = items > 0 ? (IFA4_SPARSE_WAVES + items - 1) / items : 1;
+  if (want > steps / 2) want = steps / 2;
+  SparsePlan pl{1, 1};
+  while (pl.waves < 8 && 2 * pl.waves <= want) pl.waves *= 2;
+  const int64_t s = want / pl.waves;
+  pl.splits = (int32_t)(s < 1 ? 1 : s);
+  return pl;
 }
 hipError_t launch_sparse(const SparseParams& p, int head_dim, int qkv_dtype, hipStream_t stream);
 
