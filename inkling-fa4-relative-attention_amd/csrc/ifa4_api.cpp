@@ -475,6 +475,13 @@ int32_t run_sparse(const ifa4_args* a, const ifa4_paged_kv* kv, const ifa4_block
   p.n_select = ls->n_select;
   p.waves = l.plan.waves;
   p.splits = l.plan.splits;
+  const int64_t rows = (int64_t)ls->n_select * kv->block_size, parts = p.waves * p.splits;
+  p.steps = (int32_t)((rows + ifa4::kSparseStep - 1) / ifa4::kSparseStep);
+  p.part_steps = (int32_t)((p.steps + parts - 1) / parts);
+  p.groups = (int32_t)(a->total_q * a->kv_heads * p.splits);
+  p.per_xcd = (p.groups + 7) / 8;
+  p.by_splits = ifa4::FastDiv::of(p.splits);
+  p.by_total = ifa4::FastDiv::of(p.total_q);
   p.kv_fp8 = qt != nullptr ? 1 : 0;
   p.scale_log2 = a->softmax_scale * (qt != nullptr ? qt->k_scale : 1.f) * kLog2eHost;
   p.v_scale = qt != nullptr ? qt->v_scale : 1.f;

@@ -14,8 +14,8 @@
 // whole and away from the bias (their steps take neither mask nor bias).
 //
 // Products (16x16x32 MFMA, the group's query heads as the 16 columns, zero padded).  S^T = K Q^T,
-// A = K rows straight from memory, 16 bytes a lane from one scalar base per half (e4m3: 16 bytes
-// are the operands of two products, Q taken in the same order): lane (n, g) = (l % 16, l / 16) gets
+// A = K rows through a swizzled LDS tile (16 bytes a lane; e4m3: they are the operands of two
+// products, Q taken in the same order): lane (n, g) = (l % 16, l / 16) gets
 // keys 16 blk + 4g + j of head n.  They are the k-slots 8g + 4 blk + j of O^T += V^T P^T as they
 // stand; A = V^T through a swizzled LDS tile whose row 8g + 4 blk + j holds key 16 blk + 4g + j, by
 // transposing reads of 16 or 8 bits.
@@ -31,20 +31,29 @@ namespace ifa4 {
 namespace {
 
 constexpr int kStep = kSparseStep;
+#ifndef SPARSE_WPE8
+#define SPARSE_WPE8 2
+#endif
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 
 template <int D, int Eb>
 struct SparseShape {
-  static constexpr int kLpr = D * Eb / 16;    // lanes per V row
-  static constexpr int kRpi = 64 / kLpr;      // V rows per load
-  static constexpr int kVLoads = kStep / kRpi;
-  static constexpr int kKLoads = D * Eb / 64; // 16-byte loads per lane and half
+  static constexpr int kLpr = D * Eb / 16;    // lanes (16-byte chunks) per row
+  static constexpr int kRpi = 64 / kLpr;      // rows per load
+  static constexpr int kLoads = kStep / kRpi; // of K, and of V
   static constexpr int kKSteps = D / 32;      // products per half
   static constexpr int kDBlocks = D / 16;
-  static constexpr int kVBytes = kStep * D * Eb;
+  static constexpr int kBytes = kStep * D * Eb;  // of a tile
 };
 
-// Tile row of key `key` of a step (see above).
+// K tile: chunk c of row `row` (the step's keys in order) sits at c ^ kswz(row): the 16 rows that a
+// read of the A operand covers at one chunk lie in distinct banks.
+template <int D, int Eb>
+__device__ __forceinline__ int kswz(int row) {
+  constexpr int kChunks = D * Eb / 16;
+  return row / (16 / kChunks) & (kChunks - 1);
+}
+// V tile: row of key `key` of a step (see above).
 __device__ __forceinline__ int tile_row(int key) {
   return 8 * ((key >> 2) & 3) + 4 * (key >> 4) + (key & 3);
 }
@@ -73,13 +82,14 @@ __device__ __forceinline__ float rel_value(const SparseParams& p, int64_t off) {
 
 // kEight: blocks of 8 rows (not where one load takes 16: e4m3, d 64).
 template <int D, typename Tag, int Eb, int kNw, bool kEight>
-__global__ __launch_bounds__(64 * kNw) __attribute__((amdgpu_waves_per_eu(2))) void
+__global__ __launch_bounds__(64 * kNw) __attribute__((amdgpu_waves_per_eu(
+    Eb == 1 || D == 64 ? SPARSE_WPE8 : 2))) void
 sparse_fwd_kernel(SparseParams p) {
   using E = Elem<Tag>;
   using S = SparseShape<D, Eb>;
   static_assert(!kEight || S::kRpi <= 8, "a load's rows lie in one block");
-  // a wave's V tile, and in the end its partial O [16][D] fp32
-  constexpr int kTileBytes = kNw > 1 && S::kVBytes < 16 * D * 4 ? 16 * D * 4 : S::kVBytes;
+  // a wave's K and V tiles, and in the end its partial O [16][D] fp32
+  constexpr int kTileBytes = 2 * S::kBytes < 16 * D * 4 ? 16 * D * 4 : 2 * S::kBytes;
   __shared__ __align__(16) uint8_t tiles[kNw][kTileBytes];
   __shared__ float part_m[kNw][16], part_l[kNw][16];
   const int lane = threadIdx.x & 63;
@@ -88,21 +98,17 @@ sparse_fwd_kernel(SparseParams p) {
 
   // workgroup -> (share, token, kv head); tokens side by side on one XCD (workgroup i runs on XCD
   // i % 8), whose L2 then serves blocks that neighbours both list
-  const uint32_t items = (uint32_t)p.total_q * (uint32_t)p.kv_heads * (uint32_t)p.splits;
-  const uint32_t per_xcd = (items + 7) / 8;
-  const uint32_t at = (blockIdx.x % 8) * per_xcd + blockIdx.x / 8;
-  if (at >= items) return;
-  const int split = (int)(at % (uint32_t)p.splits);
-  const uint32_t item = at / (uint32_t)p.splits;
-  const int kvh = (int)(item / (uint32_t)p.total_q), t = (int)(item - (uint32_t)kvh * (uint32_t)p.total_q);
+  const uint32_t at = (blockIdx.x % 8) * (uint32_t)p.per_xcd + blockIdx.x / 8;
+  if (at >= (uint32_t)p.groups) return;
+  const uint32_t item = p.by_splits.div(at);
+  const int split = (int)(at - item * (uint32_t)p.splits);
+  const int kvh = (int)p.by_total.div(item), t = (int)(item - (uint32_t)kvh * (uint32_t)p.total_q);
   const int head0 = kvh * p.group;
 
   // ---- what hangs on nothing but the item: list entries, Q --------------------------------------
   const int32_t* const list = p.blocks + (int64_t)t * p.ls_st + (int64_t)kvh * p.ls_sh;
-  const int64_t rows = (int64_t)p.n_select << p.block_shift;
-  const int steps = (int)((rows + kStep - 1) / kStep);
-  const int parts = p.splits * kNw, mine = split * kNw + wave;
-  const int s_beg = (int)((int64_t)steps * mine / parts), s_end = (int)((int64_t)steps * (mine + 1) / parts);
+  const int s_beg = min((split * kNw + wave) * p.part_steps, p.steps);
+  const int s_end = min(s_beg + p.part_steps, p.steps);
   int win = s_beg * kStep >> p.block_shift;  // lane l holds list entry win + l
   int ent = win + lane < p.n_select ? list[win + lane] : -1;
   // column n = query head n of the kv head
@@ -145,13 +151,18 @@ sparse_fwd_kernel(SparseParams p) {
 
   // ---- the window of list entries ---------------------------------------------------------------
   const int bs = 1 << p.block_shift, bmask = bs - 1;
+  const char* const k_head = static_cast<const char*>(p.k) + (int64_t)kvh * p.k_sh * Eb;
+  const char* const v_head = static_cast<const char*>(p.v) + (int64_t)kvh * p.v_sh * Eb;
   uint64_t some = 0, plain = 0;  // entries with a visible key; visible whole and off the band
+  uint64_t k_at = 0, v_at = 0;   // the entry's block; the pool's first for one without a visible key
   auto classify = [&] {
     const int first = ent << p.block_shift;  // (meaningless where phys < 0)
     const bool any = phys >= 0 && first <= pos && first + bmask >= kmin;
     some = __builtin_amdgcn_ballot_w64(any);
     plain = __builtin_amdgcn_ballot_w64(any && first + bmask <= pos && first >= kmin &&
                                         pos - (first + bmask) >= p.rel_extent);
+    k_at = reinterpret_cast<uint64_t>(k_head + (int64_t)(any ? phys : 0) * p.k_sblk * Eb);
+    v_at = reinterpret_cast<uint64_t>(v_head + (int64_t)(any ? phys : 0) * p.v_sblk * Eb);
   };
   classify();
   // Step s: entries e0 .. of the window hold its keys.
@@ -170,53 +181,51 @@ sparse_fwd_kernel(SparseParams p) {
     }
     return s;
   };
+  // What a step's products have to know: the position of each run's first key (kFar: the run has no
+  // visible key), and whether every key is visible without bias (then positions are not set).
+  constexpr int kFar = 1 << 30;
   struct Step {
-    i32x4_t blk, pos;  // of each run: its place in the pool (-1: nothing visible), its first key
+    i32x4_t pos;
     bool plain;
   };
-  auto find = [&](int s) -> Step {
+  const int vr = lane / S::kLpr, vc = lane % S::kLpr;  // row layout of the loads
+  const int k_rowb = (int)p.k_st * Eb, v_rowb = (int)p.v_st * Eb;
+  const uint32_t k_lane = (uint32_t)vr * (uint32_t)k_rowb + 16 * vc;
+  const uint32_t v_lane = (uint32_t)vr * (uint32_t)v_rowb + 16 * vc;
+  auto scalar64 = [](uint64_t x, int l) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), l) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)x, l);
+  };
+  auto load = [&](int s, u32x4_t* kr, u32x4_t* vv) -> Step {
     Step st;
     const int v0 = s * kStep, e0 = (v0 >> p.block_shift) - win;
     st.plain = ((plain >> e0) & step_bits) == step_bits;
-    st.blk = st.pos = i32x4_t{0, 0, 0, 0};
-#pragma unroll
-    for (int r = 0; r < kRuns; ++r) {
-      const int v = v0 + kStep / kRuns * r, e = (v >> p.block_shift) - win;
-      const int blk = __builtin_amdgcn_readlane(phys, e);
-      const int first = ((int)__builtin_amdgcn_readlane(ent, e) << p.block_shift) + (v & bmask);
-      st.pos[r] = first;
-      st.blk[r] = ((some >> e) & 1) && first <= pos && first + kStep / kRuns > kmin ? blk : -1;
-    }
-    return st;
-  };
-  const int vr = lane / S::kLpr, vc = lane % S::kLpr;  // row layout of the V loads
-  const char* const k_head = static_cast<const char*>(p.k) + (int64_t)kvh * p.k_sh * Eb;
-  const char* const v_head = static_cast<const char*>(p.v) + (int64_t)kvh * p.v_sh * Eb;
-  const uint32_t k_lane = (uint32_t)(kEight ? n & 7 : n) * (uint32_t)(p.k_st * Eb) + 16 * g;
-  const uint32_t v_lane = (uint32_t)vr * (uint32_t)(p.v_st * Eb) + 16 * vc;
-  auto load = [&](const Step& st, u32x4_t* kr, u32x4_t* vv) {
-    // a run without a visible key is read from the pool's first block (and masked)
+    st.pos = i32x4_t{kFar, kFar, kFar, kFar};
     const char* kb[kRuns];
     const char* vb[kRuns];
 #pragma unroll
     for (int r = 0; r < kRuns; ++r) {
-      const bool on = st.blk[r] >= 0;
-      const int64_t blk = on ? st.blk[r] : 0, row = on ? st.pos[r] & bmask : 0;
-      kb[r] = k_head + (blk * p.k_sblk + row * p.k_st) * Eb;
-      vb[r] = v_head + (blk * p.v_sblk + row * p.v_st) * Eb;
+      const int v = v0 + kStep / kRuns * r, e = (v >> p.block_shift) - win;
+      kb[r] = reinterpret_cast<const char*>(scalar64(k_at, e)) + (uint32_t)((v & bmask) * k_rowb);
+      vb[r] = reinterpret_cast<const char*>(scalar64(v_at, e)) + (uint32_t)((v & bmask) * v_rowb);
+      if (!st.plain) {
+        const int first = ((int)__builtin_amdgcn_readlane(ent, e) << p.block_shift) + (v & bmask);
+        if (((some >> e) & 1) && first <= pos && first + kStep / kRuns > kmin) st.pos[r] = first;
+      }
     }
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const char* const base = kEight ? (n < 8 ? kb[2 * b % kRuns] : kb[(2 * b + 1) % kRuns]) : kb[b];
-#pragma unroll
-      for (int i = 0; i < S::kKLoads; ++i) kr[b * S::kKLoads + i] = ld_global_16(base + k_lane + 64 * i);
-    }
-#pragma unroll
-    for (int i = 0; i < S::kVLoads; ++i) {
+    for (int i = 0; i < S::kLoads; ++i) {
       const int r = S::kRpi * i / (kStep / kRuns);  // run, first row in it
       const int off = S::kRpi * i % (kStep / kRuns);
-      vv[i] = ld_global_16(vb[r] + off * p.v_st * Eb + v_lane);
+      kr[i] = ld_global_16(kb[r] + (uint32_t)(off * k_rowb) + k_lane);
     }
+#pragma unroll
+    for (int i = 0; i < S::kLoads; ++i) {
+      const int r = S::kRpi * i / (kStep / kRuns);
+      const int off = S::kRpi * i % (kStep / kRuns);
+      vv[i] = ld_global_16(vb[r] + (uint32_t)(off * v_rowb) + v_lane);
+    }
+    return st;
   };
 
   const int64_t rel_row = (int64_t)t * p.rel_st + (int64_t)(head0 + min(n, p.group - 1)) * p.rel_sh;
@@ -225,58 +234,46 @@ sparse_fwd_kernel(SparseParams p) {
   f32x4_t o[S::kDBlocks];
 #pragma unroll
   for (int db = 0; db < S::kDBlocks; ++db) o[db] = f32x4_t{};
-  uint8_t* const tile = tiles[wave];
+  uint8_t* const k_tile = tiles[wave];
+  uint8_t* const tile = k_tile + S::kBytes;
 
   auto compute = [&](const Step& st, const u32x4_t* kr, u32x4_t* vv) {
-    // position of the lane's first key in each half, and whether its run is read
-    int kp[2];
-    bool on[2];
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      if constexpr (kEight) {
-        kp[b] = (g < 2 ? st.pos[2 * b] : st.pos[2 * b + 1]) + 4 * (g & 1);
-        on[b] = (g < 2 ? st.blk[2 * b] : st.blk[2 * b + 1]) >= 0;
-      } else {
-        kp[b] = st.pos[b] + 4 * g;
-        on[b] = st.blk[b] >= 0;
-      }
-    }
     if (!st.plain) {  // V rows that the token does not see hold anything: zero
 #pragma unroll
-      for (int i = 0; i < S::kVLoads; ++i) {
+      for (int i = 0; i < S::kLoads; ++i) {
         const int key = S::kRpi * i + vr;
-        int first, blk;
+        int first;
         if constexpr (kEight) {
           const int r = key >> 3;
-          first = r == 0 ? st.pos[0] : r == 1 ? st.pos[1] : r == 2 ? st.pos[2] : st.pos[3];
-          blk = r == 0 ? st.blk[0] : r == 1 ? st.blk[1] : r == 2 ? st.blk[2] : st.blk[3];
-          first += key & 7;
+          first = (r == 0 ? st.pos[0] : r == 1 ? st.pos[1] : r == 2 ? st.pos[2] : st.pos[3]) + (key & 7);
         } else {
           first = (key < 16 ? st.pos[0] : st.pos[1]) + (key & 15);
-          blk = key < 16 ? st.blk[0] : st.blk[1];
         }
-        if (blk < 0 || first > pos || first < kmin) vv[i] = u32x4_t{0u, 0u, 0u, 0u};
+        if (first > pos || first < kmin) vv[i] = u32x4_t{0u, 0u, 0u, 0u};
       }
     }
 #pragma unroll
-    for (int i = 0; i < S::kVLoads; ++i) {
-      const int row = tile_row(S::kRpi * i + vr);
+    for (int i = 0; i < S::kLoads; ++i) {
+      const int key = S::kRpi * i + vr, row = tile_row(key);
+      *reinterpret_cast<u32x4_t*>(k_tile + key * D * Eb + 16 * (vc ^ kswz<D, Eb>(key))) = kr[i];
       *reinterpret_cast<u32x4_t*>(tile + row * D * Eb + 16 * (vc ^ vswz<D, Eb>(row))) = vv[i];
     }
+    wave_lds_sync();
     f32x4_t acc[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       acc[b] = f32x4_t{};
+      const uint8_t* const k_row = k_tile + (16 * b + n) * D * Eb;
+      const int sw = kswz<D, Eb>(16 * b + n);
 #pragma unroll
-      for (int kk = 0; kk < S::kKSteps; ++kk) {
-        u32x4_t a;
+      for (int i = 0; i < D * Eb / 64; ++i) {
+        const u32x4_t w = *reinterpret_cast<const u32x4_t*>(k_row + 16 * ((4 * i + g) ^ sw));
         if constexpr (Eb == 2) {
-          a = kr[b * S::kKLoads + kk];
+          acc[b] = E::mfma16(w, qf[i], acc[b]);
         } else {
-          const u32x4_t w = kr[b * S::kKLoads + (kk >> 1)];
-          a = (kk & 1) ? fp8x8_operand<E>(w[2], w[3]) : fp8x8_operand<E>(w[0], w[1]);
+          acc[b] = E::mfma16(fp8x8_operand<E>(w[0], w[1]), qf[2 * i], acc[b]);
+          acc[b] = E::mfma16(fp8x8_operand<E>(w[2], w[3]), qf[2 * i + 1], acc[b]);
         }
-        acc[b] = E::mfma16(a, qf[kk], acc[b]);
       }
     }
     if (!st.plain) {
@@ -284,16 +281,22 @@ sparse_fwd_kernel(SparseParams p) {
       const float inv = kLog2e / c2;
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        const bool near = on[b] && n < p.group && pos - kp[b] - 3 < p.rel_extent;
+        // position of the lane's four keys
+        int kp;
+        if constexpr (kEight)
+          kp = (g < 2 ? st.pos[2 * b] : st.pos[2 * b + 1]) + 4 * (g & 1);
+        else
+          kp = st.pos[b] + 4 * g;
+        const bool near = n < p.group && pos - kp >= 0 && pos - kp - 3 < p.rel_extent;
         if (p.rel_extent > 0 && wave_any(near)) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const int dist = pos - kp[b] - j;
+            const int dist = pos - kp - j;
             if (near && (uint32_t)dist < (uint32_t)p.rel_extent)
               acc[b][j] = fmaf(rel_value(p, rel_row + dist), inv, acc[b][j]);
           }
         }
-        const int hi = on[b] ? pos - kp[b] : -1, lo = kmin - kp[b];
+        const int hi = pos - kp, lo = kmin - kp;
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[b][j] = j >= lo && j <= hi ? acc[b][j] : -INFINITY;
       }
@@ -321,7 +324,6 @@ sparse_fwd_kernel(SparseParams p) {
     }
     const u32x4_t pb = {E::pack2(pv[0], pv[1]), E::pack2(pv[2], pv[3]), E::pack2(pv[4], pv[5]),
                         E::pack2(pv[6], pv[7])};
-    wave_lds_sync();
 #pragma unroll
     for (int db = 0; db < S::kDBlocks; ++db) {
       u32x4_t a;
@@ -348,30 +350,21 @@ sparse_fwd_kernel(SparseParams p) {
       }
       o[db] = E::mfma16(a, pb, o[db]);
     }
-    wave_lds_sync();  // the tile is rewritten by the next step
+    wave_lds_sync();  // the tiles are rewritten by the next step
   };
 
   // ---- steps, the next one's rows in flight while one is computed ---------------------------------
   Step st0{}, st1{};
-  u32x4_t k0[2 * S::kKLoads], k1[2 * S::kKLoads], v0[S::kVLoads], v1[S::kVLoads];
+  u32x4_t k0[S::kLoads], k1[S::kLoads], v0[S::kLoads], v1[S::kLoads];
   int s0 = seek(s_beg), s1;
-  if (s0 < s_end) {
-    st0 = find(s0);
-    load(st0, k0, v0);
-  }
+  if (s0 < s_end) st0 = load(s0, k0, v0);
   while (s0 < s_end) {
     s1 = seek(s0 + 1);
-    if (s1 < s_end) {
-      st1 = find(s1);
-      load(st1, k1, v1);
-    }
+    if (s1 < s_end) st1 = load(s1, k1, v1);
     compute(st0, k0, v0);
     if (s1 >= s_end) break;
     s0 = seek(s1 + 1);
-    if (s0 < s_end) {
-      st0 = find(s0);
-      load(st0, k0, v0);
-    }
+    if (s0 < s_end) st0 = load(s0, k0, v0);
     compute(st1, k1, v1);
   }
 
@@ -398,7 +391,7 @@ sparse_fwd_kernel(SparseParams p) {
       for (int db = 0; db < S::kDBlocks; ++db) put(n, 16 * db + 4 * g, o[db], m_run, l_tot);
     }
   } else {
-    float* const own = reinterpret_cast<float*>(tile);
+    float* const own = reinterpret_cast<float*>(k_tile);
     if (n < p.group) {
 #pragma unroll
       for (int db = 0; db < S::kDBlocks; ++db)
@@ -462,8 +455,7 @@ __global__ __launch_bounds__(kJoinThreads) void sparse_join_kernel(SparseParams 
 
 template <int D, typename Tag, int Eb, int kNw>
 void launch_sparse_w(const SparseParams& p, hipStream_t stream) {
-  const int64_t items = (int64_t)p.total_q * p.kv_heads * p.splits;
-  const dim3 grid((unsigned)((items + 7) / 8 * 8)), block(64 * kNw);
+  const dim3 grid((unsigned)p.per_xcd * 8), block(64 * kNw);
   if constexpr (SparseShape<D, Eb>::kRpi <= 8) {
     if (p.block_shift == 3) {
       hipLaunchKernelGGL((sparse_fwd_kernel<D, Tag, Eb, kNw, true>), grid, block, 0, stream, p);
