@@ -478,6 +478,7 @@ int32_t run_sparse(const ifa4_args* a, const ifa4_paged_kv* kv, const ifa4_block
   const int64_t rows = (int64_t)ls->n_select * kv->block_size, parts = p.waves * p.splits;
   p.steps = (int32_t)((rows + ifa4::kSparseStep - 1) / ifa4::kSparseStep);
   p.part_steps = (int32_t)((p.steps + parts - 1) / parts);
+  p.once = a->max_seqlen_q <= 1 ? 1 : 0;
   p.groups = (int32_t)(a->total_q * a->kv_heads * p.splits);
   p.per_xcd = (p.groups + 7) / 8;
   p.by_splits = ifa4::FastDiv::of(p.splits);

@@ -265,6 +265,7 @@ struct SparseParams {
   int32_t n_select;
   int32_t waves, splits;     // waves of a workgroup, workgroups that share a list
   int32_t steps, part_steps; // of a list, of a wave
+  int32_t once;              // one token a sequence at most: rows are read once
   int32_t groups, per_xcd;   // workgroups, those of an XCD
   FastDiv by_splits, by_total;  // divisions by splits, total_q
   int32_t kv_fp8;

@@ -74,14 +74,21 @@ __device__ __forceinline__ u32x4_t fp8x8_operand(uint32_t lo, uint32_t hi) {
                  E::template fp8x2<false>(hi), E::template fp8x2<true>(hi)};
 }
 
+template <bool kOnce>
+__device__ __forceinline__ u32x4_t ld_kv(const char* p) {
+  if constexpr (kOnce) return __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p));
+  return ld_global_16(p);
+}
 __device__ __forceinline__ float rel_value(const SparseParams& p, int64_t off) {
   if (p.rel_dtype == 2) return static_cast<const float*>(p.rel)[off];
   const uint16_t x = static_cast<const uint16_t*>(p.rel)[off];
   return p.rel_dtype == 0 ? __uint_as_float((uint32_t)x << 16) : (float)__builtin_bit_cast(_Float16, x);
 }
 
-// kEight: blocks of 8 rows (not where one load takes 16: e4m3, d 64).
-template <int D, typename Tag, int Eb, int kNw, bool kEight>
+// kEight: blocks of 8 rows (not where one load takes 16: e4m3, d 64).  kOnce: one token a sequence,
+// no other will read its rows, and they pass the caches by (64 sequences x 128 blocks of 16 39.8 ->
+// 35.2 us, 128 x 256 111 -> 98; a branch in the kernel instead comes out as one plain load).
+template <int D, typename Tag, int Eb, int kNw, bool kEight, bool kOnce>
 __global__ __launch_bounds__(64 * kNw) __attribute__((amdgpu_waves_per_eu(
     Eb == 1 || D == 64 ? SPARSE_WPE8 : 2))) void
 sparse_fwd_kernel(SparseParams p) {
@@ -217,13 +224,13 @@ sparse_fwd_kernel(SparseParams p) {
     for (int i = 0; i < S::kLoads; ++i) {
       const int r = S::kRpi * i / (kStep / kRuns);  // run, first row in it
       const int off = S::kRpi * i % (kStep / kRuns);
-      kr[i] = ld_global_16(kb[r] + (uint32_t)(off * k_rowb) + k_lane);
+      kr[i] = ld_kv<kOnce>(kb[r] + (uint32_t)(off * k_rowb) + k_lane);
     }
 #pragma unroll
     for (int i = 0; i < S::kLoads; ++i) {
       const int r = S::kRpi * i / (kStep / kRuns);
       const int off = S::kRpi * i % (kStep / kRuns);
-      vv[i] = ld_global_16(vb[r] + (uint32_t)(off * v_rowb) + v_lane);
+      vv[i] = ld_kv<kOnce>(vb[r] + (uint32_t)(off * v_rowb) + v_lane);
     }
     return st;
   };
@@ -453,26 +460,34 @@ __global__ __launch_bounds__(kJoinThreads) void sparse_join_kernel(SparseParams 
     p.lse[(int64_t)head * p.lse_sh + t] = lt > 0.f ? (mt + __log2f(lt)) * kLn2 : -INFINITY;
 }
 
-template <int D, typename Tag, int Eb, int kNw>
+template <int D, typename Tag, int Eb, int kNw, bool kOnce>
 void launch_sparse_w(const SparseParams& p, hipStream_t stream) {
   const dim3 grid((unsigned)p.per_xcd * 8), block(64 * kNw);
   if constexpr (SparseShape<D, Eb>::kRpi <= 8) {
     if (p.block_shift == 3) {
-      hipLaunchKernelGGL((sparse_fwd_kernel<D, Tag, Eb, kNw, true>), grid, block, 0, stream, p);
+      hipLaunchKernelGGL((sparse_fwd_kernel<D, Tag, Eb, kNw, true, kOnce>), grid, block, 0, stream, p);
       return;
     }
   }
-  hipLaunchKernelGGL((sparse_fwd_kernel<D, Tag, Eb, kNw, false>), grid, block, 0, stream, p);
+  hipLaunchKernelGGL((sparse_fwd_kernel<D, Tag, Eb, kNw, false, kOnce>), grid, block, 0, stream, p);
+}
+
+template <int D, typename Tag, int Eb, bool kOnce>
+void launch_sparse_o(const SparseParams& p, hipStream_t stream) {
+  switch (p.waves) {
+    case 1: launch_sparse_w<D, Tag, Eb, 1, kOnce>(p, stream); break;
+    case 2: launch_sparse_w<D, Tag, Eb, 2, kOnce>(p, stream); break;
+    case 4: launch_sparse_w<D, Tag, Eb, 4, kOnce>(p, stream); break;
+    default: launch_sparse_w<D, Tag, Eb, 8, kOnce>(p, stream);
+  }
 }
 
 template <int D, typename Tag, int Eb>
 hipError_t launch_sparse_t(const SparseParams& p, hipStream_t stream) {
-  switch (p.waves) {
-    case 1: launch_sparse_w<D, Tag, Eb, 1>(p, stream); break;
-    case 2: launch_sparse_w<D, Tag, Eb, 2>(p, stream); break;
-    case 4: launch_sparse_w<D, Tag, Eb, 4>(p, stream); break;
-    default: launch_sparse_w<D, Tag, Eb, 8>(p, stream);
-  }
+  if (p.once)
+    launch_sparse_o<D, Tag, Eb, true>(p, stream);
+  else
+    launch_sparse_o<D, Tag, Eb, false>(p, stream);
   if (p.splits > 1) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
