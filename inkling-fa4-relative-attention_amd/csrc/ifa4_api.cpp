@@ -263,10 +263,14 @@ struct PrefillWorkspace {
   int64_t o_bytes, lse_bytes;
   int64_t total() const { return split.chunk_tiles > 0 ? o_bytes + lse_bytes : 0; }
 };
-PrefillWorkspace prefill_workspace(const ifa4_args* a, bool proj = false) {
+PrefillWorkspace prefill_workspace(const ifa4_args* a, bool proj = false, bool paged = false) {
   PrefillWorkspace w;
   w.pack = proj ? 1 : prefill_pack(a);
   w.split = prefill_split(a, w.pack, proj);
+  if (paged && w.split.chunk_tiles == 0)
+    w.split = ifa4::paged_ragged_split(a->batch, a->n_heads / w.pack, a->total_q, a->max_seqlen_q,
+                                       a->max_seqlen_k, a->window_left,
+                                       ifa4::prefill_block_q() / w.pack, ifa4::prefill_block_k());
   const int64_t rows = (int64_t)w.split.n_chunks * a->n_heads * a->total_q;
   w.o_bytes = (rows * a->head_dim * 4 + 255) / 256 * 256;
   w.lse_bytes = (rows * 4 + 255) / 256 * 256;
@@ -369,7 +373,7 @@ int32_t run_prefill_paged(const ifa4_args* a, const ifa4_paged_kv* kv, const ifa
   ifa4_args b = *a;
   b.total_k = (int64_t)a->batch * a->max_seqlen_k;  // the lengths are on the device only
   ifa4::PrefillParams p = make_prefill_params(&b);
-  const PrefillWorkspace w = prefill_workspace(a);
+  const PrefillWorkspace w = prefill_workspace(a, false, true);
   set_tiles(p, a, ifa4::prefill_block_q(), w.pack);
   if (!set_split(p, w, workspace, workspace_bytes)) return IFA4_EWORKSPACE;
   p.block_table = kv->block_table;
@@ -850,7 +854,7 @@ int32_t ifa4_prefill_rproj_fwd_ws(const ifa4_args* args, const ifa4_rel_proj* pr
 size_t ifa4_prefill_paged_workspace_bytes(const ifa4_args* args, const ifa4_paged_kv* kv,
                                           const ifa4_kv_quant* quant) {
   if (check_prefill_paged(args, kv, quant) != IFA4_OK || no_queries(args)) return 0;
-  return (size_t)prefill_workspace(args).total();
+  return (size_t)prefill_workspace(args, false, true).total();
 }
 
 int32_t ifa4_prefill_paged_fwd(const ifa4_args* args, const ifa4_paged_kv* kv,

@@ -441,6 +441,29 @@ inline PrefillSplit prefill_split_for(int64_t batch, int64_t n_heads, int64_t ma
   return s;
 }
 
+// Prefill over a paged cache, whose lengths only the device knows: a batch of unequal query counts
+// (total_q against batch * max_q) has unequal caches too, and its grid, planned by the longest, looks
+// full where it is not.  A call that the plan above leaves whole, with up to 1.5 resident rounds of
+// live workgroups over ranges of 96 tiles and more, is cut into chunks of two fifths of the
+// longest range (without, chunks of 0.3 / 0.4 / 0.5 of it; one box, us, Hq 8 / Hkv 2, d 128, bias of
+// extent 1024): 16 x 3..500 queries over 90..8000 keys 211 -> 181 / 152 / 160, 32 x the same 300 ->
+// 282 / 289 / 277, 8 x 10..1000 over 90..20K 452 -> 257 / 238 / -, 20 x 1..600 over 2K..30K 887 ->
+// 700 at 0.25; shorter ranges lose (40 x 1..400 over 90..3000, 53 tiles, 145 -> 152, 10 x 1..2000 over
+// 1..2000 131 -> 135), and so do equal query counts (8 x 512 over 4K 107 -> 117).
+inline PrefillSplit paged_ragged_split(int64_t batch, int64_t n_heads, int64_t total_q, int64_t max_q,
+                                       int64_t max_k, int64_t window_left, int32_t block_q,
+                                       int32_t block_k) {
+  PrefillSplit s{0, 1, 1};
+  const int64_t tiles = (max_k + block_k - 1) / block_k;
+  const int64_t live = (total_q / block_q + batch / 2) * n_heads;
+  if (batch < 2 || window_left >= 0 || 16 * total_q >= 15 * batch * max_q || tiles < 96 ||
+      2 * live > 3 * kPrefillSlots)
+    return s;
+  s.chunk_tiles = (int32_t)(2 * tiles / 5);
+  s.n_chunks = s.seen_chunks = (int32_t)((tiles + s.chunk_tiles - 1) / s.chunk_tiles);
+  return s;
+}
+
 // Decode behind a shared prefix (decode_shared.hip): how the prefix is cut into pieces of 128 rows
 // x chunk_keys, and each (sequence, kv head)'s own keys into own_chunks pieces; own_first: pieces of
 // own keys that a workgroup without a prefix piece takes before the others take one.
