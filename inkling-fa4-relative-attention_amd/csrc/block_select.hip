@@ -167,14 +167,13 @@ __device__ __forceinline__ int token_blocks(const SelectParams& p, const TokenSp
 // l % 16), held in registers over the blocks; C (lane l, register r) = block 4 r + l / 16, token
 // l % 16.
 constexpr int kScoreWaves = 4;
-#ifndef SCORE_GROUPS
-#define SCORE_GROUPS 512
-#endif
-constexpr int kScoreGroups = SCORE_GROUPS;
-#ifndef STEP_TOKENS
-#define STEP_TOKENS 4
-#endif
-constexpr int kStepTokens = STEP_TOKENS;
+constexpr int kHeadsAtOnce = 4;  // query heads whose loads are in flight together
+// Workgroups of the tile kernel in all: one resident round (512 tokens over 1900 blocks of e4m3, us a
+// call with 256 / 512 / 768 / 1024: 43.5 / 41.6 / 47.3 / 44.7).
+constexpr int kScoreGroups = 512;
+// Tokens of a sequence up to which the vector unit takes them one by one (16 sequences over 1900
+// blocks, vector / matrix: 2 tokens 20.6 / 26.3, 4 tokens 27.1 / 26.8).
+constexpr int kStepTokens = 3;
 template <int D, typename Tag, int Eb>
 __global__ __launch_bounds__(64 * kScoreWaves) void score_tile_kernel(SelectParams p) {
   constexpr int kEpc = 16 / Eb;                // elements of a 16-byte chunk
@@ -200,18 +199,42 @@ __global__ __launch_bounds__(64 * kScoreWaves) void score_tile_kernel(SelectPara
   const int64_t tok = s.start + min(i0 + m, s.len - 1);
   const char* const q_row = static_cast<const char*>(p.q) +
                             (tok * p.q_st + (int64_t)h * p.group * p.q_sh) * 2;
+  const int32_t* const table = p.block_table + seq * p.bt_stride;
+  auto load = [&](int t, u32x4_t* w) {
+    const int blk = min(16 * t + m, most - 1);
+    const int ent = table[blk];
+    const bool good = (uint32_t)ent < (uint32_t)p.num_blocks;
+    const char* src = static_cast<const char*>(p.bounds) +
+                      ((int64_t)(good ? ent : 0) * p.b_sblk + (int64_t)h * p.b_sh) * Eb + 16 * g;
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      w[i] = ld_global_16(src + 64 * i);
+      if (!good) w[i] = u32x4_t{0u, 0u, 0u, 0u};
+    }
+  };
+  u32x4_t w[kChunks], next[kChunks];
+  load(tile, w);  // (a tile past the last is read as the last block)
   if (wave < kUnits) {
     const int d = kEpc * (4 * (wave / (kEpc / 8)) + g) + 8 * (wave % (kEpc / 8));
     double neg[8], up[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) neg[e] = up[e] = 0.0;
-    for (int head = 0; head < p.group; ++head) {
-      float f[8];
-      unpack16<Tag, 2>(ld_global_16(q_row + (head * p.q_sh + d) * 2), f);
+    for (int head = 0; head < p.group; head += kHeadsAtOnce) {
+      u32x4_t x[kHeadsAtOnce];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        neg[e] += (double)(f[e] > 0.f ? 0.f : f[e]);  // a NaN in both
-        up[e] += (double)(f[e] < 0.f ? 0.f : f[e]);
+      for (int i = 0; i < kHeadsAtOnce; ++i)
+        x[i] = ld_global_16(q_row + (min(head + i, p.group - 1) * p.q_sh + d) * 2);
+#pragma unroll
+      for (int i = 0; i < kHeadsAtOnce; ++i) {
+        if (head + i < p.group) {
+          float f[8];
+          unpack16<Tag, 2>(x[i], f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            neg[e] += (double)(f[e] > 0.f ? 0.f : f[e]);  // a NaN in both
+            up[e] += (double)(f[e] < 0.f ? 0.f : f[e]);
+          }
+        }
       }
     }
 #pragma unroll
@@ -228,22 +251,7 @@ __global__ __launch_bounds__(64 * kScoreWaves) void score_tile_kernel(SelectPara
 #pragma unroll
     for (int e = 0; e < kEpc; ++e) q[i][e] = q_lds[i * (kEpc / 8) + e / 8][lane][e % 8];
 
-  const int32_t* const table = p.block_table + seq * p.bt_stride;
-  auto load = [&](int t, u32x4_t* w) {
-    const int blk = min(16 * t + m, most - 1);
-    const int ent = table[blk];
-    const bool good = (uint32_t)ent < (uint32_t)p.num_blocks;
-    const char* src = static_cast<const char*>(p.bounds) +
-                      ((int64_t)(good ? ent : 0) * p.b_sblk + (int64_t)h * p.b_sh) * Eb + 16 * g;
-#pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-      w[i] = ld_global_16(src + 64 * i);
-      if (!good) w[i] = u32x4_t{0u, 0u, 0u, 0u};
-    }
-  };
   const int step = p.score_parts * kScoreWaves;
-  u32x4_t w[kChunks], next[kChunks];
-  load(tile, w);
   for (; tile * 16 < last; tile += step) {
     if ((tile + step) * 16 < last) load(tile + step, next);
     f64x4_t acc = {0.0, 0.0, 0.0, 0.0}, acc1 = acc;
@@ -309,20 +317,33 @@ __global__ __launch_bounds__(64 * kScoreWaves) void score_step_kernel(SelectPara
 #pragma unroll
     for (int e = 0; e < kEpc; ++e) q[i][e] = 0.0;
   // chunk c: elements d = kEpc (c % kHalf) .., of lo for c < kHalf, else of hi
-  for (int head = 0; head < p.group; ++head) {
+  for (int head = 0; head < p.group; head += 2) {
+    u32x4_t x[2][kChunks][kEpc / 8];
 #pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-      const int c = sub + 8 * i;
-      const bool up = c >= kHalf;
-      const int d = kEpc * (c & (kHalf - 1));
+    for (int k = 0; k < 2; ++k)
 #pragma unroll
-      for (int part = 0; part < kEpc / 8; ++part) {
-        float f[8];
-        unpack16<Tag, 2>(ld_global_16(q_row + (head * p.q_sh + d + 8 * part) * 2), f);
+      for (int i = 0; i < kChunks; ++i)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float x = up ? f[e] : -f[e];
-          q[i][8 * part + e] += (double)(x < 0.f ? 0.f : f[e]);  // a NaN in both
+        for (int part = 0; part < kEpc / 8; ++part)
+          x[k][i][part] = ld_global_16(
+              q_row + (min(head + k, p.group - 1) * p.q_sh +
+                       kEpc * ((sub + 8 * i) & (kHalf - 1)) + 8 * part) * 2);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (head + k < p.group) {
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) {
+          const bool up = sub + 8 * i >= kHalf;
+#pragma unroll
+          for (int part = 0; part < kEpc / 8; ++part) {
+            float f[8];
+            unpack16<Tag, 2>(x[k][i][part], f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float y = up ? f[e] : -f[e];
+              q[i][8 * part + e] += (double)(y < 0.f ? 0.f : f[e]);  // a NaN in both
+            }
+          }
         }
       }
     }
@@ -396,6 +417,18 @@ __global__ __launch_bounds__(kPickThreads) void pick_blocks_kernel(SelectParams 
   const int64_t row = blockIdx.x;
   const int t = (int)(row / p.kv_heads);
   int32_t* const list = p.out + row * p.n_select;
+  const int first = p.sink;  // competing blocks [first, first + n)
+  const uint64_t* const keys = p.scores + row * (int64_t)p.cols + first;
+  uint64_t mine[kPer];
+  auto load = [&](int r0, int end) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int b = r0 + tid * kPer + i;
+      mine[i] = b < end ? keys[b] : 0;
+    }
+  };
+  // before n is known, and with it which of them were written
+  if constexpr (kOne) load(0, p.scores != nullptr ? p.cols - first : 0);
 
   // the token's sequence: the first whose tokens end past it
   int nb = 0;
@@ -415,24 +448,14 @@ __global__ __launch_bounds__(kPickThreads) void pick_blocks_kernel(SelectParams 
   for (int i = tid; i < p.sink; i += kPickThreads) list[i] = i;
   for (int i = tid; i < p.recent; i += kPickThreads)
     list[p.n_select - p.recent + i] = nb - p.recent + i;
-  const int first = p.sink, n = nb - p.recent - p.sink;  // competing blocks, n > 0
+  const int n = nb - p.recent - p.sink;  // > 0
   int need = p.n_select - p.sink - p.recent;
   if (need == 0) return;
-  const uint64_t* const keys = p.scores + row * (int64_t)p.cols + first;
-  uint64_t mine[kPer];
-  auto load = [&](int r0) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int b = r0 + tid * kPer + i;
-      mine[i] = b < n ? keys[b] : 0;
-    }
-  };
   const int rounds = kOne ? 1 : (n + kRound - 1) / kRound;
-  if constexpr (kOne) load(0);
   // every key of the row, in any order
   auto each = [&](auto&& f) {
     for (int r = 0; r < rounds; ++r) {
-      if constexpr (!kOne) load(r * kRound);
+      if constexpr (!kOne) load(r * kRound, n);
 #pragma unroll
       for (int i = 0; i < kPer; ++i)
         if (r * kRound + tid * kPer + i < n) f(mine[i], r * kRound + tid * kPer + i);
@@ -558,7 +581,7 @@ __global__ __launch_bounds__(kPickThreads) void pick_blocks_kernel(SelectParams 
   // the list: blocks with keys above `top`, and the first `equal` of those equal to it
   int at = p.sink, met = 0;  // places filled, keys equal to top met
   for (int r = 0; r < rounds; ++r) {
-    if constexpr (!kOne) load(r * kRound);
+    if constexpr (!kOne) load(r * kRound, n);
     int a = 0, e = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {

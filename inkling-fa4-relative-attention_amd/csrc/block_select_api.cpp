@@ -151,7 +151,7 @@ int32_t ifa4_select_blocks_paged(const ifa4_block_select* a, const ifa4_paged_kv
   p.seqused_k = kv->seqused_k;
   p.block_table = kv->block_table;
   p.out = a->blocks;
-  p.scores = static_cast<uint64_t*>(workspace);
+  p.scores = need > 0 ? static_cast<uint64_t*>(workspace) : nullptr;
   p.q_st = a->q_stride_t;
   p.q_sh = a->q_stride_h;
   p.b_sh = a->bounds_stride_h;
