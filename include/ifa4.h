@@ -512,8 +512,10 @@ int32_t ifa4_key_bounds_paged(const ifa4_key_bounds* args, const ifa4_paged_kv* 
  * more than n_select of them it reads all; else the first sink_blocks, the last recent_blocks
  * and the best of those between by
  *   score(blk) = sum over the kv head's query heads g and d of max(q_gd lo_d, q_gd hi_d),
- * summed in 64 bits (NaN counts as infinity; equal scores: the lower block; a table entry outside
- * the pool has bounds of zero).  blocks [total_q, kv_heads, n_select] (contiguous) gets the block
+ * summed in 64 bits, in an order that sizes choose (scores closer than such a sum's rounding may
+ * rank either way; equal bounds score equal, and equal scores go to the lower block).  A score of
+ * NaN counts as infinity, and so does a block with a bound that is infinite or NaN; a table entry
+ * outside the pool has bounds of zero.  blocks [total_q, kv_heads, n_select] (contiguous) gets the block
  * indexes ascending, then -1; a token of no sequence gets -1 throughout.  n_select >=
  * sink_blocks + recent_blocks, recent_blocks >= 1.  max_seqlen_q and max_seqlen_k must bound the
  * lengths.  The workspace (256-byte aligned, contents on entry irrelevant) is scratch for one

@@ -5,7 +5,8 @@
 //     exactly; NaN where a key is NaN)
 //   score[t, h, b] = sum over the query heads g of kv head h and d of max(q_gd lo_d, q_gd hi_d)
 //                  = sum_d qn_d lo_d + qp_d hi_d,  qn = sum_g min(q_g, 0), qp = sum_g max(q_g, 0):
-//     no key of the block has a greater sum of its group's dot products.
+//     no key of the block has a greater sum of its group's dot products.  (An infinite bound meets
+//     a qn or qp of 0 as NaN: the block counts as the best, which it may be.)
 //   list[t, h] = the first `sink` blocks, the last `recent` ones up to the token's own, and the
 //     best by score of those between (a score of NaN as infinity, equal ones the lower block
 //     first), ascending; all blocks where there are no more than the list holds.

@@ -10,6 +10,9 @@
 
 namespace {
 
+// Workgroups of 256 threads in a grid of less than 2^32 threads.
+constexpr int64_t kMostGroups = int64_t(1) << 24;
+
 bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 // Block tables, lengths and the new tokens' offsets of `batch` sequences.
@@ -75,15 +78,18 @@ int32_t check_select(const ifa4_block_select* a, const ifa4_paged_kv* kv) {
   int32_t st = check_table(kv, a->cu_seqlens, a->batch);
   if (st != IFA4_OK || a->total_q == 0) return st;
   if (a->blocks == nullptr || !aligned(a->blocks, 4)) return IFA4_EINVAL;
-  // lists are addressed by rows of 32 bits
-  if (a->total_q * a->n_heads > (int64_t(1) << 28)) return IFA4_EUNSUPPORTED;
+  // a workgroup for each list, of at most 2^32 threads in all
+  if (a->total_q * a->kv_heads >= kMostGroups) return IFA4_EUNSUPPORTED;
   if (a->batch == 0) return IFA4_OK;
   if ((int64_t)kv->max_blocks_per_seq * kv->block_size < a->max_seqlen_k) return IFA4_EINVAL;
   if (a->q == nullptr || a->q_stride_t < 0 || a->q_stride_h < 0) return IFA4_EINVAL;
   if (!aligned(a->q, 16) || ((a->total_q > 1 ? a->q_stride_t : 0) | (a->n_heads > 1 ? a->q_stride_h : 0)) % 8 != 0)
     return IFA4_EUNSUPPORTED;
+  // workgroups that score: a few tokens against 256 blocks each, 16 tokens against any number
   const int64_t q_tiles = ((int64_t)a->max_seqlen_q + 15) / 16;
-  if (q_tiles * a->kv_heads > (int64_t(1) << 20)) return IFA4_EUNSUPPORTED;
+  const int64_t spans = (int64_t)a->max_seqlen_k / kv->block_size / 256 + 2;
+  if (q_tiles * a->kv_heads > (int64_t(1) << 20) || spans * a->kv_heads * 3 >= kMostGroups)
+    return IFA4_EUNSUPPORTED;
   return check_bounds(a->bounds, a->bounds_stride_block, a->bounds_stride_h, kv, a->kv_heads,
                       a->head_dim, a->kv_dtype == IFA4_FP8_E4M3 ? 1 : 2, false);
 }
@@ -128,7 +134,7 @@ int32_t ifa4_key_bounds_paged(const ifa4_key_bounds* a, const ifa4_paged_kv* kv,
   // n keys in a row meet at most this many blocks
   const int64_t slots = ((int64_t)a->max_seqlen_q + kv->block_size - 2) / kv->block_size + 1;
   p.slots = (int32_t)(slots < p.max_blocks ? slots : p.max_blocks);
-  if ((int64_t)p.slots * a->kv_heads > INT32_MAX) return IFA4_EUNSUPPORTED;
+  if ((int64_t)p.slots * a->kv_heads >= kMostGroups) return IFA4_EUNSUPPORTED;
   return status_of(ifa4::launch_key_bounds(p, a->head_dim, a->kv_dtype, a->kv_dtype == IFA4_FP8_E4M3,
                                            static_cast<hipStream_t>(stream)));
 }

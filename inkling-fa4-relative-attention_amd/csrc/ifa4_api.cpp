@@ -406,9 +406,9 @@ int32_t check_sparse(const ifa4_args* a, const ifa4_paged_kv* kv, const ifa4_blo
     return IFA4_EUNSUPPORTED;
   if (no_queries(a)) return IFA4_OK;
   if (ls->blocks == nullptr || !aligned(ls->blocks, 4)) return IFA4_EINVAL;
-  // rows of a list and workgroups are counted in 32 bits
+  // rows of a list, and threads (64 a token and kv head and more), are counted in 32 bits
   if ((int64_t)ls->n_select * kv->block_size > (int64_t(1) << 30) ||
-      a->total_q * a->n_heads > (int64_t(1) << 28))
+      a->total_q * a->kv_heads >= (int64_t(1) << 26) - 8)
     return IFA4_EUNSUPPORTED;
   return IFA4_OK;
 }

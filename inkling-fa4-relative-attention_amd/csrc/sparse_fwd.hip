@@ -31,9 +31,6 @@ namespace ifa4 {
 namespace {
 
 constexpr int kStep = kSparseStep;
-#ifndef SPARSE_WPE8
-#define SPARSE_WPE8 2
-#endif
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 
 template <int D, int Eb>
@@ -89,8 +86,7 @@ __device__ __forceinline__ float rel_value(const SparseParams& p, int64_t off) {
 // no other will read its rows, and they pass the caches by (64 sequences x 128 blocks of 16 39.8 ->
 // 35.2 us, 128 x 256 111 -> 98; a branch in the kernel instead comes out as one plain load).
 template <int D, typename Tag, int Eb, int kNw, bool kEight, bool kOnce>
-__global__ __launch_bounds__(64 * kNw) __attribute__((amdgpu_waves_per_eu(
-    Eb == 1 || D == 64 ? SPARSE_WPE8 : 2))) void
+__global__ __launch_bounds__(64 * kNw) __attribute__((amdgpu_waves_per_eu(2))) void
 sparse_fwd_kernel(SparseParams p) {
   using E = Elem<Tag>;
   using S = SparseShape<D, Eb>;

@@ -9,6 +9,7 @@
 
 namespace {
 
+using ifa4_torch::check_no_tangent;
 using ifa4_torch::check_status;
 using ifa4_torch::dtype_code;
 using ifa4_torch::empty_on;
@@ -155,9 +156,11 @@ void key_bounds_in_place(const at::Tensor& k_cache, const at::Tensor& bounds, co
   if (!bounds.is_inference()) bounds.unsafeGetTensorImpl()->bump_version();
 }
 
-// There is no gradient: bounds that require one would go on as if they had not been written.
+// There is no derivative: a tangent is refused, and so are bounds that require a gradient, which
+// would go on as if they had not been written.
 void key_bounds_autograd(const at::Tensor& k_cache, const at::Tensor& bounds, const at::Tensor& cu_q,
                          const at::Tensor& seqused_k, const at::Tensor& block_table, int64_t max_q) {
+  check_no_tangent("key_bounds_paged", k_cache, bounds);
   TORCH_CHECK(!at::GradMode::is_enabled() || !bounds.requires_grad(),
               "inkling_fa4.key_bounds_paged: bounds that require a gradient are written in place");
   key_bounds_in_place(k_cache, bounds, cu_q, seqused_k, block_table, max_q);

@@ -14,21 +14,13 @@
 
 namespace {
 
+using ifa4_torch::check_no_tangent;
 using ifa4_torch::check_status;
 using ifa4_torch::dtype_code;
 using ifa4_torch::empty_on;
 using OptTensor = std::optional<at::Tensor>;
 
 bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
-
-// A tangent (forward-mode differentiation) is refused: below autograd it would vanish.
-bool has_tangent(const at::Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
-bool has_tangent(const OptTensor& t) { return t.has_value() && has_tangent(*t); }
-template <typename... T>
-void check_no_tangent(const char* op, const T&... inputs) {
-  TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(inputs) || ...), "inkling_fa4.", op,
-                              ": no forward-mode derivative");
-}
 
 void check_heads(const at::Tensor& x, const at::Tensor& like, const char* op, const char* name) {
   TORCH_CHECK(x.is_cuda() && x.device() == like.device(), "inkling_fa4.", op, ": ", name,

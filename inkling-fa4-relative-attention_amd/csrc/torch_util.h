@@ -1,8 +1,10 @@
-// What the sources of the torch binding share: type codes, output allocation, status checks.
+// What the sources of the torch binding share: type codes, output allocation, status and tangent checks.
 #pragma once
 
 #include <ATen/ATen.h>
 #include <ATen/hip/EmptyTensor.h>
+
+#include <optional>
 
 #include "ifa4.h"
 
@@ -29,6 +31,19 @@ inline at::Tensor empty_on(const at::Tensor& q, at::IntArrayRef sizes, at::Scala
 
 inline void check_status(int32_t st, const char* what) {
   TORCH_CHECK(st == IFA4_OK, "inkling_fa4.", what, ": ", ifa4_status_str(st));
+}
+
+// A tangent (forward-mode differentiation) is refused: below autograd it would vanish.
+inline bool has_tangent(const at::Tensor& t) {
+  return t.defined() && t._fw_grad(/*level=*/0).defined();
+}
+inline bool has_tangent(const std::optional<at::Tensor>& t) {
+  return t.has_value() && has_tangent(*t);
+}
+template <typename... T>
+void check_no_tangent(const char* op, const T&... inputs) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(inputs) || ...), "inkling_fa4.", op,
+                              ": no forward-mode derivative");
 }
 
 }  // namespace ifa4_torch

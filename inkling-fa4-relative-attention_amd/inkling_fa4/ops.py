@@ -12,7 +12,8 @@ plus the same entry points under names without the `_triton` suffix, and
 the format of the serving caller (outputs/architecture.md:117-120), and
 `inkling_fa4_rel_attention_rproj` with the bias computed in the kernel from the
 RelLogitsProj factors (outputs/architecture.md:24,52-54);
-`inkling_fa4_rel_attention_decode_shared_prefix` for a paged batch behind one prompt.
+`inkling_fa4_rel_attention_decode_shared_prefix` for a paged batch behind one prompt;
+`inkling_fa4_rel_attention_paged` for chunks of prompts over a paged KV cache.
 
 Differences from the reference wrappers (all deliberate):
   * one kernel launch for the whole batch and no host synchronisation (the
@@ -209,6 +210,8 @@ def inkling_fa4_rel_attention_paged(q, k_cache, v_cache, rel_logits, cu_seqlens_
     sequence holds are not written.  max_seqlen_q and max_seqlen_k must bound the lengths.
     Keys and values that one of a tile's queries (128 at most) sees and another does not must
     be finite; what lies past the last key, or left of every query's window, may be anything.
+    The bias joins the products as bias / (softmax_scale * k_scale) in fp32: a value so far below
+    zero that the quotient overflows hides its key, as -inf does.
     """
     if k_cache.dim() != 4:
         raise ValueError("k_cache must be [num_blocks, block_size, kv_heads, head_dim]")

@@ -25,8 +25,8 @@ def inkling_fa4_key_bounds_paged(k_cache, bounds, cu_seqlens_q, seqused_k, block
     whole, so a block given to another sequence needs nothing but this call after its append.
     Two sequences that share a block they fill to unequal lengths leave the bounds of one.
 
-    max_seqlen_q must bound the new tokens of a sequence.  There is no gradient: bounds that
-    require one are refused (outside torch.no_grad()).
+    max_seqlen_q must bound the new tokens of a sequence.  There is no derivative: tangents are
+    refused, and so are bounds that require a gradient (outside torch.no_grad()).
     """
     _op("key_bounds_paged")(k_cache, bounds, cu_seqlens_q, seqused_k, block_table,
                             int(max_seqlen_q))
@@ -44,9 +44,10 @@ def inkling_fa4_select_blocks_paged(q, bounds, cu_seqlens_q, seqused_k, block_ta
         score = sum over the kv head's query heads g and d of max(q_gd lo_d, q_gd hi_d),
     an upper bound of what any key of the block can reach, from q [total_q, Hq, D] (bf16, fp16)
     and bounds as inkling_fa4_key_bounds_paged leaves them (of q's dtype or float8_e4m3fn).
-    Scores are summed in 64 bits, so a list does not depend on the batch around it; equal scores
-    go to the lower block, a NaN counts as infinity.  max_seqlen_q and max_seqlen_k must bound
-    the lengths.
+    Scores are summed in 64 bits: only those closer than such a sum's rounding may rank either
+    way from one batch to another; equal bounds score equal, and equal scores go to the lower
+    block.  A score of NaN counts as infinity, and so does a block with an infinite or NaN bound.
+    max_seqlen_q and max_seqlen_k must bound the lengths.
     """
     return _call("select_blocks_paged", q, bounds, cu_seqlens_q, seqused_k, block_table,
                  int(block_size), int(max_seqlen_q), int(max_seqlen_k), int(n_select),
@@ -62,7 +63,8 @@ def inkling_fa4_rel_attention_sparse_paged(q, k_cache, v_cache, rel_logits, cu_s
     lists: blocks int32 [total_q, Hkv, n_select], as inkling_fa4_select_blocks_paged gives them
     or any other way.  An entry that is no block of the sequence (-1), lies past the token, or
     whose table entry lies outside the pool is passed over; a block named twice counts twice.
-    A token whose list holds no visible key: out 0, lse -inf.
+    A token whose list holds no visible key: out 0, lse -inf; rows of tokens that no sequence
+    holds are not written.  What a token does not see may hold anything, infinities and NaN too.
 
     The bias and the window go by the keys' positions in the sequence, listed or not.  GQA groups
     up to 16; caches, types and the other arguments as in inkling_fa4_rel_attention_paged.

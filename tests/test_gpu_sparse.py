@@ -5,6 +5,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwad
 
 from inkling_fa4 import (inkling_fa4_key_bounds_paged, inkling_fa4_kv_append_paged,
                          inkling_fa4_rel_attention_paged, inkling_fa4_rel_attention_sparse_paged,
@@ -118,6 +119,8 @@ def test_bounds_refusals(cuda):
             call(**kw)
     with pytest.raises(RuntimeError, match="gradient"):
         call(x=b.clone().requires_grad_())
+    with fwad.dual_level(), pytest.raises(NotImplementedError):
+        call(k=fwad.make_dual(kc, torch.ones_like(kc)))
     before = b._version
     call()
     assert b._version > before  # autograd sees the change

@@ -177,3 +177,13 @@ def test_select_workspace_and_nothing_to_do():
     # every list holds all blocks: no scores
     assert lib.ifa4_select_blocks_workspace_bytes(ref(select_args(n_select=500)), ref(paged())) == 0
     assert select(total_q=0) == OK and select(total_q=0, blocks=0, q=0) == OK
+
+
+def test_grids_of_less_than_2_to_the_32_threads():
+    """More workgroups than a launch holds are refused before it."""
+    wide = dict(kv_heads=1 << 12, n_heads=1 << 12, q_stride_t=1 << 19)
+    assert select(paged(max_blocks_per_seq=1 << 20), total_q=1, max_seqlen_q=1, max_seqlen_k=1 << 24,
+                  **wide) == EUNSUPPORTED
+    assert select(total_q=1 << 23) == EUNSUPPORTED
+    assert bounds(paged(max_blocks_per_seq=1 << 24), max_seqlen_q=1 << 28) == EUNSUPPORTED
+    assert sparse(args(total_q=(1 << 25) - 4), paged(), lists()) == EUNSUPPORTED
