@@ -479,9 +479,8 @@ int32_t run_sparse(const ifa4_args* a, const ifa4_paged_kv* kv, const ifa4_block
   p.n_select = ls->n_select;
   p.waves = l.plan.waves;
   p.splits = l.plan.splits;
-  const int64_t rows = (int64_t)ls->n_select * kv->block_size, parts = p.waves * p.splits;
+  const int64_t rows = (int64_t)ls->n_select * kv->block_size;
   p.steps = (int32_t)((rows + ifa4::kSparseStep - 1) / ifa4::kSparseStep);
-  p.part_steps = (int32_t)((p.steps + parts - 1) / parts);
   p.once = a->max_seqlen_q <= 1 ? 1 : 0;
   p.groups = (int32_t)(a->total_q * a->kv_heads * p.splits);
   p.per_xcd = (p.groups + 7) / 8;

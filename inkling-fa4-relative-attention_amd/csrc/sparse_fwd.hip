@@ -6,9 +6,9 @@
 //   out = softmax(x) V, lse = log sum exp(x), as in the paged decode.
 //
 // Work decomposition.  A workgroup of kNw waves takes one (token, kv head) or, for few of them, one
-// of `splits` shares of its list.  The listed rows laid end to end are cut into steps of 32 keys and
-// every wave takes an equal run of steps, with a softmax of its own; the waves meet in LDS, the
-// shares in a second pass.  A step is two halves of 16 keys, each in one block (blocks of 8 rows:
+// of `splits` shares of its list.  The listed rows laid end to end are cut into steps of 32 keys,
+// dealt to the waves in turn, each with a softmax of its own; the waves meet in LDS, the shares in
+// a second pass.  A step is two halves of 16 keys, each in one block (blocks of 8 rows:
 // four runs of 8).  A wave holds 64 entries of the list, one a lane, with what the steps need of
 // them as bit masks: which have a visible key at all (others are passed over), which are visible
 // whole and away from the bias (their steps take neither mask nor bias).
@@ -71,20 +71,36 @@ __device__ __forceinline__ u32x4_t fp8x8_operand(uint32_t lo, uint32_t hi) {
                  E::template fp8x2<false>(hi), E::template fp8x2<true>(hi)};
 }
 
+// 16 bytes at a wave's address plus a lane's offset, declared global memory: an address made from
+// integers counts as a flat one otherwise, and a wait for an LDS read then waits for the loads.
 template <bool kOnce>
-__device__ __forceinline__ u32x4_t ld_kv(const char* p) {
-  if constexpr (kOnce) return __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p));
-  return ld_global_16(p);
+__device__ __forceinline__ u32x4_t ld_kv(uint64_t base, uint32_t off) {
+  typedef const __attribute__((address_space(1))) char* bytes_t;
+  typedef const __attribute__((address_space(1))) u32x4_t* vec_t;
+  const vec_t p = reinterpret_cast<vec_t>(reinterpret_cast<bytes_t>(base) + off);
+  if constexpr (kOnce) return __builtin_nontemporal_load(p);
+  return *p;
 }
-__device__ __forceinline__ float rel_value(const SparseParams& p, int64_t off) {
-  if (p.rel_dtype == 2) return static_cast<const float*>(p.rel)[off];
-  const uint16_t x = static_cast<const uint16_t*>(p.rel)[off];
-  return p.rel_dtype == 0 ? __uint_as_float((uint32_t)x << 16) : (float)__builtin_bit_cast(_Float16, x);
+// Bias at distances d, d - 1, d - 2, d - 3 of a row; anything where that is none.
+__device__ __forceinline__ void rel_values(const SparseParams& p, int64_t row, int d, float* x) {
+  if (p.rel_dtype == 2) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      x[j] = static_cast<const float*>(p.rel)[row + min(max(d - j, 0), p.rel_extent - 1)];
+    return;
+  }
+  uint16_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    w[j] = static_cast<const uint16_t*>(p.rel)[row + min(max(d - j, 0), p.rel_extent - 1)];
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    x[j] = p.rel_dtype == 0 ? __uint_as_float((uint32_t)w[j] << 16) : (float)__builtin_bit_cast(_Float16, w[j]);
 }
 
 // kEight: blocks of 8 rows (not where one load takes 16: e4m3, d 64).  kOnce: one token a sequence,
-// no other will read its rows, and they pass the caches by (64 sequences x 128 blocks of 16 39.8 ->
-// 35.2 us, 128 x 256 111 -> 98; a branch in the kernel instead comes out as one plain load).
+// no other will read its rows, and they pass the caches by (64 sequences x 128 blocks of 16, a call,
+// 39.8 -> 35.2 us, 128 x 256 111 -> 98; a branch in the kernel instead comes out as one plain load).
 template <int D, typename Tag, int Eb, int kNw, bool kEight, bool kOnce>
 __global__ __launch_bounds__(64 * kNw) __attribute__((amdgpu_waves_per_eu(2))) void
 sparse_fwd_kernel(SparseParams p) {
@@ -107,18 +123,27 @@ sparse_fwd_kernel(SparseParams p) {
   const int split = (int)(at - item * (uint32_t)p.splits);
   const int kvh = (int)p.by_total.div(item), t = (int)(item - (uint32_t)kvh * (uint32_t)p.total_q);
   const int head0 = kvh * p.group;
+  const int my_head = head0 + min(n, p.group - 1);  // of column n
 
   // ---- what hangs on nothing but the item: list entries, Q --------------------------------------
   const int32_t* const list = p.blocks + (int64_t)t * p.ls_st + (int64_t)kvh * p.ls_sh;
-  const int s_beg = min((split * kNw + wave) * p.part_steps, p.steps);
-  const int s_end = min(s_beg + p.part_steps, p.steps);
-  int win = s_beg * kStep >> p.block_shift;  // lane l holds list entry win + l
-  int ent = win + lane < p.n_select ? list[win + lane] : -1;
-  // column n = query head n of the kv head
+  // Own step k of a wave is step k * stride + first of the list: steps near the token's position
+  // take the bias, and every wave has some of them.
+  const int stride = kNw * p.splits, first_step = split * kNw + wave;
+  const int s_end = first_step < p.steps ? (p.steps - first_step - 1) / stride + 1 : 0;
+  // Lane l holds the list entry of own step win + l / 4 or l / 2 in blocks of 8 and 16,
+  // which hold a quarter or a half of a step, else of win + l.
+  const int per_shift = p.block_shift < 5 ? 5 - p.block_shift : 0;
+  auto entry_of = [&](int step0) {
+    const int s = (step0 + (lane >> per_shift)) * stride + first_step;
+    return p.block_shift < 5 ? (s << per_shift) + (lane & ((1 << per_shift) - 1)) : s >> (p.block_shift - 5);
+  };
+  int win = 0, ent = -1;
+  if (const int e = entry_of(0); e < p.n_select) ent = list[e];
   u32x4_t qf[S::kKSteps];
   {
     const uint16_t* const src = static_cast<const uint16_t*>(p.q) + (int64_t)t * p.q_st +
-                                (int64_t)(head0 + min(n, p.group - 1)) * p.q_sh;
+                                (int64_t)my_head * p.q_sh;
 #pragma unroll
     for (int kk = 0; kk < S::kKSteps; ++kk) {
       const int d = Eb == 2 ? 32 * kk + 8 * g : 64 * (kk >> 1) + 16 * g + 8 * (kk & 1);
@@ -168,19 +193,18 @@ sparse_fwd_kernel(SparseParams p) {
     v_at = reinterpret_cast<uint64_t>(v_head + (int64_t)(any ? phys : 0) * p.v_sblk * Eb);
   };
   classify();
-  // Step s: entries e0 .. of the window hold its keys.
   constexpr int kRuns = kEight ? 4 : 2;
   const uint64_t step_bits = kEight ? 15 : bs == 16 ? 3 : 1;
-  auto seek = [&](int s) {  // first step from s on that reads anything
+  auto seek = [&](int s) {  // first own step from s on that reads anything
     for (; s < s_end; ++s) {
-      const int e0 = s * kStep >> p.block_shift, e3 = (s * kStep + kStep - 8) >> p.block_shift;
-      if (e3 >= win + 64) {
-        win = e0;
-        ent = win + lane < p.n_select ? list[win + lane] : -1;
+      if (s >= win + (64 >> per_shift)) {
+        win = s;
+        const int e = entry_of(win);
+        ent = e < p.n_select ? list[e] : -1;
         phys = lookup(ent);
         classify();
       }
-      if ((some >> (e0 - win)) & step_bits) break;
+      if ((some >> ((s - win) << per_shift)) & step_bits) break;
     }
     return s;
   };
@@ -201,16 +225,15 @@ sparse_fwd_kernel(SparseParams p) {
   };
   auto load = [&](int s, u32x4_t* kr, u32x4_t* vv) -> Step {
     Step st;
-    const int v0 = s * kStep, e0 = (v0 >> p.block_shift) - win;
+    const int v0 = (s * stride + first_step) * kStep, e0 = (s - win) << per_shift;
     st.plain = ((plain >> e0) & step_bits) == step_bits;
     st.pos = i32x4_t{kFar, kFar, kFar, kFar};
-    const char* kb[kRuns];
-    const char* vb[kRuns];
+    uint64_t kb[kRuns], vb[kRuns];
 #pragma unroll
     for (int r = 0; r < kRuns; ++r) {
-      const int v = v0 + kStep / kRuns * r, e = (v >> p.block_shift) - win;
-      kb[r] = reinterpret_cast<const char*>(scalar64(k_at, e)) + (uint32_t)((v & bmask) * k_rowb);
-      vb[r] = reinterpret_cast<const char*>(scalar64(v_at, e)) + (uint32_t)((v & bmask) * v_rowb);
+      const int v = v0 + kStep / kRuns * r, e = e0 + (kStep / kRuns * r >> p.block_shift);
+      kb[r] = scalar64(k_at, e) + (uint32_t)((v & bmask) * k_rowb);
+      vb[r] = scalar64(v_at, e) + (uint32_t)((v & bmask) * v_rowb);
       if (!st.plain) {
         const int first = ((int)__builtin_amdgcn_readlane(ent, e) << p.block_shift) + (v & bmask);
         if (((some >> e) & 1) && first <= pos && first + kStep / kRuns > kmin) st.pos[r] = first;
@@ -220,18 +243,18 @@ sparse_fwd_kernel(SparseParams p) {
     for (int i = 0; i < S::kLoads; ++i) {
       const int r = S::kRpi * i / (kStep / kRuns);  // run, first row in it
       const int off = S::kRpi * i % (kStep / kRuns);
-      kr[i] = ld_kv<kOnce>(kb[r] + (uint32_t)(off * k_rowb) + k_lane);
+      kr[i] = ld_kv<kOnce>(kb[r] + (uint32_t)(off * k_rowb), k_lane);
     }
 #pragma unroll
     for (int i = 0; i < S::kLoads; ++i) {
       const int r = S::kRpi * i / (kStep / kRuns);
       const int off = S::kRpi * i % (kStep / kRuns);
-      vv[i] = ld_kv<kOnce>(vb[r] + (uint32_t)(off * v_rowb) + v_lane);
+      vv[i] = ld_kv<kOnce>(vb[r] + (uint32_t)(off * v_rowb), v_lane);
     }
     return st;
   };
 
-  const int64_t rel_row = (int64_t)t * p.rel_st + (int64_t)(head0 + min(n, p.group - 1)) * p.rel_sh;
+  const int64_t rel_row = (int64_t)t * p.rel_st + (int64_t)my_head * p.rel_sh;
   const float c2 = p.scale_log2;
   float m_run = -INFINITY, l_run = 0.f;  // of head n (same over g; the sum over this lane's keys)
   f32x4_t o[S::kDBlocks];
@@ -240,7 +263,7 @@ sparse_fwd_kernel(SparseParams p) {
   uint8_t* const k_tile = tiles[wave];
   uint8_t* const tile = k_tile + S::kBytes;
 
-  auto compute = [&](const Step& st, const u32x4_t* kr, u32x4_t* vv) {
+  auto stage = [&](const Step& st, const u32x4_t* kr, u32x4_t* vv) {
     if (!st.plain) {  // V rows that the token does not see hold anything: zero
 #pragma unroll
       for (int i = 0; i < S::kLoads; ++i) {
@@ -261,6 +284,8 @@ sparse_fwd_kernel(SparseParams p) {
       *reinterpret_cast<u32x4_t*>(k_tile + key * D * Eb + 16 * (vc ^ kswz<D, Eb>(key))) = kr[i];
       *reinterpret_cast<u32x4_t*>(tile + row * D * Eb + 16 * (vc ^ vswz<D, Eb>(row))) = vv[i];
     }
+  };
+  auto compute = [&](const Step& st) {
     wave_lds_sync();
     f32x4_t acc[2];
 #pragma unroll
@@ -280,26 +305,31 @@ sparse_fwd_kernel(SparseParams p) {
       }
     }
     if (!st.plain) {
+      // positions of the lane's four keys of either half
+      int kp[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        if constexpr (kEight)
+          kp[b] = (g < 2 ? st.pos[2 * b] : st.pos[2 * b + 1]) + 4 * (g & 1);
+        else
+          kp[b] = st.pos[b] + 4 * g;
+      }
       // bias / softmax_scale joins the products, keys out of sight become -inf
       const float inv = kLog2e / c2;
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        // position of the lane's four keys
-        int kp;
-        if constexpr (kEight)
-          kp = (g < 2 ? st.pos[2 * b] : st.pos[2 * b + 1]) + 4 * (g & 1);
-        else
-          kp = st.pos[b] + 4 * g;
-        const bool near = n < p.group && pos - kp >= 0 && pos - kp - 3 < p.rel_extent;
-        if (p.rel_extent > 0 && wave_any(near)) {
+        const int d0 = pos - kp[b];
+        if (p.rel_extent > 0 && wave_any(d0 >= 0 && d0 - 3 < p.rel_extent)) {
+          float bias[4];  // loads in flight together
+          rel_values(p, rel_row, d0, bias);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int dist = pos - kp - j;
-            if (near && (uint32_t)dist < (uint32_t)p.rel_extent)
-              acc[b][j] = fmaf(rel_value(p, rel_row + dist), inv, acc[b][j]);
-          }
+          for (int j = 0; j < 4; ++j)
+            acc[b][j] = fmaf((uint32_t)(d0 - j) < (uint32_t)p.rel_extent ? bias[j] : 0.f, inv, acc[b][j]);
         }
-        const int hi = pos - kp, lo = kmin - kp;
+      }
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const int hi = pos - kp[b], lo = kmin - kp[b];
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[b][j] = j >= lo && j <= hi ? acc[b][j] : -INFINITY;
       }
@@ -357,18 +387,16 @@ sparse_fwd_kernel(SparseParams p) {
   };
 
   // ---- steps, the next one's rows in flight while one is computed ---------------------------------
-  Step st0{}, st1{};
-  u32x4_t k0[S::kLoads], k1[S::kLoads], v0[S::kLoads], v1[S::kLoads];
-  int s0 = seek(s_beg), s1;
-  if (s0 < s_end) st0 = load(s0, k0, v0);
-  while (s0 < s_end) {
-    s1 = seek(s0 + 1);
-    if (s1 < s_end) st1 = load(s1, k1, v1);
-    compute(st0, k0, v0);
-    if (s1 >= s_end) break;
-    s0 = seek(s1 + 1);
-    if (s0 < s_end) st0 = load(s0, k0, v0);
-    compute(st1, k1, v1);
+  u32x4_t kr[S::kLoads], vv[S::kLoads];
+  Step next{};
+  int s = seek(0);
+  if (s < s_end) next = load(s, kr, vv);
+  while (s < s_end) {
+    const Step st = next;
+    stage(st, kr, vv);
+    s = seek(s + 1);
+    if (s < s_end) next = load(s, kr, vv);
+    compute(st);
   }
 
   // ---- the waves' partials meet ---------------------------------------------------------------------

@@ -439,6 +439,82 @@ def test_sparse_reads_no_other_block(cuda, kv):
     c.check(got)
 
 
+# Many tokens.
+
+
+@pytest.mark.parametrize("hq,hkv,d,dtype,block", [
+    (8, 2, 128, torch.bfloat16, 16), (8, 2, 64, torch.float16, 16), (4, 4, 64, torch.bfloat16, 8),
+    (8, 1, 128, torch.float16, 32), (6, 2, 128, torch.bfloat16, 8), (10, 2, 64, torch.float16, 64),
+    (4, 2, 128, torch.bfloat16, 256), (7, 1, 128, torch.bfloat16, 16)])
+@pytest.mark.parametrize("kv", [None, F8])
+@pytest.mark.parametrize("messy", [False, True])
+def test_sparse_many_tokens(cuda, hq, hkv, d, dtype, block, kv, messy):
+    if kv and block * d < 1024:
+        pytest.skip("e4m3 blocks of one load at least")
+    news = [1400, 3, 700] if hkv > 2 else [900, 3, 170] if hkv > 1 else [530, 3, 40]
+    c = Sparse(news, [1500, 70, 2300], 9, messy, hq=hq, hkv=hkv, d=d, dtype=dtype, block=block, kv=kv,
+               extent=50, seed=hq + d + block)
+    c.check(run(c, cuda))
+
+
+@pytest.mark.parametrize("top", [1, 2, 40, 129, 512])
+@pytest.mark.parametrize("kv", [None, F8])
+def test_sparse_many_tokens_lists(cuda, top, kv):
+    c = Sparse([600, 0, 600], [1700, 9, 600], top, kv=kv, window=300 if top == 40 else -1, seed=top)
+    c.check(run(c, cuda))
+
+
+@pytest.mark.parametrize("kv", [None, F8])
+def test_sparse_many_tokens_that_list_alike(cuda, kv):
+    """All tokens the same blocks, one of them many times over."""
+    c = Sparse([1100], [1900], 20, kv=kv, seed=22)
+    c.lists[:] = torch.randint(0, 60, (20,), generator=torch.Generator().manual_seed(22)).to(torch.int32)
+    c.lists[500:, :, 3:9] = 7
+    c.check(run(c, cuda))
+    again = run(c, cuda)
+    assert all(torch.equal(a, b) for a, b in zip(again, run(c, cuda)))
+
+
+def test_sparse_many_tokens_edges(cuda):
+    """Tokens before the first key or with empty lists, entries outside the pool, other strides."""
+    c = Sparse([900, 200, 1], [500, 200, 40], 9, messy=True, seed=23)
+    c.table[0, 4], c.table[1, 3], c.table[1, 5] = -1, 1 << 20, c.kc.shape[0]
+    c.lists[300:420] = -1
+    c.check(run(c, cuda))
+    wide = torch.full((c.lists.shape[0], 3, 20), 5, dtype=torch.int32)
+    wide[:, 1:, 7:16] = c.lists
+    c.check(run(c, cuda, lists=wide.to(cuda)[:, 1:, 7:16]))
+
+
+@pytest.mark.parametrize("kv", [None, F8])
+def test_sparse_many_tokens_read_no_other_block(cuda, kv):
+    """Blocks that no list names, rows past the last key and rows left of the windows may hold NaN,
+    and a block that only a neighbour lists."""
+    c = Sparse([1040], [1600], 9, kv=kv, window=700, seed=24)
+    clean = c.kc, c.vc
+    c.lists[:, :, :4] = torch.randint(36, 60, (4,), generator=torch.Generator().manual_seed(24)).to(torch.int32)
+    c.lists[(c.lists >= 60) & (c.lists < 90)] = -1
+    keep = torch.zeros(c.kc.shape[:2], dtype=torch.bool)
+    for i in range(1040):
+        pos = 560 + i
+        for blk in set(c.lists[i].flatten().tolist()) - {-1}:
+            rows = torch.arange(c.block) + blk * c.block
+            keep[int(c.table[0, blk])] |= (rows <= pos) & (rows >= pos - 700)
+    assert not keep[c.table[0, 60:90].long()].any()
+    c.kc, c.vc = (torch.where(keep[..., None, None], x.float(), math.nan).to(x.dtype) for x in clean)
+    got = run(c, cuda)
+    c.kc, c.vc = (torch.nan_to_num(x.float(), 0.0).to(x.dtype) for x in (c.kc, c.vc))
+    c.check(got)
+    # a block of NaN costs the tokens that list it, no other
+    c.kc[int(c.table[0, 70])] = c.vc[int(c.table[0, 70])] = math.nan
+    c.lists = c.lists.clone()
+    c.lists[600:900:7, :, 5] = 70
+    out, lse = run(c, cuda)
+    hit = torch.zeros(1040, dtype=torch.bool)
+    hit[600:900:7] = True
+    assert not out[~hit].isnan().any() and not lse[:, ~hit].isnan().any()
+
+
 @pytest.mark.parametrize("layout", ["heads", "joint"])
 @pytest.mark.parametrize("kv", [None, F8])
 def test_sparse_layouts(cuda, layout, kv):
