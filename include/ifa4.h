@@ -312,7 +312,9 @@ int32_t ifa4_decode_quant_fwd(const ifa4_args* args, const ifa4_paged_kv* kv,
  * group.  The result is that of ifa4_prefill_fwd on the same keys stored contiguously, up to
  * the order of a split's merge.  Rows left of the first key that a tile of queries (128 at
  * most) sees and rows past the last may hold anything; of a key that one query of a tile sees
- * and another does not, key and value must be finite.  The workspace
+ * and another does not, key and value must be finite.  The bias joins the products as bias /
+ * (softmax_scale * k_scale) in fp32: a value so far below zero that the quotient overflows hides
+ * its key, as -inf does.  The workspace
  * (ifa4_prefill_paged_workspace_bytes, 0 for a call that does not split) as in
  * ifa4_prefill_fwd_ws.  The reference has no kernel for it.
  */
@@ -555,7 +557,8 @@ int32_t ifa4_select_blocks_paged(const ifa4_block_select* args, const ifa4_paged
  * window, j >= pos - window_left; the bias by pos - j.  An entry outside the sequence's table
  * (-1), a block past pos, and a block whose table entry lies outside the pool are passed over; a
  * block named twice counts twice.  A list that names all blocks gives ifa4_prefill_paged_fwd's
- * result up to rounding.  GQA groups up to 16; quant: NULL for a 16-bit cache.  The workspace
+ * result up to rounding (the bias as there).  What a token does not see may hold anything.  Rows of
+ * tokens of no sequence are not written.  GQA groups up to 16; quant: NULL for a 16-bit cache.  The workspace
  * (ifa4_sparse_paged_workspace_bytes, 0 where one pass takes the call) is scratch for one
  * call, 256-byte aligned.  The reference has no kernel for it.
  */

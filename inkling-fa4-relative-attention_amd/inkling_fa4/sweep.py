@@ -30,7 +30,8 @@ pointing at its directory; a variant whose output on a small case differs from
 the in-tree build's (atol 2e-2 on out, 1e-3 on lse) is reported and not timed.
 
 Knobs (macros of the kernel sources):
-  prefill_kernel.hpp  IFA4_LOOK_K, IFA4_LOOK_V   LDS reads in flight ahead of the QK / PV MFMAs
+  prefill_kernel.hpp
+                   IFA4_LOOK_K, IFA4_LOOK_V   LDS reads in flight ahead of the QK / PV MFMAs
                    IFA4_PRIO                  raised wave priority around MFMA blocks (0/1)
                    IFA4_SCHED                 scheduling groups (0/1)
                    IFA4_PV2                   key-block-major PV (0/1)
