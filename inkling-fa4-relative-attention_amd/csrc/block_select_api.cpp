@@ -94,14 +94,16 @@ int32_t check_select(const ifa4_block_select* a, const ifa4_paged_kv* kv) {
                       a->head_dim, a->kv_dtype == IFA4_FP8_E4M3 ? 1 : 2, false);
 }
 
+// Blocks of the longest sequence; 0 where no sequence has a token.
 int32_t select_cols(const ifa4_block_select* a, const ifa4_paged_kv* kv) {
+  if (a->batch == 0 || a->max_seqlen_q == 0) return 0;
   return (int32_t)(((int64_t)a->max_seqlen_k + kv->block_size - 1) / kv->block_size);
 }
 
 // Scores of all tokens, where a list can leave a block out.
 size_t select_bytes(const ifa4_block_select* a, const ifa4_paged_kv* kv) {
   const int64_t cols = select_cols(a, kv);
-  if (a->total_q == 0 || a->batch == 0 || cols <= a->n_select) return 0;
+  if (a->total_q == 0 || cols <= a->n_select) return 0;
   return (size_t)((a->total_q * a->kv_heads * cols * 8 + 255) / 256 * 256);
 }
 

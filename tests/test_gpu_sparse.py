@@ -268,6 +268,17 @@ def test_select_edges(cuda):
     assert run_select(c, key_like_bounds(c), 3, 0, 1, cuda).shape == (0, 2, 3)
 
 
+def test_select_without_sequences_or_queries(cuda):
+    """Tokens of no sequence: -1 throughout, also where there is no sequence, or none has a query."""
+    c = Case([2, 20], [1500, 3000], seed=13)
+    q, _, _, _, cu, used, table = c.on(cuda)
+    b = key_like_bounds(c).to(cuda)
+    for cu2, n in ((cu[:1], 0), (torch.zeros_like(cu), 2)):
+        got = inkling_fa4_select_blocks_paged(q, b, cu2, used[:n], table[:n], 16, 0, 3000, 20)
+        assert got.shape == (22, 2, 20) and (got == -1).all()
+    torch.cuda.synchronize()
+
+
 def test_select_strides(cuda):
     c = Case([2, 20], [1500, 3000], seed=14)
     b = key_like_bounds(c)
@@ -513,6 +524,29 @@ def test_sparse_many_tokens_read_no_other_block(cuda, kv):
     hit = torch.zeros(1040, dtype=torch.bool)
     hit[600:900:7] = True
     assert not out[~hit].isnan().any() and not lse[:, ~hit].isnan().any()
+
+
+@pytest.mark.parametrize("low", [-math.inf, torch.finfo(torch.bfloat16).min])
+@pytest.mark.parametrize("news,lens", [([70, 1, 9], [200, 40, 60]), ([1, 1, 1], [900, 40, 5])])
+def test_biases_that_hide_keys(cuda, low, news, lens):
+    """-inf, and the type's lowest value, whose quotient by the scale leaves fp32: the key is hidden;
+    a row whose bias hides all of its keys is empty.  Listed blocks and the whole cache alike."""
+    c = Sparse(news, lens, 130, extent=64, seed=25)
+    c.lists = torch.arange(130, dtype=torch.int32).expand(sum(news), c.hkv, 130).contiguous()
+    g = torch.Generator().manual_seed(25)
+    c.rel[torch.rand(c.rel.shape, generator=g) < 0.3] = low
+    c.rel[-1] = low
+    args, lists = c.on(cuda), c.lists.to(cuda)
+    got = [x.cpu() for x in inkling_fa4_rel_attention_sparse_paged(*args, lists, c.max_q, c.max_k,
+                                                                   c.extent, **c.settings())]
+    whole = [x.cpu() for x in inkling_fa4_rel_attention_paged(*args, c.max_q, c.max_k, c.extent,
+                                                              **c.settings())]
+    c.rel[c.rel == low] = -math.inf
+    for out, lse in (got, whole):
+        assert not out.isnan().any() and not lse.isnan().any()
+        c.check((out, lse))
+    if lens[-1] <= 64:
+        assert not got[0][-1].any() and got[1][:, -1].isneginf().all()
 
 
 @pytest.mark.parametrize("layout", ["heads", "joint"])

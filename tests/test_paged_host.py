@@ -176,6 +176,9 @@ def test_select_workspace_and_nothing_to_do():
     assert select(ws=P + 8, n=n) == EWORKSPACE
     # every list holds all blocks: no scores
     assert lib.ifa4_select_blocks_workspace_bytes(ref(select_args(n_select=500)), ref(paged())) == 0
+    # nor where no sequence has a token
+    for kw in (dict(batch=0), dict(max_seqlen_q=0)):
+        assert lib.ifa4_select_blocks_workspace_bytes(ref(select_args(**kw)), ref(paged())) == 0
     assert select(total_q=0) == OK and select(total_q=0, blocks=0, q=0) == OK
 
 
