@@ -419,9 +419,11 @@ struct SparseLayout {
   int64_t o_bytes, ml_bytes;
   int64_t total() const { return plan.splits > 1 ? o_bytes + ml_bytes : 0; }
 };
-SparseLayout sparse_layout(const ifa4_args* a, const ifa4_paged_kv* kv, const ifa4_block_list* ls) {
+SparseLayout sparse_layout(const ifa4_args* a, const ifa4_paged_kv* kv, const ifa4_block_list* ls,
+                           const ifa4_kv_quant* qt) {
   SparseLayout l;
-  l.plan = ifa4::sparse_plan(a->total_q * a->kv_heads, (int64_t)ls->n_select * kv->block_size);
+  l.plan = ifa4::sparse_plan(a->total_q * a->kv_heads, (int64_t)ls->n_select * kv->block_size,
+                             2 * a->head_dim * (qt != nullptr ? 1 : 2));
   const int64_t rows = l.plan.splits * a->total_q * a->n_heads;
   l.o_bytes = (rows * a->head_dim * 4 + 255) / 256 * 256;
   l.ml_bytes = (rows * 8 + 255) / 256 * 256;
@@ -432,7 +434,7 @@ int32_t run_sparse(const ifa4_args* a, const ifa4_paged_kv* kv, const ifa4_block
                    const ifa4_kv_quant* qt, void* workspace, size_t workspace_bytes, void* stream) {
   const int32_t st = check_sparse(a, kv, ls, qt);
   if (st != IFA4_OK || no_queries(a)) return st;
-  const SparseLayout l = sparse_layout(a, kv, ls);
+  const SparseLayout l = sparse_layout(a, kv, ls, qt);
   if (l.total() > 0 && (workspace == nullptr || workspace_bytes < (size_t)l.total() ||
                         !aligned(workspace, 256)))
     return IFA4_EWORKSPACE;
@@ -865,7 +867,7 @@ int32_t ifa4_prefill_paged_fwd(const ifa4_args* args, const ifa4_paged_kv* kv,
 size_t ifa4_sparse_paged_workspace_bytes(const ifa4_args* args, const ifa4_paged_kv* kv,
                                          const ifa4_block_list* list, const ifa4_kv_quant* quant) {
   if (check_sparse(args, kv, list, quant) != IFA4_OK || no_queries(args)) return 0;
-  return (size_t)sparse_layout(args, kv, list).total();
+  return (size_t)sparse_layout(args, kv, list, quant).total();
 }
 
 int32_t ifa4_sparse_paged_fwd(const ifa4_args* args, const ifa4_paged_kv* kv,

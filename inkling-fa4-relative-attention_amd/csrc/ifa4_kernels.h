@@ -278,16 +278,22 @@ constexpr int kSparseStep = 32;
 // whose partials a second pass joins.  Kernel us with 2048 / 4096 waves: 64 sequences x 128 blocks of
 // 16 28.6 / 32.1, 512 tokens x 100 blocks of e4m3 40.5 / 39.5, 4 sequences x 16 blocks of 64 9.0 / 8.2.
 constexpr int kSparseWaves = 2048;
+// A workgroup takes in about 53 KB a us, the second pass takes 3.5 us: shares pay where they take more
+// than this many bytes of K and V off a workgroup.  A call in us, one workgroup a list / shares:
+// lists of 256 KiB (16 blocks of 64, d 64; 4 sequences, 2 shares) 9.3 / 11.9, of 512 KiB (128 of 16, e4m3;
+// 4 sequences, 4 shares) 15.6 / 13.0, of 1 MiB (the same, bf16) 24.8 / 15.6.
+constexpr int64_t kSparseSplitBytes = 192 << 10;
 struct SparsePlan {
   int32_t waves, splits;
 };
-inline SparsePlan sparse_plan(int64_t items, int64_t rows) {
+inline SparsePlan sparse_plan(int64_t items, int64_t rows, int64_t row_bytes) {
   const int64_t steps = (rows + kSparseStep - 1) / kSparseStep;
   int64_t want = items > 0 ? (kSparseWaves + items - 1) / items : 1;
   if (want > steps / 2) want = steps / 2;
   SparsePlan pl{1, 1};
   while (pl.waves < 8 && 2 * pl.waves <= want) pl.waves *= 2;
-  const int64_t s = want / pl.waves;
+  int64_t s = want / pl.waves;
+  if (s > 1 && rows * row_bytes / s * (s - 1) <= kSparseSplitBytes) s = 1;
   pl.splits = (int32_t)(s < 1 ? 1 : s);
   return pl;
 }
