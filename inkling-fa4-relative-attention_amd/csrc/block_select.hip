@@ -281,7 +281,7 @@ __global__ __launch_bounds__(64 * kScoreWaves) void score_tile_kernel(SelectPara
 // One token of a sequence against its blocks, on the vector unit: a lane group of 8 takes a block
 // (lane `sub`: the chunks sub modulo 8), qn and qp of a lane's elements stay in registers, a wave
 // walks over 64 blocks (one load of their table entries), the next 8 blocks' bounds in flight
-// while 8 are summed.
+// while 8 are summed (24 or 32 in flight cost a wave per SIMD: 39 us instead of 30).
 constexpr int kStepBlocks = 64;  // of a wave
 template <int Ctrl>
 __device__ __forceinline__ double dpp_add(double x) {
@@ -297,8 +297,10 @@ __global__ __launch_bounds__(64 * kScoreWaves) void score_step_kernel(SelectPara
   constexpr int kChunks = 2 * kHalf / 8;     // of a lane
   const int lane = threadIdx.x & 63, wave = (int)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int seq = blockIdx.y;
-  const int part0 = blockIdx.x % p.score_parts, rest = blockIdx.x / p.score_parts;
-  const int h = rest % p.kv_heads, i0 = rest / p.kv_heads;
+  // kv heads side by side: their bounds of a block are neighbours in memory (64 sequences over 2000
+  // blocks, a call: 31.1 -> 30.2 us)
+  const int h = blockIdx.x % p.kv_heads, rest = blockIdx.x / p.kv_heads;
+  const int part0 = rest % p.score_parts, i0 = rest / p.score_parts;
   const TokenSpan s = token_span(p, seq);
   if (i0 >= s.len) return;
   const int nb = token_blocks(p, s, i0);
