@@ -409,12 +409,13 @@ sparse_fwd_kernel(SparseParams p) {
       if (d == 0) p.part_ml[row] = make_float2(m, l);
       return;
     }
-    const float inv = l > 0.f ? p.v_scale / l : 0.f;
+    // l is 0 for a row without keys, NaN where a key is: then the LSE is too
+    const float inv = l == 0.f ? 0.f : p.v_scale / l;
     *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(p.out) + (int64_t)t * p.o_st +
                                 (int64_t)head * p.o_sh + d) =
         u32x2_t{E::pack2(sum[0] * inv, sum[1] * inv), E::pack2(sum[2] * inv, sum[3] * inv)};
     if (p.lse != nullptr && d == 0)
-      p.lse[(int64_t)head * p.lse_sh + t] = l > 0.f ? (m + __log2f(l)) * kLn2 : -INFINITY;
+      p.lse[(int64_t)head * p.lse_sh + t] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
   };
   if constexpr (kNw == 1) {
     if (n < p.group) {
@@ -477,11 +478,11 @@ __global__ __launch_bounds__(kJoinThreads) void sparse_join_kernel(SparseParams 
     lt += a * ml.y;
     sum += a * *reinterpret_cast<const f32x4_t*>(p.part_o + (s * rows + row) * D + d);
   }
-  const float inv = lt > 0.f ? p.v_scale / lt : 0.f;
+  const float inv = lt == 0.f ? 0.f : p.v_scale / lt;
   *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(p.out) + t * p.o_st + (int64_t)head * p.o_sh + d) =
       u32x2_t{E::pack2(sum[0] * inv, sum[1] * inv), E::pack2(sum[2] * inv, sum[3] * inv)};
   if (p.lse != nullptr && d == 0)
-    p.lse[(int64_t)head * p.lse_sh + t] = lt > 0.f ? (mt + __log2f(lt)) * kLn2 : -INFINITY;
+    p.lse[(int64_t)head * p.lse_sh + t] = lt == 0.f ? -INFINITY : (mt + __log2f(lt)) * kLn2;
 }
 
 template <int D, typename Tag, int Eb, int kNw, bool kOnce>
