@@ -1363,7 +1363,8 @@ __device__ __forceinline__ void prefill_work(const PrefillParams& p, const WorkI
 #pragma unroll
   for (int qb = 0; qb < kNqb; ++qb) {
     const float l_tot = add_xor32(l_run[qb]);
-    const float inv = l_tot > 0.f ? (kRaw ? p.v_scale : 1.f) / l_tot : 0.f;
+    // l_tot is 0 for a row without keys, NaN where a key is: then the LSE is too
+    const float inv = l_tot == 0.f ? 0.f : (kRaw ? p.v_scale : 1.f) / l_tot;
     const int r_e = row0 + 32 * qb + (lane_e & 31);
     const int ql_e = kPack ? packed_query(p, r_e) : r_e;
     const int qi_e = q0 + ql_e;
@@ -1380,7 +1381,7 @@ __device__ __forceinline__ void prefill_work(const PrefillParams& p, const WorkI
           *reinterpret_cast<f32x4_t*>(pbase + 32 * db + 8 * i + 4 * half_e) =
               f32x4_t{o[qb][db][4 * i] * inv, o[qb][db][4 * i + 1] * inv,
                       o[qb][db][4 * i + 2] * inv, o[qb][db][4 * i + 3] * inv};
-      if (half_e == 0) p.part_lse[prow] = l_tot > 0.f ? m_run[qb] + __log2f(l_tot) : -INFINITY;
+      if (half_e == 0) p.part_lse[prow] = l_tot == 0.f ? -INFINITY : m_run[qb] + __log2f(l_tot);
     } else if (ok_e) {
       uint16_t* obase = static_cast<uint16_t*>(p.out) + (int64_t)(qs + qi_e) * p.o_st +
                         (int64_t)head_e * p.o_sh;
@@ -1395,7 +1396,7 @@ __device__ __forceinline__ void prefill_work(const PrefillParams& p, const WorkI
         }
       }
       if (p.lse != nullptr && half_e == 0) {
-        const float lse = l_tot > 0.f ? (m_run[qb] + __log2f(l_tot)) * kLn2 : -INFINITY;
+        const float lse = l_tot == 0.f ? -INFINITY : (m_run[qb] + __log2f(l_tot)) * kLn2;
         p.lse[(int64_t)head_e * p.lse_sh + qs + qi_e] = lse;
       }
     }
@@ -1555,7 +1556,7 @@ __global__ __launch_bounds__(kMergeThreads) void prefill_merge_kernel(PrefillPar
     }
     m = mn;
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
   uint16_t* dst = static_cast<uint16_t*>(p.out) + (int64_t)(bq.start + row) * p.o_st +
                   (int64_t)head * p.o_sh + d0;
   if constexpr (kPer == 4) {
@@ -1566,7 +1567,7 @@ __global__ __launch_bounds__(kMergeThreads) void prefill_merge_kernel(PrefillPar
   }
   if (p.lse != nullptr && d0 == 0)
     p.lse[(int64_t)head * p.lse_sh + bq.start + row] =
-        l > 0.f ? (m + __log2f(l)) * kLn2 : -INFINITY;
+        l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
 }
 
 static_assert(ProjShape::kBlockK == Shape::kBlockK, "one merge kernel for both");

@@ -5,7 +5,8 @@ import math
 import pytest
 import torch
 
-from inkling_fa4 import inkling_fa4_rel_attention_sparse_paged
+from inkling_fa4 import (inkling_fa4_rel_attention, inkling_fa4_rel_attention_paged,
+                         inkling_fa4_rel_attention_rproj, inkling_fa4_rel_attention_sparse_paged)
 from paged_cases import F8, Case
 
 pytestmark = pytest.mark.gpu
@@ -27,20 +28,32 @@ def spoil(c, hits):
     return rows
 
 
-def check(c, rows, got, clean):
+def tiles(c, hits):
+    """Rows of the sequences and heads of the hits: those beside a row that sees a hit which they do
+    not see are unspecified in the prefill, whose tiles of queries take finite keys only."""
+    rows = torch.zeros(sum(c.news), c.hq, dtype=torch.bool)
+    group = c.hq // c.hkv
+    for seq, _, kvh in hits:
+        start = sum(c.news[:seq])
+        rows[start:start + c.news[seq], kvh * group:(kvh + 1) * group] = True
+    return rows
+
+
+def check(c, rows, got, clean, beside):
     print("nan rows:", c.told(), flush=True)
     (out, lse), (out0, lse0) = ([x.cpu() for x in r] for r in (got, clean))
     assert rows.any() and not rows.all()
     assert out[rows].isnan().all() and lse.t()[rows].isnan().all()
-    assert torch.equal(out[~rows], out0[~rows]) and torch.equal(lse.t()[~rows], lse0.t()[~rows])
+    same = ~(rows | beside)
+    assert torch.equal(out[same], out0[same]) and torch.equal(lse.t()[same], lse0.t()[same])
 
 
-def both(c, hits, dev, call):
+def both(c, hits, dev, call, tiled=False):
     clean = call(*c.on(dev))
     rows = spoil(c, hits)
     got = call(*c.on(dev))
     torch.cuda.synchronize()
-    check(c, rows, got, clean)
+    check(c, rows, got, clean, tiles(c, hits) if tiled else torch.zeros_like(rows))
 
 
 # sequences x tokens x list: one wave a list, some waves, lists shared by several workgroups
@@ -69,3 +82,56 @@ def test_sparse_rows_of_nothing_but_nan(cuda, lens):
                                                       **c.settings())
 
     both(c, [(0, j, 0) for j in range(lens[0])], cuda, call)
+
+
+# one pass, packed heads, few tiles cut into chunks, a ragged batch cut into chunks
+PREFILLS = [([100, 3], [100, 90]), ([4, 3], [1000, 700]), ([128, 40], [3000, 2000]),
+            ([500] + [60] * 15, [7000] + [500] * 15)]
+
+
+@pytest.mark.parametrize("news,lens", PREFILLS)
+@pytest.mark.parametrize("kv", [None, F8])
+def test_paged_prefill(cuda, news, lens, kv):
+    c = Case(news, lens, kv=kv, seed=len(news))
+
+    def call(*a):
+        return inkling_fa4_rel_attention_paged(*a, c.max_q, c.max_k, c.extent, **c.settings())
+
+    both(c, [(0, 0, 1), (1, 5, 0)], cuda, call, tiled=True)
+
+
+def contiguous(c, kc, vc, table):
+    """K and V of a case's sequences one after the other, and their offsets."""
+    k, v = (torch.cat([x[table[b, torch.arange(lk, device=x.device) // c.block].long(),
+                         torch.arange(lk, device=x.device) % c.block]
+                       for b, lk in enumerate(c.lens)]) for x in (kc, vc))
+    cu = torch.tensor([0] + c.lens, dtype=torch.int32).cumsum(0).to(torch.int32)
+    return k, v, cu.to(k.device)
+
+
+@pytest.mark.parametrize("news,lens", PREFILLS[:3] + [([500, 300], [9000, 200])])
+def test_prefill(cuda, news, lens):
+    c = Case(news, lens, seed=7)
+
+    def call(q, kc, vc, rel, cu, used, table):
+        k, v, cu_k = contiguous(c, kc, vc, table)
+        return inkling_fa4_rel_attention(q, k, v, rel, cu, cu_k, c.max_q, c.max_k, c.extent,
+                                         softmax_scale=c.scale, return_lse=True, bottom_right=True)
+
+    both(c, [(0, 0, 1), (1, 5, 0)], cuda, call, tiled=True)
+
+
+@pytest.mark.parametrize("news,lens", [([100, 3], [100, 90]), ([128, 40], [3000, 2000])])
+def test_projected_prefill(cuda, news, lens):
+    c = Case(news, lens, seed=8)
+    g = torch.Generator().manual_seed(8)
+    r = torch.randn(sum(news), c.hq, 16, generator=g).to(cuda)
+    w = torch.randn(16, c.extent, generator=g).to(cuda)
+
+    def call(q, kc, vc, rel, cu, used, table):
+        k, v, cu_k = contiguous(c, kc, vc, table)
+        return inkling_fa4_rel_attention_rproj(q, k, v, r, w, cu, cu_k, c.max_q, c.max_k, c.extent,
+                                               softmax_scale=c.scale, return_lse=True,
+                                               bottom_right=True)
+
+    both(c, [(0, 0, 1), (1, 5, 0)], cuda, call, tiled=True)
