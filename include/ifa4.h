@@ -18,7 +18,8 @@
  *     out[qs+i,h] = softmax_j(s) @ v[ks+j,kh]           (written in the q dtype)
  *     lse[h, qs+i] = ln sum_j exp(s)  over visible j     (fp32, optional)
  * A row with no visible key gets out = 0 and lse = -inf (the reference oracle
- * yields NaN there; the reference Triton kernels yield 0).
+ * yields NaN there; the reference Triton kernels yield 0).  A row that sees a key
+ * whose score is NaN gets NaN in both.
  */
 #ifndef IFA4_H_
 #define IFA4_H_

@@ -862,8 +862,9 @@ decode_stream_kernel(DecodeParams p) {
     if (kNw > 0 || !last) return;
     // ---- partial of (segment, wave): normalise, store ------------------------------
     const float l_tot = add_xor32(add_xor16(l_run));  // per head n, all g
-    const float inv = l_tot > 0.f ? p.v_scale / l_tot : 0.f;  // V scale (1 for 16-bit V)
-    const float lse2 = l_tot > 0.f ? m_run + __log2f(l_tot) : -INFINITY;
+    // l_tot is 0 for a row without keys, NaN where a key is: then the LSE is too
+    const float inv = l_tot == 0.f ? 0.f : p.v_scale / l_tot;  // V scale (1 for 16-bit V)
+    const float lse2 = l_tot == 0.f ? -INFINITY : m_run + __log2f(l_tot);
     put_partial(cu.seg + w, inv, lse2);
   };
 
@@ -1040,7 +1041,7 @@ decode_stream_kernel(DecodeParams p) {
         out += a * *reinterpret_cast<const f32x4_t*>(reinterpret_cast<const float*>(k_tiles[i]) +
                                                      h * D + d);
       }
-      const float inv = lt > 0.f ? p.v_scale / lt : 0.f;
+      const float inv = lt == 0.f ? 0.f : p.v_scale / lt;
       const int head = cur[0].kvh * g_act + h;
       uint16_t* dst = static_cast<uint16_t*>(p.out) + (int64_t)cur[0].qs * p.o_st +
                       (int64_t)head * p.o_sh + d;
@@ -1048,7 +1049,7 @@ decode_stream_kernel(DecodeParams p) {
           u32x2_t{E::pack2(out[0] * inv, out[1] * inv), E::pack2(out[2] * inv, out[3] * inv)};
       if (p.lse != nullptr && d == 0)
         p.lse[(int64_t)head * p.lse_sh + cur[0].qs] =
-            lt > 0.f ? (mt + __log2f(lt)) * kLn2 : -INFINITY;
+            lt == 0.f ? -INFINITY : (mt + __log2f(lt)) * kLn2;
     }
   }
 }
@@ -1164,13 +1165,13 @@ __global__ __launch_bounds__(64 * kCombineWaves) void decode_combine_kernel(Deco
     lt += a * part_l[g];
     out += a * part_o[g][c];
   }
-  const float inv = lt > 0.f ? 1.f / lt : 0.f;
+  const float inv = lt == 0.f ? 0.f : 1.f / lt;
   uint16_t* dst = static_cast<uint16_t*>(p.out) + (int64_t)qs * p.o_st + (int64_t)head * p.o_sh +
                   4 * cc;
   *reinterpret_cast<u32x2_t*>(dst) =
       u32x2_t{E::pack2(out[0] * inv, out[1] * inv), E::pack2(out[2] * inv, out[3] * inv)};
   if (p.lse != nullptr && cc == 0) {
-    p.lse[(int64_t)head * p.lse_sh + qs] = lt > 0.f ? (mu + __log2f(lt)) * kLn2 : -INFINITY;
+    p.lse[(int64_t)head * p.lse_sh + qs] = lt == 0.f ? -INFINITY : (mu + __log2f(lt)) * kLn2;
   }
 }
 

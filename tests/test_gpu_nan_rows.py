@@ -1,12 +1,16 @@
 """A key of NaN that a row sees makes both of the row's results NaN: an LSE of -inf beside it
-would tell a caller that merges partial results that the row has no keys."""
+would tell a caller that merges partial results that the row has no keys.  Every attention
+operator, in the forms that a call can take (one pass, shares joined by a second)."""
 import math
 
 import pytest
 import torch
 
-from inkling_fa4 import (inkling_fa4_rel_attention, inkling_fa4_rel_attention_paged,
-                         inkling_fa4_rel_attention_rproj, inkling_fa4_rel_attention_sparse_paged)
+from inkling_fa4 import (inkling_fa4_rel_attention, inkling_fa4_rel_attention_decode,
+                         inkling_fa4_rel_attention_decode_paged,
+                         inkling_fa4_rel_attention_decode_shared_prefix,
+                         inkling_fa4_rel_attention_paged, inkling_fa4_rel_attention_rproj,
+                         inkling_fa4_rel_attention_sparse_paged)
 from paged_cases import F8, Case
 
 pytestmark = pytest.mark.gpu
@@ -135,3 +139,34 @@ def test_projected_prefill(cuda, news, lens):
                                                bottom_right=True)
 
     both(c, [(0, 0, 1), (1, 5, 0)], cuda, call, tiled=True)
+
+
+# one launch, and waves whose partials are combined
+@pytest.mark.parametrize("lens", [[300, 90], [9000, 5000, 70]])
+@pytest.mark.parametrize("kv", [None, F8])
+@pytest.mark.parametrize("paged", [False, True])
+def test_decode(cuda, lens, kv, paged):
+    c = Case([1] * len(lens), lens, kv=kv, seed=9)
+
+    def call(q, kc, vc, rel, cu, used, table):
+        if paged:
+            return inkling_fa4_rel_attention_decode_paged(
+                q, kc, vc, rel, cu, used, table, 1, c.max_k, c.extent, bottom_right=True, **c.settings())
+        raw = [x.view(torch.uint8) if kv else x for x in (kc, vc)]
+        k, v, cu_k = contiguous(c, *raw, table)
+        return inkling_fa4_rel_attention_decode(q, k.view(kc.dtype), v.view(kc.dtype), rel, cu, cu_k, 1,
+                                                c.max_k, c.extent, bottom_right=True, **c.settings())
+
+    both(c, [(0, 0, 1), (1, 60, 0)], cuda, call)
+
+
+@pytest.mark.parametrize("kv", [None, F8])
+def test_shared_prefix_decode(cuda, kv):
+    c = Case([1, 1, 1], [900, 700, 40], kv=kv, seed=10)
+
+    def call(q, kc, vc, rel, cu, used, table):
+        return inkling_fa4_rel_attention_decode_shared_prefix(
+            q, kc, vc, rel, cu, used, table, table[0, :2].contiguous(), 0, 1, c.max_k, c.extent,
+            **c.settings())
+
+    both(c, [(0, 0, 1), (1, 60, 0)], cuda, call)
