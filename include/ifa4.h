@@ -311,9 +311,9 @@ int32_t ifa4_decode_quant_fwd(const ifa4_args* args, const ifa4_paged_kv* kv,
  * (bottom-right alignment; args.flags must hold IFA4_FLAG_BOTTOM_RIGHT) for the causal mask,
  * the window and the bias distance.  quant: NULL for a 16-bit cache, else an e4m3 one; any GQA
  * group.  The result is that of ifa4_prefill_fwd on the same keys stored contiguously, up to
- * the order of a split's merge.  Rows left of the first key that a tile of queries (128 at
- * most) sees and rows past the last may hold anything; of a key that one query of a tile sees
- * and another does not, key and value must be finite.  The bias joins the products as bias /
+ * the order of a split's merge.  For the results of a tile of queries (128 at most), rows left
+ * of the first key that one of them sees and rows past the last such key may hold anything; of a
+ * key that one query of a tile sees and another does not, key and value must be finite.  The bias joins the products as bias /
  * (softmax_scale * k_scale) in fp32: a value so far below zero that the quotient overflows hides
  * its key, as -inf does.  The workspace
  * (ifa4_prefill_paged_workspace_bytes, 0 for a call that does not split) as in

@@ -62,12 +62,13 @@
 // Paged cache (KvPaged, KvPaged8).  A wave DMA covers 1 KiB of one tensor, 4 to 16 rows that
 // lie in one block (the host checks that a block holds them), so each DMA goes through a
 // resource of its own: base at the DMA's first row in its block, size ending with the
-// sequence's last row, empty for an entry outside the pool.  Lane u works out DMA u's
+// last row that the tile's queries see, empty for an entry outside the pool.  Lane u works out DMA u's
 // resource (one table entry, two 64-bit products) and the wave reads the lanes' results
 // into scalar registers, so eight resources cost what one would; the table entry of the
 // tile after next is loaded while a tile is computed.  Rows left of the first key that
-// the tile's queries see read as zero too: a cache may hold anything in blocks that a
-// window has left behind.
+// the tile's queries see read as zero too.  So what a window has left behind and what
+// later tokens have written may be anything; the masks are additive and take finite
+// scores only.
 //   e4m3 (KvPaged8): the DMA brings the bytes into two raw stages of half the size; when a
 // tile's bytes have landed, every thread turns its share into the 16-bit type (exact, one
 // conversion a pair) in the one stage that the products read.  Its scales go into the
@@ -482,25 +483,26 @@ __device__ __forceinline__ void prefill_work(const PrefillParams& p, const WorkI
   [[maybe_unused]] const rsrc_t rtable =
       make_rsrc(kPaged ? p.block_table + it.seq * p.bt_stride : nullptr,
                 kPaged ? (uint32_t)p.max_blocks * 4u : 0u);
+  // keys [kzero, kseen) hold those that some query of the tile sees: other rows read as zero
+  const int kzero = kPaged && wl >= 0 && !p.no_prune ? max(0, q0 + qpos - wl) : 0;
+  const int kseen = kPaged && p.causal && !p.no_prune ? min(lk, it.q_end + qpos) : lk;
   auto load_entry = [&](int kt) {
     const int key = kt * kBlockK + dma_first;
     dma_entry = (int)buf_load_4(
-        rtable, key < lk ? (uint32_t)(key >> p.block_shift) * 4u : kOutOfRange);
+        rtable, key < kseen ? (uint32_t)(key >> p.block_shift) * 4u : kOutOfRange);
   };
-  // first key that some query of the tile sees: rows left of it read as zero
-  const int kzero = kPaged && wl >= 0 && !p.no_prune ? max(0, q0 + qpos - wl) : 0;
   auto dma_paged = [&](int kt, uint16_t* stage) {
     const int kb = kt * kBlockK;
     const uint32_t stage_lds = lds_stages + (uint32_t)((stage - stages) * 2);
     const int key = kb + dma_first;
-    const bool ok = key < lk && (uint32_t)dma_entry < (uint32_t)p.num_blocks;
+    const bool ok = key < kseen && (uint32_t)dma_entry < (uint32_t)p.num_blocks;
     const int64_t row = key & ((1 << p.block_shift) - 1);
     const uint64_t base =
         reinterpret_cast<uint64_t>(dma_base) +
         (uint64_t)(((int64_t)(ok ? dma_entry : 0) * (dma_v ? p.v_sblk : p.k_sblk) +
                     row * (dma_v ? p.v_st : p.k_st)) * Kv::kEb);
     const uint32_t size =
-        ok ? (uint32_t)(min(lk - key, St::kRowsPerDma) - 1) * dma_rowb + D * Kv::kEb : 0u;
+        ok ? (uint32_t)(min(kseen - key, St::kRowsPerDma) - 1) * dma_rowb + D * Kv::kEb : 0u;
     const uint32_t lo = (uint32_t)base, hi = (uint32_t)(base >> 32);
     auto issue = [&](int u, uint32_t voff) {
       const int id = wave * St::kDmaPerWave + u;

@@ -209,7 +209,8 @@ def inkling_fa4_rel_attention_paged(q, k_cache, v_cache, rel_logits, cu_seqlens_
     lets it see every key.  A row with no visible key: out 0, lse -inf; rows of tokens that no
     sequence holds are not written.  max_seqlen_q and max_seqlen_k must bound the lengths.
     Keys and values that one of a tile's queries (128 at most) sees and another does not must
-    be finite; what lies past the last key, or left of every query's window, may be anything.
+    be finite; what lies past the last key that a tile's queries see, or left of every one's
+    window, may be anything.
     The bias joins the products as bias / (softmax_scale * k_scale) in fp32: a value so far below
     zero that the quotient overflows hides its key, as -inf does.
     """
