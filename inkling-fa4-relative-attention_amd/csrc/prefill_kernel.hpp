@@ -451,14 +451,16 @@ __device__ __forceinline__ void prefill_work(const PrefillParams& p, const WorkI
   // that chunk; its bytes are swizzled when they are converted).
   const int dma_row = lane / St::kDmaChunks;
   const int dma_slot = lane % St::kDmaChunks;
-#if IFA4_DMA2
-  // Each wave DMAs rows of one tensor (K for the first half of the waves, V for
+  // IFA4_DMA2 (a paged cache always, a DMA's resource being its block's):
+  // each wave DMAs rows of one tensor (K for the first half of the waves, V for
   // the second).  A lane's offset within a DMA is relative to the tile's first
   // row: one register per DMA of the wave (its tile row's offset and swizzled
   // chunk), set once.  The tile's start goes into the base of a resource built
   // per tile (scalar arithmetic), whose size ends with the sequence's last row,
   // so rows of a partial last tile past the sequence end read as zero.
-  static_assert(St::kDmaPerWave <= St::kDmaPerTensor && St::kDmaPerTensor % St::kDmaPerWave == 0,
+  constexpr bool kDma2 = IFA4_DMA2 || kPaged;
+  static_assert(!kDma2 || (St::kDmaPerWave <= St::kDmaPerTensor &&
+                           St::kDmaPerTensor % St::kDmaPerWave == 0),
                 "a wave's DMAs stay within one tensor");
   const bool dma_v = wave * St::kDmaPerWave >= St::kDmaPerTensor;
   const uint32_t dma_rowb = dma_v ? v_row : k_row;
@@ -556,18 +558,8 @@ __device__ __forceinline__ void prefill_work(const PrefillParams& p, const WorkI
       dma_16_tile(r, dma_voff[u], dst);
     }
   };
-  // (paged: and the table entries of the tile after it)
-  auto dma_tile = [&](int kt, uint16_t* stage) {
-    if constexpr (kPaged) {
-      dma_paged(kt, stage);
-      load_entry(kt + 1);
-    } else {
-      dma_rows(kt, stage);
-    }
-  };
-#else
-  static_assert(!kPaged, "a paged cache takes a DMA's resource per block");
-  auto dma_tile = [&](int kt, uint16_t* stage) {
+  // without IFA4_DMA2: a wave's DMAs may be of either tensor, their offsets vector sums
+  auto dma_either = [&](int kt, uint16_t* stage) {
     const int kb = kt * kBlockK;
 #pragma unroll
     for (int u = 0; u < St::kDmaPerWave; ++u) {
@@ -581,7 +573,17 @@ __device__ __forceinline__ void prefill_work(const PrefillParams& p, const WorkI
       dma_16(is_v ? rv : rk, off, dst);
     }
   };
-#endif
+  // (paged: and the table entries of the tile after it)
+  auto dma_tile = [&](int kt, uint16_t* stage) {
+    if constexpr (kPaged) {
+      dma_paged(kt, stage);
+      load_entry(kt + 1);
+    } else if constexpr (kDma2) {
+      dma_rows(kt, stage);
+    } else {
+      dma_either(kt, stage);
+    }
+  };
 
   // Bias resource: the (sequence, head) rows of the bias (with kProj: of r,
   // 16 values per row); each lane reads its rows.
