@@ -20,6 +20,7 @@
 
 namespace {
 
+using ifa4_torch::check_no_tangent;
 using ifa4_torch::check_status;
 using ifa4_torch::dtype_code;
 using ifa4_torch::empty_on;
@@ -319,6 +320,7 @@ std::tuple<at::Tensor, at::Tensor> fwd_paged(
     const at::Tensor& block_table, int64_t max_q, int64_t max_k, int64_t rel_extent, bool causal,
     int64_t window_left, double softmax_scale, bool return_lse, double k_scale, double v_scale) {
   constexpr const char* op = "fwd_paged";
+  check_no_tangent(op, q, k_cache, v_cache, rel);
   ifa4_paged_kv kv;
   ifa4_args a = paged_args(op, q, k_cache, v_cache, rel, cu_q, seqused_k, block_table, max_q, max_k,
                            rel_extent, causal, window_left, softmax_scale, IFA4_FLAG_BOTTOM_RIGHT,
@@ -345,6 +347,7 @@ std::tuple<at::Tensor, at::Tensor> sparse_paged(
     int64_t rel_extent, int64_t window_left, double softmax_scale, bool return_lse, double k_scale,
     double v_scale) {
   constexpr const char* op = "sparse_paged";
+  check_no_tangent(op, q, k_cache, v_cache, rel);
   ifa4_paged_kv kv;
   ifa4_args a = paged_args(op, q, k_cache, v_cache, rel, cu_q, seqused_k, block_table, max_q, max_k,
                            rel_extent, true, window_left, softmax_scale, IFA4_FLAG_BOTTOM_RIGHT, &kv);

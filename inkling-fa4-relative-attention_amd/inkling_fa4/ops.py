@@ -213,6 +213,8 @@ def inkling_fa4_rel_attention_paged(q, k_cache, v_cache, rel_logits, cu_seqlens_
     window, may be anything.
     The bias joins the products as bias / (softmax_scale * k_scale) in fp32: a value so far below
     zero that the quotient overflows hides its key, as -inf does.
+
+    There is no gradient: the result never requires one, and tangents are refused.
     """
     if k_cache.dim() != 4:
         raise ValueError("k_cache must be [num_blocks, block_size, kv_heads, head_dim]")

@@ -67,7 +67,8 @@ def inkling_fa4_rel_attention_sparse_paged(q, k_cache, v_cache, rel_logits, cu_s
     holds are not written.  What a token does not see may hold anything, infinities and NaN too.
 
     The bias and the window go by the keys' positions in the sequence, listed or not.  GQA groups
-    up to 16; caches, types and the other arguments as in inkling_fa4_rel_attention_paged.
+    up to 16; caches, types and the other arguments as in inkling_fa4_rel_attention_paged; no
+    gradient either.
     """
     if k_cache.dim() != 4:
         raise ValueError("k_cache must be [num_blocks, block_size, kv_heads, head_dim]")
