@@ -228,20 +228,22 @@ __device__ __forceinline__ void dma_16(rsrc_t r, uint32_t byte_off, const void* 
 // instruction the compiler schedules between two DMAs can expose one.
 // IFA4_DMA_COVER_EACH=0 (a sweep knob) restores the earlier form, one s_nop 4
 // per batch issued by the caller and s_nop 0 here, which is only safe while no
-// VALU writes those SGPRs inside the batch.
+// VALU writes those SGPRs inside the batch: kCover asks for the cover whatever
+// the knob, for a caller that builds a resource per DMA.
 #ifndef IFA4_DMA_COVER_EACH
 #define IFA4_DMA_COVER_EACH 1
 #endif
+template <bool kCover = (IFA4_DMA_COVER_EACH != 0)>
 __device__ __forceinline__ void dma_16_tile(rsrc_t r, uint32_t lane_off, uint32_t lds_addr) {
-#if IFA4_DMA_COVER_EACH
-  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(lane_off), "s"(r),
-               "{m0}"(lds_addr)
-               : "memory");
-#else
-  asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(lane_off), "s"(r),
-               "{m0}"(lds_addr)
-               : "memory");
-#endif
+  if constexpr (kCover) {
+    asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(lane_off), "s"(r),
+                 "{m0}"(lds_addr)
+                 : "memory");
+  } else {
+    asm volatile("s_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(lane_off), "s"(r),
+                 "{m0}"(lds_addr)
+                 : "memory");
+  }
 }
 __device__ __forceinline__ void hazard_nop5() { asm volatile("s_nop 4" ::: "memory"); }
 

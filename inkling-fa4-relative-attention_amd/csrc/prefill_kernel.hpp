@@ -513,7 +513,8 @@ __device__ __forceinline__ void prefill_work(const PrefillParams& p, const WorkI
                          (uint32_t)__builtin_amdgcn_readlane((int)lo, u);
       const rsrc_t r = make_rsrc(reinterpret_cast<const void*>(b),
                                  (uint32_t)__builtin_amdgcn_readlane((int)size, u));
-      dma_16_tile(r, voff, stage_lds + (uint32_t)((dma_v ? St::kTileBytes : 0) + blk * 1024));
+      // (v_readlane has just written r: covered whatever IFA4_DMA_COVER_EACH says)
+      dma_16_tile<true>(r, voff, stage_lds + (uint32_t)((dma_v ? St::kTileBytes : 0) + blk * 1024));
     };
     if (kb < kzero) {
 #pragma unroll

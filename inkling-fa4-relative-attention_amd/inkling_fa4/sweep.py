@@ -47,7 +47,8 @@ Knobs (macros of the kernel sources):
                    IFA4_MERGE_BATCH           split-KV merge pass: chunks whose loads are in
                                               flight together (2/4/8)
   ifa4_device.hpp  IFA4_DMA_COVER_EACH        hazard cover on every LDS DMA (1) or one per
-                                              batch of a tile's DMAs (0)
+                                              batch of a tile's DMAs (0; a paged cache's DMAs
+                                              keep theirs)
   decode_fwd.hip   IFA4_DECODE_WPE            waves per SIMD the stream pass's registers target
                    IFA4_COMBINE_SPLIT         combine of many-part segments over 2 or 4
                                               workgroups per (head, sequence) (0/1)
