@@ -14,6 +14,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <tuple>
 
 #include "torch_util.h"
@@ -56,6 +57,9 @@ ifa4_args make_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& 
               "inkling_fa4: cu_seqlens_q/k must be 1-D of equal length batch+1");
   TORCH_CHECK(cu_q.is_contiguous() && cu_k.is_contiguous(),
               "inkling_fa4: cu_seqlens must be contiguous");
+  TORCH_CHECK(std::max({max_q, max_k, rel_extent}) <= INT32_MAX &&
+                  std::min({max_q, max_k, rel_extent}) >= 0,
+              "inkling_fa4: max_seqlen_q, max_seqlen_k or rel_extent out of range");
   const int32_t qd = dtype_code(q.scalar_type());
   const int32_t rd = dtype_code(rel.scalar_type());
   TORCH_CHECK(qd == IFA4_BF16 || qd == IFA4_FP16, "inkling_fa4: q/k/v must be bf16 or fp16");
@@ -88,7 +92,8 @@ ifa4_args make_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& 
   a.rel_width = static_cast<int32_t>(rel.size(2));
   a.max_seqlen_q = static_cast<int32_t>(max_q);
   a.max_seqlen_k = static_cast<int32_t>(max_k);
-  a.window_left = window_left < 0 ? -1 : static_cast<int32_t>(window_left);
+  // (a window past every position is as good as none)
+  a.window_left = window_left < 0 ? -1 : static_cast<int32_t>(std::min<int64_t>(window_left, INT32_MAX));
   a.causal = causal ? 1 : 0;
   a.softmax_scale = static_cast<float>(softmax_scale);
   a.qkv_dtype = qd;
