@@ -489,7 +489,7 @@ int32_t ifa4_kv_append_paged(const ifa4_norm_rope* args, const ifa4_kv_append* a
  * key is NaN):
  *   bounds[blk, h, 0, d] = min over rows, bounds[blk, h, 1, d] = max.
  * Other blocks' bounds stay as they are, and so do those behind table entries outside the pool.
- * Two sequences that hold one block at unequal lengths leave the bounds of one of them.
+ * Where two sequences hold one block at unequal lengths, each bound is that of either.
  * max_seqlen_q must bound n.  Of kv the fields v_stride_block is not read.  The reference has
  * no kernel for it.
  */
@@ -515,14 +515,19 @@ int32_t ifa4_key_bounds_paged(const ifa4_key_bounds* args, const ifa4_paged_kv* 
  * more than n_select of them it reads all; else the first sink_blocks, the last recent_blocks
  * and the best of those between by
  *   score(blk) = sum over the kv head's query heads g and d of max(q_gd lo_d, q_gd hi_d),
- * summed in 64 bits, in an order that sizes choose (scores closer than such a sum's rounding may
- * rank either way; equal bounds score equal, and equal scores go to the lower block).  A score of
+ * which bounds the sum over the group of the products with any key of the block (the bias has no
+ * part in it), summed in 64 bits, in an order that sizes choose (scores closer than such a sum's
+ * rounding may rank either way; equal bounds score equal, and equal scores go to the lower block).  A score of
  * NaN counts as infinity, and so does a block with a bound that is infinite or NaN; a table entry
  * outside the pool has bounds of zero.  blocks [total_q, kv_heads, n_select] (contiguous) gets the block
  * indexes ascending, then -1; a token of no sequence gets -1 throughout.  n_select >=
  * sink_blocks + recent_blocks, recent_blocks >= 1.  max_seqlen_q and max_seqlen_k must bound the
  * lengths.  The workspace (256-byte aligned, contents on entry irrelevant) is scratch for one
- * call.  Of kv the fields k_stride_block and v_stride_block are not read.  The reference has no
+ * call: a score of 8 bytes for each token, kv head and block of max_seqlen_k (total_q * kv_heads *
+ * ceil(max_seqlen_k / block_size) * 8 bytes, rounded up to 256; 0 where max_seqlen_k has no more
+ * than n_select blocks): long chunks over long caches are better taken in parts.
+ * Sequences of few tokens (three at most) are scored faster in a call of their own than beside a
+ * longer chunk.  Of kv the fields k_stride_block and v_stride_block are not read.  The reference has no
  * kernel for it.
  */
 typedef struct ifa4_block_select {

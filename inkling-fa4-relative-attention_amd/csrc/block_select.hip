@@ -297,8 +297,8 @@ __global__ __launch_bounds__(64 * kScoreWaves) void score_step_kernel(SelectPara
   constexpr int kChunks = 2 * kHalf / 8;     // of a lane
   const int lane = threadIdx.x & 63, wave = (int)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int seq = blockIdx.y;
-  // kv heads side by side: their bounds of a block are neighbours in memory (64 sequences over 2000
-  // blocks, a call: 31.1 -> 30.2 us)
+  // kv heads side by side: their bounds of a block are neighbours in memory (64 sequences over
+  // 2000..32700 keys in blocks of 16, a call: 29.2 -> 27.0 us; over 32000 each 38.9 -> 38.7)
   const int h = blockIdx.x % p.kv_heads, rest = blockIdx.x / p.kv_heads;
   const int part0 = rest % p.score_parts, i0 = rest / p.score_parts;
   const TokenSpan s = token_span(p, seq);
@@ -636,8 +636,10 @@ hipError_t launch_select_t(const SelectParams& p_in, hipStream_t stream) {
                          dim3(64 * kScoreWaves), 0, stream, p);
     } else {
       const int tiles = (p.cols + 15) / 16, q_tiles = (p.max_q + 15) / 16;
-      // workgroups for every tile of blocks, or two rounds of them where there are many tokens:
-      // each begins with the sums over its query heads
+      // workgroups for every tile of blocks, or kScoreGroups of them where there are many tokens:
+      // each begins with the sums over its query heads.  (Counted by the longest sequence: beside
+      // one chunk, single tokens get a workgroup each.  512 tokens over 30000 keys and 63 single
+      // ones over 2K..32K 390 us in one call, 44 and 27 in two.)
       const int per = (tiles + kScoreWaves - 1) / kScoreWaves;
       const int64_t others = (int64_t)q_tiles * p.kv_heads * p.batch;
       p.score_parts = (int)max(int64_t(1), min((int64_t)per, kScoreGroups / max(int64_t(1), others)));

@@ -275,8 +275,9 @@ struct SparseParams {
 constexpr int kSparseStep = 32;
 // Waves that share a list of `rows` rows, for `items` (token, kv head) pairs: enough of them in all
 // to fill the chip, each with two steps at least; up to 8 in a workgroup, the rest as workgroups
-// whose partials a second pass joins.  Kernel us with 2048 / 4096 waves: 64 sequences x 128 blocks of
-// 16 28.6 / 32.1, 512 tokens x 100 blocks of e4m3 40.5 / 39.5, 4 sequences x 16 blocks of 64 9.0 / 8.2.
+// whose partials a second pass joins.  A call in us with 2048 / 4096 waves: 64 sequences x 128 blocks
+// of 16 30.4 / 34.1, of e4m3 21.1 / 23.6, 512 tokens x 128 blocks 55.1 / 57.6, x 100 blocks of e4m3
+// 38.8 / 37.7, 4 sequences x 16 blocks of 64 9.9 / 9.8.
 constexpr int kSparseWaves = 2048;
 // A workgroup takes in about 53 KB a us, the second pass takes 3.5 us: shares pay where they take more
 // than this many bytes of K and V off a workgroup.  A call in us, one workgroup a list / shares:

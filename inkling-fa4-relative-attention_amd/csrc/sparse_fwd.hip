@@ -355,6 +355,9 @@ sparse_fwd_kernel(SparseParams p) {
       pv[e] = fast_exp2(fmaf(acc[e >> 2][e & 3], c2, -m_use));
       l_run += pv[e];
     }
+    // The second product takes the weights in q's type, as in the framework's other attentions (its
+    // 16-bit matrix instructions; half a step of each weight, about as much as the output's own
+    // rounding); their sum is that of the fp32 ones.
     const u32x4_t pb = {E::pack2(pv[0], pv[1]), E::pack2(pv[2], pv[3]), E::pack2(pv[4], pv[5]),
                         E::pack2(pv[6], pv[7])};
 #pragma unroll

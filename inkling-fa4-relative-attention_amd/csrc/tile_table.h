@@ -442,14 +442,17 @@ inline PrefillSplit prefill_split_for(int64_t batch, int64_t n_heads, int64_t ma
 }
 
 // Prefill over a paged cache, whose lengths only the device knows: a batch of unequal query counts
-// (total_q against batch * max_q) has unequal caches too, and its grid, planned by the longest, looks
-// full where it is not.  A call that the plan above leaves whole, with up to 1.5 resident rounds of
-// live workgroups over ranges of 96 tiles and more, is cut into chunks of two fifths of the
-// longest range (without, chunks of 0.3 / 0.4 / 0.5 of it; one box, us, Hq 8 / Hkv 2, d 128, bias of
-// extent 1024): 16 x 3..500 queries over 90..8000 keys 211 -> 181 / 152 / 160, 32 x the same 300 ->
-// 282 / 289 / 277, 8 x 10..1000 over 90..20K 452 -> 257 / 238 / -, 20 x 1..600 over 2K..30K 887 ->
-// 700 at 0.25; shorter ranges lose (40 x 1..400 over 90..3000, 53 tiles, 145 -> 152, 10 x 1..2000 over
-// 1..2000 131 -> 135), and so do equal query counts (8 x 512 over 4K 107 -> 117).
+// (total_q against batch * max_q) mostly has unequal caches too, and its grid, planned by the longest,
+// looks full where it is not.  A call that the plan above leaves whole, with up to 1.5 resident rounds
+// of live workgroups over ranges of 96 tiles and more, is cut into chunks of two fifths of the
+// longest range (without / with; one box, us a call, Hq 8 / Hkv 2, d 128, bias of extent 1024): 16 x
+// 3..500 queries over 90..8000 keys 210 / 160, e4m3 248 / 167, over 8000 each 248 / 230, 32 x the same
+// over 90..8000 290 / 256, 8 x 10..1000 over 90..20K 450 / 232, 20 x 1..600 over 2K..30K 878 / 773.
+// Other fractions, when this one was chosen: 0.3 / 0.4 / 0.5 181 / 152 / 160 on the first, 282 / 289 /
+// 277 on the 32, 257 / 238 / - on the 8, 700 at 0.25 on the 20.  Shorter ranges lose (40 x 1..400 over
+// 90..3000, 53 tiles, 145 / 152, 10 x 1..2000 over 1..2000 131 / 135), and so do equal query counts (8 x
+// 512 over 4K 107 / 117): max_q being a bound, equal counts well below it are taken for unequal ones
+// (16 x 512 over 16K 527 under max_q 512, not cut; 542 / 628 under 1024).
 inline PrefillSplit paged_ragged_split(int64_t batch, int64_t n_heads, int64_t total_q, int64_t max_q,
                                        int64_t max_k, int64_t window_left, int32_t block_q,
                                        int32_t block_k) {

@@ -23,7 +23,7 @@ def inkling_fa4_key_bounds_paged(k_cache, bounds, cu_seqlens_q, seqused_k, block
     in place, bounds[block, h, 0] the minimum over the block's keys below seqused_k, [.., 1] the
     maximum (exact; NaN where a key is NaN).  Other blocks keep theirs.  The blocks are read
     whole, so a block given to another sequence needs nothing but this call after its append.
-    Two sequences that share a block they fill to unequal lengths leave the bounds of one.
+    Where two sequences share a block they fill to unequal lengths, each bound is that of either.
 
     max_seqlen_q must bound the new tokens of a sequence.  There is no derivative: tangents are
     refused, and so are bounds that require a gradient (outside torch.no_grad()).
@@ -42,12 +42,19 @@ def inkling_fa4_select_blocks_paged(q, bounds, cu_seqlens_q, seqused_k, block_ta
     0 .. p // block_size.  Where they are more than n_select, it reads the first sink_blocks,
     the last recent_blocks (at least one, its own), and the best of the others by
         score = sum over the kv head's query heads g and d of max(q_gd lo_d, q_gd hi_d),
-    an upper bound of what any key of the block can reach, from q [total_q, Hq, D] (bf16, fp16)
-    and bounds as inkling_fa4_key_bounds_paged leaves them (of q's dtype or float8_e4m3fn).
+    an upper bound of the sum over those heads of q . k for any key of the block (the relative
+    bias has no part in it: recent_blocks covers what it favours), from q [total_q, Hq, D] (bf16,
+    fp16) and bounds as inkling_fa4_key_bounds_paged leaves them (of q's dtype or float8_e4m3fn).
     Scores are summed in 64 bits: only those closer than such a sum's rounding may rank either
     way from one batch to another; equal bounds score equal, and equal scores go to the lower
     block.  A score of NaN counts as infinity, and so does a block with an infinite or NaN bound.
     max_seqlen_q and max_seqlen_k must bound the lengths.
+
+    Where max_seqlen_k has more than n_select blocks, the call holds a score of 8 bytes for every
+    token, kv head and block of max_seqlen_k: 8 * total_q * Hkv * ceil(max_seqlen_k / block_size)
+    bytes from torch's allocator (512 MiB for 4096 tokens, 2 heads and 128K keys in blocks of 16).
+    Take long chunks over long caches in parts, and give a tight max_seqlen_k.  A step that mixes a
+    chunk with single tokens is faster as two calls, one for each kind.
     """
     return _call("select_blocks_paged", q, bounds, cu_seqlens_q, seqused_k, block_table,
                  int(block_size), int(max_seqlen_q), int(max_seqlen_k), int(n_select),

@@ -36,8 +36,8 @@ Knobs (macros of the kernel sources):
                    IFA4_SCHED                 scheduling groups (0/1)
                    IFA4_PV2                   key-block-major PV (0/1)
                    IFA4_BIAS_LDS              shared bias table in LDS (0/1)
-                   IFA4_PREFILL_NQB           32-row blocks per wave (1/2)
-                   IFA4_BLOCK_K               keys per KV tile (32/64)
+                   IFA4_PREFILL_NQB           32-row blocks per wave (1; packed rows do not take 2)
+                   IFA4_BLOCK_K               keys per KV tile (64, as the projection's)
                    IFA4_WPE                   waves per SIMD the register budget targets
                    IFA4_PREFILL_WAVES         waves per workgroup (4: 128 query rows, 8: 256)
                    IFA4_PROJ_SKIP             fused projection: skip distance blocks outside
